@@ -38,8 +38,9 @@ enum nova_status {
 NOVA_API const char* nova_version(void);
 /* sizeof of the argument structs, in this order: nova_attn_int8_args,
  * nova_nf4_args, nova_qk_args, nova_prefill_attn_args, nova_qk_prefill_args,
- * nova_sample_args, nova_tp_allreduce_args (n entries at most are written;
- * returns how many there are).  Lets a binding check its struct mirrors. */
+ * nova_sample_args, nova_tp_allreduce_args, nova_paged_plan_args,
+ * nova_paged_plan_info, nova_paged_append_args, nova_paged_attn_args (n
+ * entries at most are written; returns how many there are).  Lets a binding check its struct mirrors. */
 NOVA_API int nova_abi_sizes(int64_t* out, int n);
 NOVA_API const char* nova_last_error(void);
 
@@ -558,6 +559,137 @@ typedef struct nova_sample_args {
 } nova_sample_args;
 
 NOVA_API int nova_sample_topk(const nova_sample_args* args, void* stream);
+
+/* ------------------------------------------- batches of independent requests */
+
+/*
+ * Paged int8 cache of many requests, each with a length of its own.  A page
+ * holds 64 consecutive tokens of one request in the int8t64 form of
+ * nova_kv_quant_int8 (one group: asymmetric codes per channel over the page's
+ * tokens); the tokens of the page that is not yet full stay in fp16 in a tail
+ * buffer, as the ring of nova_kv_append_int8 keeps them.  Per layer:
+ *   codes  uint8 [num_pages, kv_heads, 2, 64, 128]   (K, V)
+ *   scales fp16  [num_pages, kv_heads, 4, 128]       (K min, K step, V min, V step)
+ *   tails  fp16  [num_tails, kv_heads, 2, 64, 128]   (K, V; position p at slot p % 64)
+ * all contiguous, 16-byte aligned.  A stored value is fp16(code * step + min).
+ * Pages are scattered: request i's page j is pages[page_off[i] + j], the same
+ * number in every layer.  The reference's caches have one length for all rows
+ * (src/nova/kvattn.py:488-660); these calls have no counterpart there.
+ */
+
+#define NOVA_PAGED_MAX_WINDOWS 4
+
+/* One step of such a batch, in host memory: request i brings q_lens[i] >= 0
+ * new tokens, its cache holds kv_lens[i] >= q_lens[i] tokens with them.  Its
+ * token rows (q|k|v, q, out) follow those of request i - 1.  tail_in: the tail
+ * buffer of its open page before the step; tail_out: after it (the same one
+ * when the open page stays the same page; another one otherwise, so that a
+ * step can be run again).  read_from: the first position that nova_paged_read
+ * copies (NULL: the start of the first page that the new tokens touch). */
+typedef struct nova_paged_plan_args {
+    int64_t seqs, q_heads, kv_heads, sms;
+    const int64_t* q_lens;
+    const int64_t* kv_lens;
+    const int64_t* page_off;  /* [seqs + 1]                                     */
+    const int64_t* pages;
+    const int64_t* tail_in;
+    const int64_t* tail_out;
+    const int64_t* read_from;
+    int64_t n_windows;        /* attention windows that the layers use (0: none) */
+    int64_t windows[NOVA_PAGED_MAX_WINDOWS];
+} nova_paged_plan_args;
+
+typedef struct nova_paged_schedule {
+    int64_t window;
+    int64_t rows_off, n_rows, rows_per_tile;   /* work items of few query rows   */
+    int64_t n_parts;                           /* partial results of split items */
+} nova_paged_schedule;
+
+/* What a plan holds and where (offsets in int32 from the plan's start). */
+typedef struct nova_paged_plan_info {
+    int64_t ints;             /* length of the plan                              */
+    int64_t workspace_bytes;  /* nova_paged_attention's workspace, zeroed once   */
+    int64_t seqs, tokens, read_rows, q_heads, kv_heads;
+    int64_t max_page, max_tail;                /* largest page / tail number used */
+    int64_t max_pos;          /* largest position of a new token, -1: none       */
+    int64_t seq_off, page_off, pos_off;
+    int64_t write_off, n_write, read_off, n_read;
+    int64_t n_windows;
+    nova_paged_schedule sched[NOVA_PAGED_MAX_WINDOWS];
+} nova_paged_plan_info;
+
+/* Builds the plan of a step on the host: `out` (int32 [capacity]) is what the
+ * calls below read on the device, copied there by the caller.  With out ==
+ * NULL or too small a capacity only `info` is filled (ints = what is needed)
+ * and NOVA_OK returned; the caller compares.  No GPU is used. */
+NOVA_API int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, int64_t capacity,
+                             nova_paged_plan_info* info);
+
+/*
+ * q|k|v rows of the step's new tokens (fp16 [tokens, (q_heads + 2 kv_heads) *
+ * 128]) -> q [tokens, q_heads, 128] with q_norm and RoPE, and K (k_norm, RoPE)
+ * and V into the cache: pages that fill are quantized from their 64 tokens
+ * (the open page's, taken from tail_in, and the new ones), the rest goes to
+ * tail_out.  Norms and rotation in fp32, rounded once to fp16 (the fused
+ * decode step keeps the reference's intermediate fp16 roundings).  NULL norm
+ * weights: no norm; NULL cos / sin (fp16 [rope_len, 128]): no rotation.
+ */
+typedef struct nova_paged_append_args {
+    const void* qkv;
+    int64_t qkv_stride;
+    const void* q_norm_weight;
+    const void* k_norm_weight;
+    double eps;
+    const void* cos;
+    const void* sin;
+    int64_t rope_len;
+    void* q_out;
+    int64_t q_t_stride;       /* elements between tokens; heads are contiguous   */
+    void* codes;
+    void* scales;
+    void* tails;
+    int64_t num_pages, num_tails;
+    const int32_t* plan;      /* device                                          */
+} nova_paged_append_args;
+
+NOVA_API int nova_paged_append(const nova_paged_append_args* args, const nova_paged_plan_info* info, void* stream);
+
+/* The stored values of positions [read_from, kv_len) of every request as fp16
+ * rows k_out, v_out [read_rows, kv_heads, 128], requests one after another. */
+NOVA_API int nova_paged_read(const void* codes, const void* scales, const void* tails, int64_t num_pages,
+                             int64_t num_tails, const int32_t* plan, const nova_paged_plan_info* info, void* k_out,
+                             void* v_out, void* stream);
+
+/*
+ * Attention of the step's new tokens over the paged cache (after the append):
+ * the query at position p of a request sees its keys j <= p, and j > p -
+ * window where window > 0.  q fp16 [tokens, q_heads, 128], out fp16 [tokens,
+ * q_heads, 128] (element strides; the last dimension contiguous), lse
+ * (optional) fp32 [tokens, q_heads] contiguous.  sched: which of the plan's
+ * windows.  q_heads a multiple of kv_heads.
+ */
+typedef struct nova_paged_attn_args {
+    const void* q;
+    int64_t q_t_stride, q_h_stride;
+    const void* codes;
+    const void* scales;
+    const void* tails;
+    int64_t num_pages, num_tails;
+    void* out;
+    int64_t o_t_stride, o_h_stride;
+    void* lse;
+    double scale;             /* of the scores, > 0                              */
+    const int32_t* plan;      /* device                                          */
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t sched;
+} nova_paged_attn_args;
+
+NOVA_API int nova_paged_attention(const nova_paged_attn_args* args, const nova_paged_plan_info* info, void* stream);
+
+/* Error word of a nova_paged_attention workspace (non-zero: a bounded wait
+ * gave up and that launch's output is not valid), copied and cleared. */
+NOVA_API int nova_paged_attention_read_error(void* workspace, int* host_value);
 
 /* --------------------------------------------------- tensor parallelism */
 

@@ -17,6 +17,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libnova_b200.so")
 NOVA_OK, NOVA_ERR_INVALID, NOVA_ERR_ALIGN, NOVA_ERR_UNSUPPORTED, NOVA_ERR_CUDA = range(5)
 NF4_PLAIN, NF4_RESIDUAL, NF4_SILU_MUL, NF4_ARGMAX, NF4_F32, NF4_SLOTS = range(6)
 NOVA_ATTN_NOALLOC_SCRATCH_BYTES = 4 << 20   # built-in scratch of nova_attn_decode_int8_noalloc
+PAGED_MAX_WINDOWS = 4   # attention windows that one plan may hold
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int64
@@ -114,6 +115,53 @@ class TPAllReduceArgs(ctypes.Structure):
     ]
 
 
+class PagedPlanArgs(ctypes.Structure):
+    """Mirror of ``nova_paged_plan_args``."""
+
+    _fields_ = [
+        ("seqs", _I), ("q_heads", _I), ("kv_heads", _I), ("sms", _I),
+        ("q_lens", _P), ("kv_lens", _P), ("page_off", _P), ("pages", _P), ("tail_in", _P), ("tail_out", _P),
+        ("read_from", _P), ("n_windows", _I), ("windows", _I * PAGED_MAX_WINDOWS),
+    ]
+
+
+class PagedSchedule(ctypes.Structure):
+    """Mirror of ``nova_paged_schedule``."""
+
+    _fields_ = [("window", _I), ("rows_off", _I), ("n_rows", _I), ("rows_per_tile", _I), ("n_parts", _I)]
+
+
+class PagedPlanInfo(ctypes.Structure):
+    """Mirror of ``nova_paged_plan_info``."""
+
+    _fields_ = [
+        ("ints", _I), ("workspace_bytes", _I), ("seqs", _I), ("tokens", _I), ("read_rows", _I), ("q_heads", _I),
+        ("kv_heads", _I), ("max_page", _I), ("max_tail", _I), ("max_pos", _I), ("seq_off", _I), ("page_off", _I),
+        ("pos_off", _I), ("write_off", _I), ("n_write", _I), ("read_off", _I), ("n_read", _I), ("n_windows", _I),
+        ("sched", PagedSchedule * PAGED_MAX_WINDOWS),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """Mirror of ``nova_paged_append_args``."""
+
+    _fields_ = [
+        ("qkv", _P), ("qkv_stride", _I), ("q_norm_weight", _P), ("k_norm_weight", _P), ("eps", ctypes.c_double),
+        ("cos", _P), ("sin", _P), ("rope_len", _I), ("q_out", _P), ("q_t_stride", _I),
+        ("codes", _P), ("scales", _P), ("tails", _P), ("num_pages", _I), ("num_tails", _I), ("plan", _P),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """Mirror of ``nova_paged_attn_args``."""
+
+    _fields_ = [
+        ("q", _P), ("q_t_stride", _I), ("q_h_stride", _I), ("codes", _P), ("scales", _P), ("tails", _P),
+        ("num_pages", _I), ("num_tails", _I), ("out", _P), ("o_t_stride", _I), ("o_h_stride", _I), ("lse", _P),
+        ("scale", ctypes.c_double), ("plan", _P), ("workspace", _P), ("workspace_bytes", _I), ("sched", _I),
+    ]
+
+
 # name -> argtypes (every entry point returns int status unless noted)
 _SIGNATURES: dict[str, list] = {
     "nova_abi_sizes": [_P, _i],
@@ -150,10 +198,16 @@ _SIGNATURES: dict[str, list] = {
     "nova_sample_topk": [ctypes.POINTER(SampleArgs), _P],
     "nova_attn_prefill_int8": [ctypes.POINTER(PrefillAttnArgs), _P],
     "nova_qk_prefill": [ctypes.POINTER(QKPrefillArgs), _P],
+    "nova_paged_plan": [ctypes.POINTER(PagedPlanArgs), _P, _I, ctypes.POINTER(PagedPlanInfo)],
+    "nova_paged_append": [ctypes.POINTER(PagedAppendArgs), ctypes.POINTER(PagedPlanInfo), _P],
+    "nova_paged_read": [_P, _P, _P, _I, _I, _P, ctypes.POINTER(PagedPlanInfo), _P, _P, _P],
+    "nova_paged_attention": [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(PagedPlanInfo), _P],
+    "nova_paged_attention_read_error": [_P, ctypes.POINTER(_i)],
 }
 _STRING_FNS = ("nova_version", "nova_last_error")
 _INT_FNS = ("nova_get_launch_flags",)
-ABI_STRUCTS = ("AttnArgs", "NF4Args", "QKArgs", "PrefillAttnArgs", "QKPrefillArgs", "SampleArgs", "TPAllReduceArgs")
+ABI_STRUCTS = ("AttnArgs", "NF4Args", "QKArgs", "PrefillAttnArgs", "QKPrefillArgs", "SampleArgs", "TPAllReduceArgs",
+               "PagedPlanArgs", "PagedPlanInfo", "PagedAppendArgs", "PagedAttnArgs")
 
 _lib: ctypes.CDLL | None = None
 

@@ -91,7 +91,9 @@ extern "C" int nova_abi_sizes(int64_t* out, int n) {
     const int64_t sizes[] = {int64_t(sizeof(nova_attn_int8_args)),    int64_t(sizeof(nova_nf4_args)),
                              int64_t(sizeof(nova_qk_args)),           int64_t(sizeof(nova_prefill_attn_args)),
                              int64_t(sizeof(nova_qk_prefill_args)),   int64_t(sizeof(nova_sample_args)),
-                             int64_t(sizeof(nova_tp_allreduce_args))};
+                             int64_t(sizeof(nova_tp_allreduce_args)), int64_t(sizeof(nova_paged_plan_args)),
+                             int64_t(sizeof(nova_paged_plan_info)),   int64_t(sizeof(nova_paged_append_args)),
+                             int64_t(sizeof(nova_paged_attn_args))};
     const int count = int(sizeof(sizes) / sizeof(sizes[0]));
     for (int i = 0; i < n && i < count && out; ++i) out[i] = sizes[i];
     return count;

@@ -1,0 +1,364 @@
+// Paged int8 cache: q|k|v rows of a step's new tokens into it (per-head norm,
+// RoPE, quantization of the pages that fill), and stored values back out.
+//
+// Both kernels move each byte once and compute little, so what bounds them is
+// HBM for prompts and the latency of a launch and two dependent loads for
+// single tokens.  One thread holds channels 4c..4c+3 and 64+4c..64+4c+3 of a
+// row (c = lane % 16): the two halves that RoPE combines are then in one
+// thread, a row is two 128-byte requests of a half warp, and the mean of
+// squares is four shuffles.
+#include "paged.cuh"
+
+namespace nova {
+namespace paged {
+
+constexpr int THREADS = 256;
+constexpr int PAIRS = 64;       // (token, query head) rows per CTA of the q part
+
+struct AppendParams {
+    const __half* qkv;
+    int64_t qkv_stride;
+    const __half* wq;
+    const __half* wk;
+    float eps;
+    const __half* cos;
+    const __half* sin;
+    __half* q;
+    int64_t q_stride;
+    uint8_t* codes;
+    __half* scales;
+    __half* tails;
+    const Seq* seqs;
+    const int* pages;
+    const int* pos;
+    const Block* blocks;
+    int64_t tokens;
+    int n_write, q_heads, kv_heads;
+    int q_ctas;
+};
+
+struct Row8 {                   // channels 4c..4c+3 and 64+4c..64+4c+3 of one row
+    uint2 lo, hi;
+};
+
+__device__ __forceinline__ Row8 load_row(const __half* p, int c) {
+    Row8 r;
+    r.lo = *reinterpret_cast<const uint2*>(p + 4 * c);
+    r.hi = *reinterpret_cast<const uint2*>(p + 64 + 4 * c);
+    return r;
+}
+__device__ __forceinline__ void store_row(__half* p, int c, const Row8& r) {
+    *reinterpret_cast<uint2*>(p + 4 * c) = r.lo;
+    *reinterpret_cast<uint2*>(p + 64 + 4 * c) = r.hi;
+}
+__device__ __forceinline__ void unpack(const Row8& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.lo.x, r.lo.y, r.hi.x, r.hi.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ Row8 pack(const float (&x)[8]) {
+    Row8 r;
+    r.lo = make_uint2(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]));
+    r.hi = make_uint2(pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+    return r;
+}
+
+// RMSNorm (w != NULL) and RoPE (cos != NULL) of one row held by a half warp,
+// in fp32 and rounded to fp16 once: the reference rounds after the norm, after
+// the weight and after each rotation product, which costs half a unit in the
+// last place each time and nothing here needs its bits.
+__device__ __forceinline__ Row8 norm_rope_row(const Row8& in, const __half* w, const __half* cos, const __half* sin,
+                                              int64_t pos, float eps, int c) {
+    float x[8];
+    unpack(in, x);
+    if (w) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        const float r = rsqrt_ieee(ss * (1.0f / D) + eps);
+        float g[8];
+        unpack(load_row(w, c), g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= r * g[i];
+    }
+    if (cos) {
+        float cs[8], sn[8], y[8];
+        unpack(load_row(cos + pos * D, c), cs);
+        unpack(load_row(sin + pos * D, c), sn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[i] = x[i] * cs[i] - x[i + 4] * sn[i];
+            y[i + 4] = x[i + 4] * cs[i + 4] + x[i] * sn[i + 4];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i];
+    }
+    return pack(x);
+}
+
+__device__ __forceinline__ uint32_t hmin2u(uint32_t a, uint32_t b) {
+    __half2 r = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
+    __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// CTAs [0, q_ctas): 64 (token, query head) rows each.  The others: K or V of
+// one (touched block, KV head).  A block that the step completes is held in
+// registers (4 tokens x 8 channels a thread), its minimum and maximum per
+// channel go through shared memory once, and codes leave as 4-byte pieces of
+// 128-byte rows; a block that stays open only gets its new rows.
+__global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendParams p) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 15, part = warp * 2 + (lane >> 4);
+    if (int(blockIdx.x) < p.q_ctas) {
+        const int64_t base = int64_t(blockIdx.x) * PAIRS, n = p.tokens * p.q_heads;
+        Row8 r[4];
+        int64_t tok[4];
+        int head[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = min(base + i * 16 + part, n - 1);   // a row past the end repeats the last one, unstored
+            tok[i] = at / p.q_heads;
+            head[i] = int(at - tok[i] * p.q_heads);
+            r[i] = load_row(p.qkv + tok[i] * p.qkv_stride + head[i] * D, c);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            r[i] = norm_rope_row(r[i], p.wq, p.cos, p.sin, p.cos ? p.pos[tok[i]] : 0, p.eps, c);
+            if (base + i * 16 + part < n) store_row(p.q + tok[i] * p.q_stride + head[i] * D, c, r[i]);
+        }
+        return;
+    }
+    const int item = (blockIdx.x - p.q_ctas) / (2 * p.kv_heads), hj = (blockIdx.x - p.q_ctas) % (2 * p.kv_heads);
+    const int head = hj >> 1, j = hj & 1;
+    const Block blk = p.blocks[item];
+    const Seq s = p.seqs[blk.seq];
+    const int first = s.kv_len - s.q_len, b0 = blk.blk * PT;
+    const bool closes = b0 + PT <= s.kv_len;
+    const __half* src = p.qkv + (p.q_heads + j * p.kv_heads + head) * int64_t(D);
+    const __half* old = p.tails + half_off(s.tail_in, p.kv_heads, head, j);
+    Row8 r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int slot = i * 16 + part, pos = b0 + slot;
+        r[i] = Row8{make_uint2(0u, 0u), make_uint2(0u, 0u)};
+        if (pos >= first && pos < s.kv_len) r[i] = load_row(src + int64_t(s.q_start + pos - first) * p.qkv_stride, c);
+        else if (closes) r[i] = load_row(old + slot * D, c);   // pos < first: the open page's token
+    }
+    if (j == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int pos = b0 + i * 16 + part;
+            const bool fresh = pos >= first && pos < s.kv_len;
+            const Row8 y = norm_rope_row(r[i], p.wk, p.cos, p.sin, fresh ? pos : first, p.eps, c);
+            if (fresh) r[i] = y;
+        }
+    }
+    if (!closes) {
+        __half* dst = p.tails + half_off(s.tail_out, p.kv_heads, head, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int slot = i * 16 + part, pos = b0 + slot;
+            if (pos >= first && pos < s.kv_len) store_row(dst + slot * D, c, r[i]);
+        }
+        return;
+    }
+    __shared__ __align__(8) uint32_t lims[8][2][D / 2];   // per warp: minima, maxima of each channel pair
+    uint32_t mn[4], mx[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t w[4] = {k < 2 ? (k ? r[0].lo.y : r[0].lo.x) : (k == 2 ? r[0].hi.x : r[0].hi.y),
+                               k < 2 ? (k ? r[1].lo.y : r[1].lo.x) : (k == 2 ? r[1].hi.x : r[1].hi.y),
+                               k < 2 ? (k ? r[2].lo.y : r[2].lo.x) : (k == 2 ? r[2].hi.x : r[2].hi.y),
+                               k < 2 ? (k ? r[3].lo.y : r[3].lo.x) : (k == 2 ? r[3].hi.x : r[3].hi.y)};
+        mn[k] = hmin2u(hmin2u(w[0], w[1]), hmin2u(w[2], w[3]));
+        mx[k] = hmax2u(hmax2u(w[0], w[1]), hmax2u(w[2], w[3]));
+        mn[k] = hmin2u(mn[k], __shfl_xor_sync(0xffffffffu, mn[k], 16));
+        mx[k] = hmax2u(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 16));
+    }
+    if (lane < 16) {
+        *reinterpret_cast<uint2*>(&lims[warp][0][2 * c]) = make_uint2(mn[0], mn[1]);
+        *reinterpret_cast<uint2*>(&lims[warp][0][32 + 2 * c]) = make_uint2(mn[2], mn[3]);
+        *reinterpret_cast<uint2*>(&lims[warp][1][2 * c]) = make_uint2(mx[0], mx[1]);
+        *reinterpret_cast<uint2*>(&lims[warp][1][32 + 2 * c]) = make_uint2(mx[2], mx[3]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        const uint2 a = *reinterpret_cast<const uint2*>(&lims[w][0][2 * c]);
+        const uint2 b = *reinterpret_cast<const uint2*>(&lims[w][0][32 + 2 * c]);
+        const uint2 d = *reinterpret_cast<const uint2*>(&lims[w][1][2 * c]);
+        const uint2 e = *reinterpret_cast<const uint2*>(&lims[w][1][32 + 2 * c]);
+        mn[0] = hmin2u(mn[0], a.x); mn[1] = hmin2u(mn[1], a.y); mn[2] = hmin2u(mn[2], b.x); mn[3] = hmin2u(mn[3], b.y);
+        mx[0] = hmax2u(mx[0], d.x); mx[1] = hmax2u(mx[1], d.y); mx[2] = hmax2u(mx[2], e.x); mx[3] = hmax2u(mx[3], e.y);
+    }
+    float low[8], step[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 a = __half22float2(*reinterpret_cast<__half2*>(&mn[k]));
+        const float2 b = __half22float2(*reinterpret_cast<__half2*>(&mx[k]));
+        low[2 * k] = a.x;
+        low[2 * k + 1] = a.y;
+        step[2 * k] = fmaxf(div_rn(b.x - a.x, 255.0f), 1e-8f);
+        step[2 * k + 1] = fmaxf(div_rn(b.y - a.y, 255.0f), 1e-8f);
+    }
+    const int page = p.pages[s.page_off + blk.blk];
+    uint8_t* codes = p.codes + half_off(page, p.kv_heads, head, j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x[8];
+        unpack(r[i], x);
+        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float v = fminf(fmaxf(rintf(div_rn(x[k] - low[k], step[k])), 0.0f), 255.0f);
+            w[k >> 2] |= uint32_t(v) << (8 * (k & 3));
+        }
+        uint8_t* row = codes + (i * 16 + part) * D;
+        *reinterpret_cast<uint32_t*>(row + 4 * c) = w[0];
+        *reinterpret_cast<uint32_t*>(row + 64 + 4 * c) = w[1];
+    }
+    if (part == 0) {
+        __half* sc = p.scales + ((int64_t(page) * p.kv_heads + head) * 4 + 2 * j) * D;
+        store_row(sc, c, Row8{make_uint2(mn[0], mn[1]), make_uint2(mn[2], mn[3])});
+        store_row(sc + D, c, pack(step));
+    }
+}
+
+// K or V of one (block, KV head) as fp16 rows.
+__global__ void __launch_bounds__(THREADS)
+    paged_read_kernel(const uint8_t* codes, const __half* scales, const __half* tails, const Seq* seqs,
+                      const int* pages, const Block* blocks, int kv_heads, __half* k_out, __half* v_out) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31, c = lane & 15, part = (threadIdx.x >> 5) * 2 + (lane >> 4);
+    const int item = blockIdx.x / (2 * kv_heads), hj = blockIdx.x % (2 * kv_heads), head = hj >> 1, j = hj & 1;
+    const Block blk = blocks[item];
+    const Seq s = seqs[blk.seq];
+    const int b0 = blk.blk * PT, from = blk.pad;
+    __half* out = (j ? v_out : k_out) + head * D;
+    const int64_t stride = int64_t(kv_heads) * D;
+    if (b0 + PT > s.kv_len) {
+        const __half* src = tails + half_off(s.tail_out, kv_heads, head, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int slot = i * 16 + part;
+            if (slot >= from && b0 + slot < s.kv_len)
+                store_row(out + (int64_t(blk.row) + slot - from) * stride, c, load_row(src + slot * D, c));
+        }
+        return;
+    }
+    const int page = pages[s.page_off + blk.blk];
+    const uint8_t* src = codes + half_off(page, kv_heads, head, j);
+    const __half* sc = scales + ((int64_t(page) * kv_heads + head) * 4 + 2 * j) * D;
+    const Row8 mn = load_row(sc, c), st = load_row(sc + D, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int slot = i * 16 + part;
+        if (slot < from) continue;
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(src + slot * D + 4 * c);
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(src + slot * D + 64 + 4 * c);
+        Row8 r;   // fp16(code * step + min), one rounding
+        r.lo = make_uint2(hfma2(u8x2_lo_to_f16x2(a), st.lo.x, mn.lo.x), hfma2(u8x2_hi_to_f16x2(a), st.lo.y, mn.lo.y));
+        r.hi = make_uint2(hfma2(u8x2_lo_to_f16x2(b), st.hi.x, mn.hi.x), hfma2(u8x2_hi_to_f16x2(b), st.hi.y, mn.hi.y));
+        store_row(out + (int64_t(blk.row) + slot - from) * stride, c, r);
+    }
+}
+
+static bool misaligned(const void* p, int64_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+// Cache pointers and sizes against what the plan uses.
+int check_cache(const char* what, const void* codes, const void* scales, const void* tails, int64_t num_pages,
+                int64_t num_tails, const void* plan, const nova_paged_plan_info* info) {
+    if (!info || !plan) return fail(NOVA_ERR_INVALID, "%s: plan and info must not be NULL", what);
+    if (info->kv_heads < 1 || info->q_heads < 1) return fail(NOVA_ERR_INVALID, "%s: info was not filled", what);
+    if (info->max_page >= num_pages)
+        return fail(NOVA_ERR_INVALID, "%s: the plan uses page %lld of %lld", what, (long long)info->max_page,
+                    (long long)num_pages);
+    if (info->max_tail >= num_tails)
+        return fail(NOVA_ERR_INVALID, "%s: the plan uses tail buffer %lld of %lld", what, (long long)info->max_tail,
+                    (long long)num_tails);
+    if ((info->max_page >= 0 && (!codes || !scales)) || (info->max_tail >= 0 && !tails))
+        return fail(NOVA_ERR_INVALID, "%s: NULL cache pointer", what);
+    if (misaligned(codes, 16) || misaligned(scales, 16) || misaligned(tails, 16) || misaligned(plan, 16))
+        return fail(NOVA_ERR_ALIGN, "%s: cache and plan need 16-byte alignment", what);
+    return NOVA_OK;
+}
+
+}  // namespace paged
+}  // namespace nova
+
+using namespace nova;
+using namespace nova::paged;
+
+extern "C" int nova_paged_append(const nova_paged_append_args* a, const nova_paged_plan_info* info, void* stream) {
+    if (!a) return fail(NOVA_ERR_INVALID, "paged append: args must not be NULL");
+    if (int rc = check_cache("paged append", a->codes, a->scales, a->tails, a->num_pages, a->num_tails, a->plan, info))
+        return rc;
+    if (!info->tokens) return NOVA_OK;
+    const int64_t width = (info->q_heads + 2 * info->kv_heads) * D;
+    if (!a->qkv || !a->q_out) return fail(NOVA_ERR_INVALID, "paged append: NULL qkv or q_out");
+    if (!a->cos != !a->sin) return fail(NOVA_ERR_INVALID, "paged append: cos and sin go together");
+    if (a->cos && info->max_pos >= a->rope_len)
+        return fail(NOVA_ERR_INVALID, "paged append: position %lld is past the rotation table's %lld rows",
+                    (long long)info->max_pos, (long long)a->rope_len);
+    if (a->qkv_stride < width || a->q_t_stride < info->q_heads * D)
+        return fail(NOVA_ERR_INVALID, "paged append: row strides below the row length");
+    if (misaligned(a->qkv, 16) || misaligned(a->q_out, 16) || a->qkv_stride % 8 || a->q_t_stride % 8 ||
+        misaligned(a->q_norm_weight, 16) || misaligned(a->k_norm_weight, 16) || misaligned(a->cos, 16) ||
+        misaligned(a->sin, 16))
+        return fail(NOVA_ERR_ALIGN, "paged append: pointers need 16-byte alignment, strides multiples of 8");
+    AppendParams p{};
+    p.qkv = static_cast<const __half*>(a->qkv);
+    p.qkv_stride = a->qkv_stride;
+    p.wq = static_cast<const __half*>(a->q_norm_weight);
+    p.wk = static_cast<const __half*>(a->k_norm_weight);
+    p.eps = float(a->eps);
+    p.cos = static_cast<const __half*>(a->cos);
+    p.sin = static_cast<const __half*>(a->sin);
+    p.q = static_cast<__half*>(a->q_out);
+    p.q_stride = a->q_t_stride;
+    p.codes = static_cast<uint8_t*>(a->codes);
+    p.scales = static_cast<__half*>(a->scales);
+    p.tails = static_cast<__half*>(a->tails);
+    p.seqs = reinterpret_cast<const Seq*>(a->plan + info->seq_off);
+    p.pages = a->plan + info->page_off;
+    p.pos = a->plan + info->pos_off;
+    p.blocks = reinterpret_cast<const Block*>(a->plan + info->write_off);
+    p.tokens = info->tokens;
+    p.n_write = int(info->n_write);
+    p.q_heads = int(info->q_heads);
+    p.kv_heads = int(info->kv_heads);
+    const int64_t q_ctas = (info->tokens * info->q_heads + PAIRS - 1) / PAIRS;
+    const int64_t grid = q_ctas + info->n_write * 2 * info->kv_heads;
+    if (grid >= (1ll << 31)) return fail(NOVA_ERR_UNSUPPORTED, "paged append: too many tokens in one step");
+    p.q_ctas = int(q_ctas);
+    launch(paged_append_kernel, dim3(unsigned(grid)), dim3(THREADS), 0, static_cast<cudaStream_t>(stream), p);
+    return check_launch("paged append");
+}
+
+extern "C" int nova_paged_read(const void* codes, const void* scales, const void* tails, int64_t num_pages,
+                               int64_t num_tails, const int32_t* plan, const nova_paged_plan_info* info, void* k_out,
+                               void* v_out, void* stream) {
+    if (int rc = check_cache("paged read", codes, scales, tails, num_pages, num_tails, plan, info)) return rc;
+    if (!info->n_read) return NOVA_OK;
+    if (!k_out || !v_out) return fail(NOVA_ERR_INVALID, "paged read: NULL output");
+    if (misaligned(k_out, 16) || misaligned(v_out, 16))
+        return fail(NOVA_ERR_ALIGN, "paged read: outputs need 16-byte alignment");
+    const int64_t grid = info->n_read * 2 * info->kv_heads;
+    if (grid >= (1ll << 31)) return fail(NOVA_ERR_UNSUPPORTED, "paged read: too many rows in one call");
+    launch(paged_read_kernel, dim3(unsigned(grid)), dim3(THREADS), 0, static_cast<cudaStream_t>(stream),
+           static_cast<const uint8_t*>(codes), static_cast<const __half*>(scales), static_cast<const __half*>(tails),
+           reinterpret_cast<const Seq*>(plan + info->seq_off), static_cast<const int*>(plan + info->page_off),
+           reinterpret_cast<const Block*>(plan + info->read_off), int(info->kv_heads), static_cast<__half*>(k_out),
+           static_cast<__half*>(v_out));
+    return check_launch("paged read");
+}

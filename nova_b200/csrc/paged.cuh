@@ -1,0 +1,37 @@
+// Layout shared by the paged-cache kernels: plan records and cache addressing.
+#pragma once
+
+#include "common.cuh"
+
+namespace nova {
+namespace paged {
+
+constexpr int D = 128;          // head_dim
+constexpr int PT = 64;          // tokens per page
+constexpr int HALF_ROW = PT * D;   // elements of K (or V) of one page and head
+
+// Plan records (int32, see nova_paged_plan).
+struct Seq {                    // one request
+    int q_start, q_len, kv_len, page_off, tail_in, tail_out, pad0, pad1;
+};
+struct RowsItem {               // few query rows x a range of 64-token blocks
+    int seq, row0, nrows, blk0, blk1, part0, split, n_splits;
+};
+struct Block {                  // one 64-token block of a request (write and read lists)
+    int seq, blk, row, pad;     // row: read list only, the output row of the block's first copied position
+};
+
+constexpr int ROWS_MAX = 16;    // query rows of one KV head that the few-rows kernel takes per tile
+constexpr int PART = 132;       // floats per row of a few-rows partial: m, l, 2 unused, acc[128]
+
+// Workspace of nova_paged_attention: error word, arrival counters, partials.
+constexpr int64_t WS_HEAD = 256;
+inline int64_t ws_counters(int64_t parts, int64_t kv_heads) { return (parts * kv_heads * 4 + 255) / 256 * 256; }
+
+// Element offset of K (j = 0) or V (j = 1) of a page or tail buffer.
+__host__ __device__ __forceinline__ int64_t half_off(int64_t index, int kv_heads, int head, int j) {
+    return ((index * kv_heads + head) * 2 + j) * HALF_ROW;
+}
+
+}  // namespace paged
+}  // namespace nova

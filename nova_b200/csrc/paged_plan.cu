@@ -1,0 +1,201 @@
+// Host side of the paged calls: the plan of one step of a batch of requests
+// (lengths, pages, work lists), built without a GPU into one int32 array that
+// the caller copies to the device once per step and every layer reads.
+#include <new>
+#include <vector>
+
+#include "paged.cuh"
+
+namespace {
+
+using nova::fail;
+using namespace nova::paged;
+
+struct Builder {
+    const nova_paged_plan_args& a;
+    std::vector<int32_t> v;
+    int64_t at() {                       // sections start on 16 bytes
+        while (v.size() % 4) v.push_back(0);
+        return int64_t(v.size());
+    }
+    template <typename T>
+    void put(const T& rec) {
+        const int32_t* p = reinterpret_cast<const int32_t*>(&rec);
+        v.insert(v.end(), p, p + sizeof(T) / 4);
+    }
+};
+
+// Lengths, page numbers and tail buffers of the step.
+int check_requests(const nova_paged_plan_args& a) {
+    if (a.seqs < 1 || a.seqs > (1 << 20)) return fail(NOVA_ERR_INVALID, "plan: seqs=%lld", (long long)a.seqs);
+    if (a.kv_heads < 1 || a.q_heads < 1 || a.q_heads % a.kv_heads)
+        return fail(NOVA_ERR_INVALID, "plan: q_heads %lld is not a multiple of kv_heads %lld", (long long)a.q_heads,
+                    (long long)a.kv_heads);
+    if (a.kv_heads > 1024 || a.q_heads > 16384 || a.sms < 1)
+        return fail(NOVA_ERR_INVALID, "plan: kv_heads, q_heads or sms out of range");
+    if (a.n_windows < 0 || a.n_windows > NOVA_PAGED_MAX_WINDOWS)
+        return fail(NOVA_ERR_INVALID, "plan: at most %d windows, got %lld", NOVA_PAGED_MAX_WINDOWS,
+                    (long long)a.n_windows);
+    for (int64_t w = 0; w < a.n_windows; ++w)
+        if (a.windows[w] < 0 || a.windows[w] > (1ll << 30)) return fail(NOVA_ERR_INVALID, "plan: window out of range");
+    const int64_t lim = (1ll << 31) - 4096;
+    int64_t tokens = 0, rows = 0;
+    std::vector<std::pair<int64_t, int64_t>> bufs, written;
+    for (int64_t i = 0; i < a.seqs; ++i) {
+        const int64_t q = a.q_lens[i], kv = a.kv_lens[i], start = kv - q, np = a.page_off[i + 1] - a.page_off[i];
+        if (q < 0 || kv < q || kv >= lim)
+            return fail(NOVA_ERR_INVALID, "plan: request %lld has %lld new tokens and length %lld", (long long)i,
+                        (long long)q, (long long)kv);
+        if (a.page_off[i] < 0 || np < kv / PT)
+            return fail(NOVA_ERR_INVALID, "plan: request %lld of length %lld has %lld pages, %lld are needed",
+                        (long long)i, (long long)kv, (long long)np, (long long)(kv / PT));
+        if (a.page_off[i + 1] >= lim) return fail(NOVA_ERR_INVALID, "plan: too many pages");
+        for (int64_t j = 0; j < np; ++j) {
+            const int64_t p = a.pages[a.page_off[i] + j];
+            if (p < 0 || p >= lim) return fail(NOVA_ERR_INVALID, "plan: request %lld has page %lld", (long long)i, (long long)p);
+            if (j >= start / PT && j < kv / PT) written.push_back({p, i});
+        }
+        const bool takes = start % PT != 0, leaves = kv % PT != 0, same = start / PT == kv / PT;
+        if ((takes && (a.tail_in[i] < 0 || a.tail_in[i] >= lim)) || (leaves && (a.tail_out[i] < 0 || a.tail_out[i] >= lim)))
+            return fail(NOVA_ERR_INVALID, "plan: request %lld needs a tail buffer", (long long)i);
+        if (takes && leaves && same && a.tail_in[i] != a.tail_out[i])
+            return fail(NOVA_ERR_INVALID, "plan: the open page of request %lld stays open: tail_out must be tail_in", (long long)i);
+        if (takes && leaves && !same && a.tail_in[i] == a.tail_out[i])
+            return fail(NOVA_ERR_INVALID, "plan: request %lld opens another page: tail_out must differ from tail_in", (long long)i);
+        if (takes) bufs.push_back({a.tail_in[i], i});
+        if (leaves) bufs.push_back({a.tail_out[i], i});
+        if (a.read_from && (a.read_from[i] < 0 || a.read_from[i] > kv))
+            return fail(NOVA_ERR_INVALID, "plan: read_from %lld of request %lld outside [0, %lld]",
+                        (long long)a.read_from[i], (long long)i, (long long)kv);
+        tokens += q;
+        rows += kv - (a.read_from ? a.read_from[i] : start / PT * PT);
+        if (tokens >= lim || rows >= lim || tokens * (a.q_heads + 2 * a.kv_heads) >= lim)
+            return fail(NOVA_ERR_UNSUPPORTED, "plan: too many tokens in one step");
+    }
+    std::sort(bufs.begin(), bufs.end());
+    for (size_t i = 1; i < bufs.size(); ++i)
+        if (bufs[i].first == bufs[i - 1].first && bufs[i].second != bufs[i - 1].second)
+            return fail(NOVA_ERR_INVALID, "plan: two requests share tail buffer %lld", (long long)bufs[i].first);
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].first == written[i - 1].first)
+            return fail(NOVA_ERR_INVALID, "plan: page %lld would be written twice", (long long)written[i].first);
+    return NOVA_OK;
+}
+
+// Blocks that the query rows [row0, row0 + nrows) of request i can see.
+void seen_blocks(const nova_paged_plan_args& a, int64_t i, int64_t row0, int64_t nrows, int64_t window, int64_t* b0,
+                 int64_t* b1) {
+    const int64_t gq = a.q_heads / a.kv_heads, start = a.kv_lens[i] - a.q_lens[i];
+    const int64_t first = start + row0 / gq, last = start + (row0 + nrows - 1) / gq;
+    *b0 = window > 0 ? std::max<int64_t>(0, first - window + 1) / PT : 0;
+    *b1 = last / PT + 1;
+}
+
+// Work list of the few-rows kernel: every tile's blocks cut into splits.
+// A split is at least one block per warp (4); enough of them that the resident
+// CTAs (3 per SM) are filled about four times over, which evens out ragged
+// lengths; and at most 32 per tile, so that joining them stays short.
+void rows_schedule(Builder& b, nova_paged_schedule& s) {
+    const nova_paged_plan_args& a = b.a;
+    const int64_t gq = a.q_heads / a.kv_heads;
+    int64_t most = 0, total = 0;
+    for (int64_t i = 0; i < a.seqs; ++i) most = std::max(most, a.q_lens[i] * gq);
+    s.rows_per_tile = most <= 4 ? 4 : most <= 8 ? 8 : ROWS_MAX;
+    for (int64_t i = 0; i < a.seqs; ++i)
+        for (int64_t r = 0; r < a.q_lens[i] * gq; r += s.rows_per_tile) {
+            int64_t b0, b1;
+            seen_blocks(a, i, r, std::min(s.rows_per_tile, a.q_lens[i] * gq - r), s.window, &b0, &b1);
+            total += b1 - b0;
+        }
+    int64_t chunk = std::max<int64_t>(4, total * a.kv_heads / (a.sms * 3 * 4) / 4 * 4);
+    s.rows_off = b.at();
+    int64_t& parts = s.n_parts;
+    for (int64_t i = 0; i < a.seqs; ++i)
+        for (int64_t r = 0; r < a.q_lens[i] * gq; r += s.rows_per_tile) {
+            const int64_t n = std::min(s.rows_per_tile, a.q_lens[i] * gq - r);
+            int64_t b0, b1;
+            seen_blocks(a, i, r, n, s.window, &b0, &b1);
+            const int64_t c = std::max(chunk, ((b1 - b0 + 31) / 32 + 3) / 4 * 4);
+            const int64_t splits = (b1 - b0 + c - 1) / c;
+            for (int64_t k = 0; k < splits; ++k) {
+                RowsItem it{int(i), int(r), int(n), int(b0 + k * c), int(std::min(b1, b0 + (k + 1) * c)),
+                            splits > 1 ? int(parts) : -1, int(k), int(splits)};
+                b.put(it);
+                ++s.n_rows;
+            }
+            if (splits > 1) parts += splits;
+        }
+}
+
+}  // namespace
+
+extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, int64_t capacity,
+                               nova_paged_plan_info* info) {
+    if (!args || !info) return fail(NOVA_ERR_INVALID, "plan: args and info must not be NULL");
+    const nova_paged_plan_args& a = *args;
+    if (!a.q_lens || !a.kv_lens || !a.page_off || !a.tail_in || !a.tail_out)
+        return fail(NOVA_ERR_INVALID, "plan: NULL array");
+    try {
+        if (a.seqs > 0 && a.page_off[a.seqs] > 0 && !a.pages) return fail(NOVA_ERR_INVALID, "plan: NULL pages");
+        if (int rc = check_requests(a)) return rc;
+        *info = nova_paged_plan_info{};
+        info->seqs = a.seqs;
+        info->q_heads = a.q_heads;
+        info->kv_heads = a.kv_heads;
+        info->max_page = info->max_tail = info->max_pos = -1;
+        Builder b{a, {}};
+        info->seq_off = b.at();
+        for (int64_t i = 0; i < a.seqs; ++i) {
+            const int64_t kv = a.kv_lens[i], start = kv - a.q_lens[i];
+            const bool takes = start % PT != 0, leaves = kv % PT != 0;
+            Seq s{int(info->tokens), int(a.q_lens[i]), int(kv), int(a.page_off[i]), takes ? int(a.tail_in[i]) : 0,
+                  leaves ? int(a.tail_out[i]) : 0, 0, 0};
+            b.put(s);
+            info->tokens += a.q_lens[i];
+            if (a.q_lens[i]) info->max_pos = std::max(info->max_pos, kv - 1);
+            if (takes) info->max_tail = std::max(info->max_tail, a.tail_in[i]);
+            if (leaves) info->max_tail = std::max(info->max_tail, a.tail_out[i]);
+        }
+        info->page_off = b.at();
+        for (int64_t j = 0; j < a.page_off[a.seqs]; ++j) {
+            b.v.push_back(int32_t(a.pages[j]));
+            info->max_page = std::max(info->max_page, a.pages[j]);
+        }
+        info->pos_off = b.at();
+        for (int64_t i = 0; i < a.seqs; ++i)
+            for (int64_t j = a.kv_lens[i] - a.q_lens[i]; j < a.kv_lens[i]; ++j) b.v.push_back(int32_t(j));
+        info->write_off = b.at();
+        for (int64_t i = 0; i < a.seqs; ++i)
+            if (a.q_lens[i])
+                for (int64_t g = (a.kv_lens[i] - a.q_lens[i]) / PT; g * PT < a.kv_lens[i]; ++g) {
+                    b.put(Block{int(i), int(g), 0, 0});
+                    ++info->n_write;
+                }
+        info->read_off = b.at();
+        for (int64_t i = 0; i < a.seqs; ++i) {
+            const int64_t from = a.read_from ? a.read_from[i] : (a.kv_lens[i] - a.q_lens[i]) / PT * PT;
+            for (int64_t g = from / PT; from < a.kv_lens[i] && g * PT < a.kv_lens[i]; ++g) {
+                const int64_t first = std::max(from, g * PT);
+                b.put(Block{int(i), int(g), int(info->read_rows), int(first - g * PT)});
+                info->read_rows += std::min((g + 1) * PT, a.kv_lens[i]) - first;
+                ++info->n_read;
+            }
+        }
+        info->n_windows = a.n_windows;
+        for (int64_t w = 0; w < a.n_windows; ++w) {
+            nova_paged_schedule& s = info->sched[w];
+            s.window = a.windows[w];
+            rows_schedule(b, s);
+            const int64_t parts = s.n_parts;
+            const int64_t bytes = WS_HEAD + ws_counters(parts, a.kv_heads) +
+                                  parts * a.kv_heads * s.rows_per_tile * PART * int64_t(sizeof(float));
+            info->workspace_bytes = std::max(info->workspace_bytes, bytes);
+        }
+        info->ints = int64_t(b.v.size());
+        if (out && capacity >= info->ints) memcpy(out, b.v.data(), b.v.size() * sizeof(int32_t));
+        return NOVA_OK;
+    } catch (const std::exception& e) {
+        return fail(NOVA_ERR_INVALID, "plan: %s", e.what());
+    }
+}
