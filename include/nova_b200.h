@@ -39,8 +39,9 @@ NOVA_API const char* nova_version(void);
 /* sizeof of the argument structs, in this order: nova_attn_int8_args,
  * nova_nf4_args, nova_qk_args, nova_prefill_attn_args, nova_qk_prefill_args,
  * nova_sample_args, nova_tp_allreduce_args, nova_paged_plan_args,
- * nova_paged_plan_info, nova_paged_append_args, nova_paged_attn_args (n
- * entries at most are written; returns how many there are).  Lets a binding check its struct mirrors. */
+ * nova_paged_plan_info, nova_paged_append_args, nova_paged_attn_args,
+ * nova_lora_args, nova_logits_args (n entries at most are written; returns
+ * how many there are).  Lets a binding check its struct mirrors. */
 NOVA_API int nova_abi_sizes(int64_t* out, int n);
 NOVA_API const char* nova_last_error(void);
 
@@ -690,6 +691,82 @@ NOVA_API int nova_paged_attention(const nova_paged_attn_args* args, const nova_p
 /* Error word of a nova_paged_attention workspace (non-zero: a bounded wait
  * gave up and that launch's output is not valid), copied and cleared. */
 NOVA_API int nova_paged_attention_read_error(void* workspace, int* host_value);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *     out[row] = fp16(base[row] + scaling[a] * (x[row] A_a^T) B_a^T)
+ * for the rows of adapter a; rows without an adapter: out = base.  x fp16
+ * [tokens, k], base and out fp16 [tokens, n] (row strides in elements; out may
+ * be base), A fp16 [adapters, max_rank, k], B fp16 [adapters, n, max_rank],
+ * contiguous; scaling fp32 [adapters] or NULL (1).  tiles: int32 [n_tiles, 4]
+ * = adapter (or -1), its rank, first entry in `rows`, number of entries (1 to
+ * tile_rows); rows: int32 token rows, those of a tile all of its adapter, each
+ * row in one tile.  Rows past a rank are never read.  k, n and max_rank
+ * multiples of 8, max_rank <= 128, tile_rows 16 or 64.  No counterpart in the
+ * reference.
+ */
+typedef struct nova_lora_args {
+    const void* x;
+    int64_t x_stride;
+    const void* base;
+    int64_t base_stride;
+    void* out;
+    int64_t out_stride;
+    const void* a;
+    const void* b;
+    const void* scaling;
+    const int32_t* tiles;     /* device                                          */
+    const int32_t* rows;      /* device                                          */
+    int64_t n_tiles, tile_rows, tokens, k, n, adapters, max_rank;
+} nova_lora_args;
+
+NOVA_API int nova_lora_add(const nova_lora_args* args, void* stream);
+
+/*
+ * Controls of each request on its logits, before sampling:
+ *     v = logits[row, t]
+ *     h = history[row, t]: low 15 bits = times generated, top bit = in the prompt
+ *     h != 0: v = v > 0 ? v / repetition[row] : v * repetition[row]
+ *     v -= frequency[row] * times + (times > 0 ? presence[row] : 0)
+ *     v += bias[row, t]                    (sparse)
+ *     mask given and its bit t clear: v = -inf, whatever v is
+ * in fp32, rounded once to the type of the logits (fp16, or fp32 when
+ * logits_fp32).  out may be logits.  NULL pointers switch a control off.
+ * allowed: uint32 [n_masks, mask_stride words], bit t % 32 of word t / 32;
+ * allowed_row: int32 [rows], the mask of a row, negative: none (NULL: row i
+ * uses mask i); a number past n_masks masks the whole row.  Biases are lists
+ * by (row, 2048-token chunk): entries [bias_off[row * chunks + c], bias_off[row
+ * * chunks + c + 1]) with chunks = ceil(vocab / 2048), token numbers of that
+ * chunk in any order, none twice.  The repetition rule is the reference's
+ * (src/chat.py:58-61); the others have no counterpart there.
+ */
+typedef struct nova_logits_args {
+    const void* logits;
+    int64_t logits_stride, logits_fp32;
+    void* out;
+    int64_t out_stride;
+    const void* history;      /* int16 [rows, vocab] or NULL                     */
+    int64_t history_stride;
+    const void* repetition;   /* fp32 [rows] or NULL (1)                         */
+    const void* frequency;    /* fp32 [rows] or NULL (0)                         */
+    const void* presence;     /* fp32 [rows] or NULL (0)                         */
+    const int32_t* bias_off;
+    const int32_t* bias_token;
+    const void* bias_value;   /* fp32                                            */
+    const void* allowed;
+    int64_t n_masks, mask_stride;
+    const int32_t* allowed_row;
+    int64_t rows, vocab;
+} nova_logits_args;
+
+NOVA_API int nova_adjust_logits(const nova_logits_args* args, void* stream);
+
+/* Enters tokens in the history: int64 tokens[off[r] .. off[r + 1]) of row r
+ * (off int32 [rows + 1]; NULL: one token per row).  prompt != 0: sets the top
+ * bit; else adds one to the count (up to 32767).  Tokens outside [0, vocab)
+ * are skipped. */
+NOVA_API int nova_history_add(void* history, int64_t history_stride, const int64_t* tokens, const int32_t* off,
+                              int64_t n_tokens, int64_t rows, int64_t vocab, int prompt, void* stream);
 
 /* --------------------------------------------------- tensor parallelism */
 

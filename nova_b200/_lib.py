@@ -162,6 +162,27 @@ class PagedAttnArgs(ctypes.Structure):
     ]
 
 
+class LoraArgs(ctypes.Structure):
+    """Mirror of ``nova_lora_args``."""
+
+    _fields_ = [
+        ("x", _P), ("x_stride", _I), ("base", _P), ("base_stride", _I), ("out", _P), ("out_stride", _I),
+        ("a", _P), ("b", _P), ("scaling", _P), ("tiles", _P), ("rows", _P),
+        ("n_tiles", _I), ("tile_rows", _I), ("tokens", _I), ("k", _I), ("n", _I), ("adapters", _I), ("max_rank", _I),
+    ]
+
+
+class LogitsArgs(ctypes.Structure):
+    """Mirror of ``nova_logits_args``."""
+
+    _fields_ = [
+        ("logits", _P), ("logits_stride", _I), ("logits_fp32", _I), ("out", _P), ("out_stride", _I),
+        ("history", _P), ("history_stride", _I), ("repetition", _P), ("frequency", _P), ("presence", _P),
+        ("bias_off", _P), ("bias_token", _P), ("bias_value", _P), ("allowed", _P), ("n_masks", _I),
+        ("mask_stride", _I), ("allowed_row", _P), ("rows", _I), ("vocab", _I),
+    ]
+
+
 # name -> argtypes (every entry point returns int status unless noted)
 _SIGNATURES: dict[str, list] = {
     "nova_abi_sizes": [_P, _i],
@@ -203,11 +224,15 @@ _SIGNATURES: dict[str, list] = {
     "nova_paged_read": [_P, _P, _P, _I, _I, _P, ctypes.POINTER(PagedPlanInfo), _P, _P, _P],
     "nova_paged_attention": [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(PagedPlanInfo), _P],
     "nova_paged_attention_read_error": [_P, ctypes.POINTER(_i)],
+    "nova_lora_add": [ctypes.POINTER(LoraArgs), _P],
+    "nova_adjust_logits": [ctypes.POINTER(LogitsArgs), _P],
+    "nova_history_add": [_P, _I, _P, _P, _I, _I, _I, _i, _P],
 }
 _STRING_FNS = ("nova_version", "nova_last_error")
 _INT_FNS = ("nova_get_launch_flags",)
 ABI_STRUCTS = ("AttnArgs", "NF4Args", "QKArgs", "PrefillAttnArgs", "QKPrefillArgs", "SampleArgs", "TPAllReduceArgs",
-               "PagedPlanArgs", "PagedPlanInfo", "PagedAppendArgs", "PagedAttnArgs")
+               "PagedPlanArgs", "PagedPlanInfo", "PagedAppendArgs", "PagedAttnArgs", "LoraArgs",
+               "LogitsArgs")
 
 _lib: ctypes.CDLL | None = None
 

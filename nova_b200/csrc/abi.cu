@@ -93,7 +93,8 @@ extern "C" int nova_abi_sizes(int64_t* out, int n) {
                              int64_t(sizeof(nova_qk_prefill_args)),   int64_t(sizeof(nova_sample_args)),
                              int64_t(sizeof(nova_tp_allreduce_args)), int64_t(sizeof(nova_paged_plan_args)),
                              int64_t(sizeof(nova_paged_plan_info)),   int64_t(sizeof(nova_paged_append_args)),
-                             int64_t(sizeof(nova_paged_attn_args))};
+                             int64_t(sizeof(nova_paged_attn_args)),   int64_t(sizeof(nova_lora_args)),
+                             int64_t(sizeof(nova_logits_args))};
     const int count = int(sizeof(sizes) / sizeof(sizes[0]));
     for (int i = 0; i < n && i < count && out; ++i) out[i] = sizes[i];
     return count;

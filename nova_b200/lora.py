@@ -1,0 +1,106 @@
+"""Low-rank adapters of many requests at once, beside a projection whose weights
+they share (the NF4 linears: ``nova_b200.kernels.nf4_gemm``).
+
+    plan = LoraPlan(token_counts, adapter_of_request, ranks)       # once per step
+    y = nf4_gemm(x, ...)                                           # the shared projection
+    y = lora_add(x, y, a, b, plan, scaling=scaling, out=y)         # + s (x A^T) B^T per request
+
+No counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+from ctypes import byref
+from typing import Sequence
+
+import numpy as np
+import torch
+
+from . import _lib
+
+MAX_RANK = 128
+
+
+class LoraPlan:
+    """Which adapter each token row of a step takes.
+
+    ``token_counts``: rows of each request, one after another; ``adapters``: the
+    adapter of each request, negative for none; ``ranks``: rank of every adapter
+    (1 .. 128; 0 switches one off).  Rows of one adapter are gathered into tiles
+    whatever their requests; the plan serves every projection of the step."""
+
+    def __init__(self, token_counts: Sequence[int], adapters: Sequence[int], ranks: Sequence[int], *,
+                 device: torch.device | str = "cuda") -> None:
+        counts, which = np.asarray(token_counts, dtype=np.int64), np.asarray(adapters, dtype=np.int64)
+        rank = np.asarray(ranks, dtype=np.int64)
+        if counts.ndim != 1 or counts.shape != which.shape or rank.ndim != 1:
+            raise ValueError("token_counts and adapters must be flat and of one length, ranks flat")
+        if (counts < 0).any():
+            raise ValueError("token_counts must not be negative")
+        if len(which) and which.max() >= len(rank):
+            raise ValueError(f"adapter {which.max()} of {len(rank)}")
+        if len(rank) and (rank.min() < 0 or rank.max() > MAX_RANK):
+            raise ValueError(f"ranks must lie in [0, {MAX_RANK}]")
+        self.tokens, self.adapters = int(counts.sum()), len(rank)
+        self.max_rank = int(rank.max()) if len(rank) else 0
+        of_row = np.repeat(np.where(which < 0, -1, which), counts)
+        if len(rank):
+            of_row = np.where((of_row >= 0) & (rank[of_row] == 0), -1, of_row)
+        rows = np.argsort(of_row, kind="stable")
+        values, first, n = np.unique(of_row[rows], return_index=True, return_counts=True)
+        busy = n[values >= 0]
+        # 64-row tiles read an adapter's weights once per 64 rows; single tokens would leave them empty
+        self.tile_rows = 64 if len(busy) and busy.max() > 32 else 16
+        tiles = []
+        for v, f, m in zip(values.tolist(), first.tolist(), n.tolist()):
+            r = int(rank[v]) if v >= 0 else 0
+            tiles += [(v, r, f + i, min(self.tile_rows, m - i)) for i in range(0, m, self.tile_rows)]
+        self.n_tiles = len(tiles)
+        host = np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), rows.astype(np.int32)])
+        self.device = torch.device(device)
+        self.buffer = torch.from_numpy(host).to(self.device)
+
+
+def lora_add(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan, *,
+             scaling: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``base + scaling[a] * (x A_a^T) B_a^T`` for every row's adapter ``a``, one launch.
+
+    ``x`` fp16 ``[tokens, K]``; ``base`` fp16 ``[tokens, N]`` (the shared
+    projection's output); ``a`` fp16 ``[adapters, R, K]``; ``b`` fp16 ``[adapters,
+    N, R]``, R a multiple of 8 up to 128 and at least every rank (entries past an
+    adapter's rank are not read); ``scaling`` fp32 ``[adapters]``.  ``out`` may be
+    ``base``; rows without an adapter are then left alone.  Returns fp16
+    ``[tokens, N]``."""
+    _lib.require_cuda(x, base, a, b, scaling, out, names=("x", "base", "a", "b", "scaling", "out"))
+    for t, name in ((x, "x"), (base, "base"), (a, "a"), (b, "b")):
+        if t.dtype != torch.float16 or t.device != x.device:
+            raise ValueError(f"{name} must be float16 on the device of x, got {t.dtype} on {t.device}")
+    if x.dim() != 2 or base.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError("x and base must be 2-D, a and b 3-D")
+    tokens, k = x.shape
+    n, adapters, r = base.shape[1], a.shape[0], a.shape[1]
+    if base.shape[0] != tokens or tokens != plan.tokens or plan.buffer.device != x.device:
+        raise ValueError(f"x {tuple(x.shape)}, base {tuple(base.shape)} and the plan's {plan.tokens} rows do not match")
+    if tuple(a.shape) != (adapters, r, k) or tuple(b.shape) != (adapters, n, r) or adapters != plan.adapters:
+        raise ValueError(f"a {tuple(a.shape)} / b {tuple(b.shape)} do not match K={k}, N={n}, {plan.adapters} adapters")
+    if plan.max_rank > r:
+        raise ValueError(f"the plan has rank {plan.max_rank}, the weights hold {r}")
+    if not a.is_contiguous() or not b.is_contiguous() or x.stride(1) != 1 or base.stride(1) != 1:
+        raise ValueError("a and b must be contiguous, x and base have a contiguous last dimension")
+    if scaling is not None and (scaling.dtype != torch.float32 or tuple(scaling.shape) != (adapters,)
+                                or scaling.device != x.device or not scaling.is_contiguous()):
+        raise ValueError(f"scaling must be contiguous float32 [{adapters}]")
+    if out is None:
+        out = torch.empty((tokens, n), dtype=torch.float16, device=x.device)
+    elif out.dtype != torch.float16 or tuple(out.shape) != (tokens, n) or out.device != x.device or out.stride(1) != 1:
+        raise ValueError(f"out must be float16 [{tokens}, {n}] with a contiguous last dimension")
+    args = _lib.LoraArgs()
+    args.x, args.x_stride = x.data_ptr(), x.stride(0) if tokens > 1 else k
+    args.base, args.base_stride = base.data_ptr(), base.stride(0) if tokens > 1 else n
+    args.out, args.out_stride = out.data_ptr(), out.stride(0) if tokens > 1 else n
+    args.a, args.b, args.scaling = a.data_ptr(), b.data_ptr(), _lib.ptr(scaling)
+    args.tiles, args.rows = plan.buffer.data_ptr(), plan.buffer.data_ptr() + 16 * plan.n_tiles
+    args.n_tiles, args.tile_rows, args.tokens = plan.n_tiles, plan.tile_rows, tokens
+    args.k, args.n, args.adapters, args.max_rank = k, n, adapters, r
+    _lib.check(_lib.lib().nova_lora_add(byref(args), _lib.stream_of(x.device)), "nova_lora_add")
+    return out
