@@ -604,6 +604,8 @@ typedef struct nova_paged_schedule {
     int64_t window;
     int64_t rows_off, n_rows, rows_per_tile;   /* work items of few query rows   */
     int64_t n_parts;                           /* partial results of split items */
+    int64_t segs_off, ctas_off, n_ctas;        /* segments of many query rows    */
+    int64_t joins_off, n_joins, n_tile_parts;  /* tiles cut between CTAs         */
 } nova_paged_schedule;
 
 /* What a plan holds and where (offsets in int32 from the plan's start). */

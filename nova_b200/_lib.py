@@ -128,7 +128,8 @@ class PagedPlanArgs(ctypes.Structure):
 class PagedSchedule(ctypes.Structure):
     """Mirror of ``nova_paged_schedule``."""
 
-    _fields_ = [("window", _I), ("rows_off", _I), ("n_rows", _I), ("rows_per_tile", _I), ("n_parts", _I)]
+    _fields_ = [("window", _I), ("rows_off", _I), ("n_rows", _I), ("rows_per_tile", _I), ("n_parts", _I),
+                ("segs_off", _I), ("ctas_off", _I), ("n_ctas", _I), ("joins_off", _I), ("n_joins", _I), ("n_tile_parts", _I)]
 
 
 class PagedPlanInfo(ctypes.Structure):

@@ -17,6 +17,12 @@ struct Seq {                    // one request
 struct RowsItem {               // few query rows x a range of 64-token blocks
     int seq, row0, nrows, blk0, blk1, part0, split, n_splits;
 };
+struct TileSeg {                // many query rows (up to 256) x a range of blocks; part < 0: the whole tile
+    int seq, head, row0, nrows, blk0, blk1, part, pad;
+};
+struct TileJoin {               // a tile whose segments left partials
+    int seq, head, row0, nrows, part0, n_parts, pad0, pad1;
+};
 struct Block {                  // one 64-token block of a request (write and read lists)
     int seq, blk, row, pad;     // row: read list only, the output row of the block's first copied position
 };
@@ -27,6 +33,10 @@ constexpr int PART = 132;       // floats per row of a few-rows partial: m, l, 2
 // Workspace of nova_paged_attention: error word, arrival counters, partials.
 constexpr int64_t WS_HEAD = 256;
 inline int64_t ws_counters(int64_t parts, int64_t kv_heads) { return (parts * kv_heads * 4 + 255) / 256 * 256; }
+
+inline int64_t ws_rows_bytes(int64_t parts, int64_t kv_heads, int64_t rows_per_tile) {
+    return WS_HEAD + ws_counters(parts, kv_heads) + (parts * kv_heads * rows_per_tile * PART * 4 + 255) / 256 * 256;
+}
 
 // Element offset of K (j = 0) or V (j = 1) of a page or tail buffer.
 __host__ __device__ __forceinline__ int64_t half_off(int64_t index, int kv_heads, int head, int j) {

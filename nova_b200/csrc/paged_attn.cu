@@ -23,6 +23,9 @@ namespace paged {
 int check_cache(const char* what, const void* codes, const void* scales, const void* tails, int64_t num_pages,
                 int64_t num_tails, const void* plan, const nova_paged_plan_info* info);
 
+int launch_tiles(const nova_paged_attn_args* a, const nova_paged_plan_info* info, const nova_paged_schedule& s,
+                 cudaStream_t stream);
+
 namespace rows {
 
 constexpr int NW = 4;
@@ -508,6 +511,9 @@ extern "C" int nova_paged_attention(const nova_paged_attn_args* a, const nova_pa
         return fail(NOVA_ERR_UNSUPPORTED, "paged attention: %lld pages of %lld heads exceed 2^31 code rows",
                     (long long)a->num_pages, (long long)info->kv_heads);
     const nova_paged_schedule& s = info->sched[a->sched];
+    if (s.n_ctas)
+        if (int rc = launch_tiles(a, info, s, static_cast<cudaStream_t>(stream))) return rc;
+    if (!s.n_rows) return NOVA_OK;
     rows::Params p{};
     p.q = static_cast<const __half*>(a->q);
     p.q_t = a->q_t_stride;

@@ -92,6 +92,11 @@ void seen_blocks(const nova_paged_plan_args& a, int64_t i, int64_t row0, int64_t
     *b1 = last / PT + 1;
 }
 
+// Which kernel takes request i: one tile of the few-rows kernel holds 16 query
+// rows of a KV head; more would read the cache once per 16 rows there, and once
+// per 256 rows in the tensor-core kernel.
+bool few_rows(const nova_paged_plan_args& a, int64_t i) { return a.q_lens[i] * (a.q_heads / a.kv_heads) <= ROWS_MAX; }
+
 // Work list of the few-rows kernel: every tile's blocks cut into splits.
 // A split is at least one block per warp (4); enough of them that the resident
 // CTAs (3 per SM) are filled about four times over, which evens out ragged
@@ -100,10 +105,11 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
     const nova_paged_plan_args& a = b.a;
     const int64_t gq = a.q_heads / a.kv_heads;
     int64_t most = 0, total = 0;
-    for (int64_t i = 0; i < a.seqs; ++i) most = std::max(most, a.q_lens[i] * gq);
+    for (int64_t i = 0; i < a.seqs; ++i)
+        if (few_rows(a, i)) most = std::max(most, a.q_lens[i] * gq);
     s.rows_per_tile = most <= 4 ? 4 : most <= 8 ? 8 : ROWS_MAX;
     for (int64_t i = 0; i < a.seqs; ++i)
-        for (int64_t r = 0; r < a.q_lens[i] * gq; r += s.rows_per_tile) {
+        for (int64_t r = 0; few_rows(a, i) && r < a.q_lens[i] * gq; r += s.rows_per_tile) {
             int64_t b0, b1;
             seen_blocks(a, i, r, std::min(s.rows_per_tile, a.q_lens[i] * gq - r), s.window, &b0, &b1);
             total += b1 - b0;
@@ -112,7 +118,7 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
     s.rows_off = b.at();
     int64_t& parts = s.n_parts;
     for (int64_t i = 0; i < a.seqs; ++i)
-        for (int64_t r = 0; r < a.q_lens[i] * gq; r += s.rows_per_tile) {
+        for (int64_t r = 0; few_rows(a, i) && r < a.q_lens[i] * gq; r += s.rows_per_tile) {
             const int64_t n = std::min(s.rows_per_tile, a.q_lens[i] * gq - r);
             int64_t b0, b1;
             seen_blocks(a, i, r, n, s.window, &b0, &b1);
@@ -126,6 +132,72 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
             }
             if (splits > 1) parts += splits;
         }
+}
+
+// Segments of the tensor-core kernel: the steps (128 keys) of all 256-row tiles
+// in a row, request by request and head by head so that neighbouring CTAs read
+// the same cache, cut into equal shares.  A segment costs about SEG_COST steps
+// besides its own (Q, the first loads, the result), and none is shorter than
+// MIN_STEPS unless its tile is.
+constexpr int64_t SEG_COST = 2, MIN_STEPS = 4;
+
+void tile_schedule(Builder& b, nova_paged_schedule& s) {
+    const nova_paged_plan_args& a = b.a;
+    const int64_t gq = a.q_heads / a.kv_heads;
+    int64_t total = 0;
+    for (int64_t i = 0; i < a.seqs; ++i)
+        for (int64_t r = 0; !few_rows(a, i) && r < a.q_lens[i] * gq; r += 256) {
+            int64_t b0, b1;
+            seen_blocks(a, i, r, std::min<int64_t>(256, a.q_lens[i] * gq - r), s.window, &b0, &b1);
+            total += ((b1 - b0 + 1) / 2 + SEG_COST) * a.kv_heads;
+        }
+    if (!total) return;
+    // What a CTA takes of the rest: an even share of it, recomputed per CTA since cuts are uneven.
+    auto share = [&](int64_t rest, int64_t started) {
+        const int64_t n = std::max<int64_t>(1, a.sms - started);
+        return std::max((rest + n - 1) / n, MIN_STEPS + SEG_COST);
+    };
+    std::vector<int32_t> ctas{0};
+    std::vector<TileJoin> joins;
+    s.segs_off = b.at();
+    int64_t segs = 0, rest = total, left = share(rest, 0);   // left: what the current CTA still takes
+    for (int64_t i = 0; i < a.seqs; ++i) {
+        if (few_rows(a, i)) continue;
+        for (int64_t h = 0; h < a.kv_heads; ++h)
+            for (int64_t r = 0; r < a.q_lens[i] * gq; r += 256) {
+                const int64_t n = std::min<int64_t>(256, a.q_lens[i] * gq - r);
+                int64_t b0, b1;
+                seen_blocks(a, i, r, n, s.window, &b0, &b1);
+                const int64_t first_part = s.n_tile_parts, blk0 = b0;
+                while (b0 < b1) {
+                    if (left < MIN_STEPS + SEG_COST && int64_t(ctas.size()) < a.sms) {   // the next CTA
+                        if (ctas.back() != segs) ctas.push_back(int32_t(segs));
+                        left = share(rest, int64_t(ctas.size()) - 1);
+                    }
+                    const int64_t steps = (b1 - b0 + 1) / 2;
+                    int64_t take = std::min(steps, std::max(left - SEG_COST, MIN_STEPS));
+                    if (steps - take < MIN_STEPS || int64_t(ctas.size()) >= a.sms) take = steps;
+                    const int64_t end = std::min(b1, b0 + 2 * take);
+                    const bool cut = b0 != blk0 || end != b1;
+                    b.put(TileSeg{int(i), int(h), int(r), int(n), int(b0), int(end), cut ? int(s.n_tile_parts++) : -1, 0});
+                    ++segs;
+                    left -= take + SEG_COST;
+                    rest -= take;
+                    b0 = end;
+                }
+                rest -= SEG_COST;
+                if (s.n_tile_parts > first_part)
+                    joins.push_back(TileJoin{int(i), int(h), int(r), int(n), int(first_part),
+                                             int(s.n_tile_parts - first_part), 0, 0});
+            }
+    }
+    if (ctas.back() != segs) ctas.push_back(int32_t(segs));
+    s.n_ctas = int64_t(ctas.size()) - 1;
+    s.ctas_off = b.at();
+    b.v.insert(b.v.end(), ctas.begin(), ctas.end());
+    s.joins_off = b.at();
+    s.n_joins = int64_t(joins.size());
+    for (const TileJoin& j : joins) b.put(j);
 }
 
 }  // namespace
@@ -187,9 +259,8 @@ extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, i
             nova_paged_schedule& s = info->sched[w];
             s.window = a.windows[w];
             rows_schedule(b, s);
-            const int64_t parts = s.n_parts;
-            const int64_t bytes = WS_HEAD + ws_counters(parts, a.kv_heads) +
-                                  parts * a.kv_heads * s.rows_per_tile * PART * int64_t(sizeof(float));
+            tile_schedule(b, s);
+            const int64_t bytes = ws_rows_bytes(s.n_parts, a.kv_heads, s.rows_per_tile) + s.n_tile_parts * 256 * (D + 2) * 4;
             info->workspace_bytes = std::max(info->workspace_bytes, bytes);
         }
         info->ints = int64_t(b.v.size());

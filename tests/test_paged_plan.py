@@ -54,8 +54,9 @@ def test_read_from():
 @pytest.mark.parametrize("window", [0, 1, 63, 200])
 @pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 2), (6, 2), (16, 1)])
 def test_every_row_sees_its_blocks_once(hq, hkv, window):
-    """For each query row: the blocks of all work items that hold it are its
-    key range's blocks (or more of the same tile's), each once."""
+    """For each query row (and KV head): the blocks of all work items and
+    segments that hold it are its key range's blocks (or more of the same
+    tile's), each once; a cut tile's partials are joined in order."""
     q, kv = [1, 3, 0, 17, 1, 1], [1, 64, 10, 400, 5000, 63]
     p = make(q, kv, hq, hkv, windows=(window,))
     gq = hq // hkv
@@ -64,6 +65,28 @@ def test_every_row_sees_its_blocks_once(hq, hkv, window):
         assert 0 <= split < n and (part0 < 0) == (n == 1) and b1 > b0 and nrows >= 1
         for r in range(row0, row0 + nrows):
             seen.setdefault((seq, r), []).extend(range(b0, b1))
+    tiles = {}
+    sched = p.info.sched[0]
+    ctas = p.host[sched.ctas_off:sched.ctas_off + sched.n_ctas + 1].tolist()
+    assert ctas == sorted(set(ctas)) and len(ctas) <= 149
+    segs = p.host[sched.segs_off:sched.segs_off + 8 * ctas[-1]].reshape(-1, 8).tolist() if sched.n_ctas else []
+    for seq, head, row0, nrows, b0, b1, part, _ in segs:
+        assert b1 > b0 and 1 <= nrows <= 256
+        tiles.setdefault((seq, head, row0, nrows), []).append((b0, b1, part))
+    joins = p.host[sched.joins_off:sched.joins_off + 8 * sched.n_joins].reshape(-1, 8).tolist()
+    joins = {tuple(j[:4]): (j[4], j[5]) for j in joins}
+    for key, parts in tiles.items():
+        assert [x[1] for x in parts[:-1]] == [x[0] for x in parts[1:]]
+        if len(parts) > 1:
+            first, count = joins.pop(key)
+            assert [x[2] for x in parts] == list(range(first, first + count))
+        else:
+            assert parts[0][2] == -1
+        seq, head, row0, nrows = key
+        for r in range(row0, row0 + nrows):
+            blocks = [b for b0, b1, _ in parts for b in range(b0, b1)]
+            assert seen.setdefault((seq, r), blocks) == blocks    # every head the same
+    assert not joins and len(tiles) % hkv == 0
     for i, (m, n) in enumerate(zip(q, kv)):
         for r in range(m * gq):
             pos = n - m + r // gq
