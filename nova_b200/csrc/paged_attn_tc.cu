@@ -147,7 +147,7 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
 struct Raw {
     uint2 code[8];
     uint4 mn, st;
-    int kind;                          // 0: nothing (zeros), 1: page, 2: open page
+    int page;                          // -1: the open page, -2: nothing (zeros)
 };
 
 __device__ __forceinline__ uint4 dequant8(uint2 w, const uint4& st, const uint4& mn) {
@@ -203,33 +203,44 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
     if (warp >= 8 && warp < 12) {
         // ------------------------------------------------ loading warps
         reg_inc<REG_LOAD>();
-        const int tid = threadIdx.x - 256, c = tid & 15, r0 = tid >> 4;   // chunk, first row (of 8)
+        const int tid = threadIdx.x - 256, c = tid & 15, r0 = tid >> 4;   // 8 channels, first row (of 8)
         uint32_t kc = 0, segs = 0;     // steps and segments so far
         for (int sg = seg0; sg < seg1; ++sg, ++segs) {
             const TileSeg it = p.segs[sg];
             const Seq s = p.seqs[it.seq];
             const int n_full = s.kv_len / PT, start_row = it.row0;
             const int steps = (it.blk1 - it.blk0 + 1) >> 1;
-            auto fetch = [&](Raw& raw, int blk, int j) {
-                raw.kind = blk >= it.blk1 ? 0 : blk < n_full ? 1 : 2;
-                if (raw.kind == 1) {
-                    const int64_t ph = int64_t(p.pages[s.page_off + blk]) * p.kv_heads + it.head;
-                    const uint8_t* src = p.codes + (ph * 2 + j) * HALF_ROW + 8 * c;
+            const int* pages = p.pages + s.page_off;
+            const uint8_t* codes = p.codes + it.head * 2 * HALF_ROW + r0 * D + 8 * c;
+            const __half* scales = p.scales + it.head * 4 * D + 8 * c;
+            const int code_step = p.kv_heads * 2 * HALF_ROW, scale_step = p.kv_heads * 4 * D;   // per page
+            // Page number of the segment's block b (-1: the open page, -2: past the end).  Lane b % 32 holds
+            // those of 32 blocks, the next 32 already requested: nothing waits for a page number.
+            auto lookup = [&](int b) { return it.blk0 + b < min(it.blk1, n_full) ? pages[it.blk0 + b] : -1; };
+            int ids = lookup(lane), ids_next = lookup(32 + lane);
+            auto page_of = [&](int b) {
+                const int id = __shfl_sync(0xffffffffu, ids, b & 31);
+                return it.blk0 + b < it.blk1 ? id : -2;
+            };
+            auto fetch = [&](Raw& raw, int page, int j) {
+                raw.page = page;
+                if (page >= 0) {
+                    const uint8_t* src = codes + int64_t(page) * code_step + j * HALF_ROW;
+                    const __half* sc = scales + int64_t(page) * scale_step + j * 2 * D;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) raw.code[i] = *reinterpret_cast<const uint2*>(src + (r0 + 8 * i) * D);
-                    const __half* sc = p.scales + (ph * 4 + 2 * j) * D + 8 * c;
+                    for (int i = 0; i < 8; ++i) raw.code[i] = *reinterpret_cast<const uint2*>(src + 8 * i * D);
                     raw.mn = *reinterpret_cast<const uint4*>(sc);
                     raw.st = *reinterpret_cast<const uint4*>(sc + D);
                 }
             };
             auto store = [&](const Raw& raw, uint32_t tile, int half, int j) {
                 const uint32_t dst = tile + half * 8192 + tile_off(r0, c);   // 8 rows on: 1024 bytes, the same swizzle
-                if (raw.kind == 1) {
+                if (raw.page >= 0) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sts128(dst + i * 1024, dequant8(raw.code[i], raw.st, raw.mn));
                 } else {               // the open page (slots that hold no token read as zero) or nothing
                     const __half* src = p.tails + half_off(s.tail_out, p.kv_heads, it.head, j) + 8 * c;
-                    const int live = raw.kind == 2 ? s.kv_len - n_full * PT : 0;
+                    const int live = raw.page == -1 ? s.kv_len - n_full * PT : 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int r = r0 + 8 * i;
@@ -244,8 +255,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                 if (lane == 0) mbar_arrive(bar);
             };
             Raw k0, k1, v0, v1;
-            fetch(k0, it.blk0, 0);
-            fetch(k1, it.blk0 + 1, 0);
+            int pg0 = page_of(0), pg1 = page_of(1);
+            fetch(k0, pg0, 0);
+            fetch(k1, pg1, 0);
+            fetch(v0, pg0, 1);
+            fetch(v1, pg1, 1);
             // Q rows of this segment, once the last one's products have read theirs
             if (segs && !wait(&q_empty, (segs - 1) & 1u)) break;
             for (int r = r0; r < 256; r += 8) {
@@ -258,28 +272,28 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                 sts128(sbase + Q_OFF + (r >> 7) * TILE + tile_off(r & 127, c), v);
             }
             publish(&q_full);
-            fetch(v0, it.blk0, 1);
-            fetch(v1, it.blk0 + 1, 1);
             bool ok = true;
             for (int j = 0; j < steps; ++j, ++kc) {
                 const uint32_t st = kc & 1u, ph = ((kc >> 1) & 1u) ^ 1u;
-                const int next = it.blk0 + 2 * (j + 1);
                 if (kc >= 2 && !(ok = wait(&k_empty[st], ph))) break;
                 store(k0, sbase + K_OFF + st * TILE, 0, 0);
                 store(k1, sbase + K_OFF + st * TILE, 1, 0);
                 publish(&k_full[st]);
-                if (j + 1 < steps) {
-                    fetch(k0, next, 0);
-                    fetch(k1, next + 1, 0);
+                const int b = 2 * j + 2;
+                if ((b & 31) == 0) {
+                    ids = ids_next;
+                    ids_next = lookup(b + 32 + lane);
                 }
+                pg0 = page_of(b);
+                pg1 = page_of(b + 1);
+                fetch(k0, pg0, 0);
+                fetch(k1, pg1, 0);
                 if (kc >= 2 && !(ok = wait(&v_empty[st], ph))) break;
                 store(v0, sbase + V_OFF + st * TILE, 0, 1);
                 store(v1, sbase + V_OFF + st * TILE, 1, 1);
                 publish(&v_full[st]);
-                if (j + 1 < steps) {
-                    fetch(v0, next, 1);
-                    fetch(v1, next + 1, 1);
-                }
+                fetch(v0, pg0, 1);
+                fetch(v1, pg1, 1);
             }
             if (!ok) break;
         }
