@@ -18,7 +18,8 @@ struct RowsItem {               // few query rows x a range of 64-token blocks
     int seq, row0, nrows, blk0, blk1, part0, split, n_splits;
 };
 struct TileSeg {                // many query rows (up to 256) x a range of blocks; part < 0: the whole tile
-    int seq, head, row0, nrows, blk0, blk1, part, pad;
+    int seq, head, row0, nrows, blk0, blk1, part, q_start;
+    int start, kv_len, page_off, tail, pad0, pad1, pad2, pad3;   // the request's: position of its first new token, ...
 };
 struct TileJoin {               // a tile whose segments left partials
     int seq, head, row0, nrows, part0, n_parts, pad0, pad1;

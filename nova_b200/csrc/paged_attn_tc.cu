@@ -47,12 +47,12 @@ struct Params {
     __half* out;
     int64_t o_t, o_h;
     float* lse;
-    const Seq* seqs;
+    const Seq* seqs;                   // the joining kernel's; segments carry what they need
     const int* pages;
     const TileSeg* segs;
     const int* cta_first;
     int* err;
-    float* part;                       // [part][256][128], then [part][256] (m, l)
+    float* part;                       // [part][32][256][4]: four channels of all rows, then the next four
     float2* part_ml;
     int q_heads, kv_heads, gq, window;
     float scale_log2;
@@ -158,7 +158,7 @@ __device__ __forceinline__ uint4 dequant8(uint2 w, const uint4& st, const uint4&
 __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __grid_constant__ Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, q_empty, s_full[2], p_ready[2],
+    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], p_ready[2],
         o_full[2], drain;
     __shared__ uint32_t tmem_s;
     __shared__ int dead_s;
@@ -174,9 +174,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], 4);
             mbar_init(&o_full[i], 1);
+            mbar_init(&q_full[i], 4);
         }
-        mbar_init(&q_full, 4);
-        mbar_init(&q_empty, 1);
         mbar_init(&drain, 1);
         fence_mbar_init();
         dead_s = 0;
@@ -204,13 +203,12 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
         // ------------------------------------------------ loading warps
         reg_inc<REG_LOAD>();
         const int tid = threadIdx.x - 256, c = tid & 15, r0 = tid >> 4;   // 8 channels, first row (of 8)
-        uint32_t kc = 0, segs = 0;     // steps and segments so far
-        for (int sg = seg0; sg < seg1; ++sg, ++segs) {
+        uint32_t kc = 0;               // steps so far
+        for (int sg = seg0; sg < seg1; ++sg) {
             const TileSeg it = p.segs[sg];
-            const Seq s = p.seqs[it.seq];
-            const int n_full = s.kv_len / PT, start_row = it.row0;
+            const int n_full = it.kv_len / PT;
             const int steps = (it.blk1 - it.blk0 + 1) >> 1;
-            const int* pages = p.pages + s.page_off;
+            const int* pages = p.pages + it.page_off;
             const uint8_t* codes = p.codes + it.head * 2 * HALF_ROW + r0 * D + 8 * c;
             const __half* scales = p.scales + it.head * 4 * D + 8 * c;
             const int code_step = p.kv_heads * 2 * HALF_ROW, scale_step = p.kv_heads * 4 * D;   // per page
@@ -239,8 +237,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sts128(dst + i * 1024, dequant8(raw.code[i], raw.st, raw.mn));
                 } else {               // the open page (slots that hold no token read as zero) or nothing
-                    const __half* src = p.tails + half_off(s.tail_out, p.kv_heads, it.head, j) + 8 * c;
-                    const int live = raw.page == -1 ? s.kv_len - n_full * PT : 0;
+                    const __half* src = p.tails + half_off(it.tail, p.kv_heads, it.head, j) + 8 * c;
+                    const int live = raw.page == -1 ? it.kv_len - n_full * PT : 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int r = r0 + 8 * i;
@@ -260,18 +258,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
             fetch(k1, pg1, 0);
             fetch(v0, pg0, 1);
             fetch(v1, pg1, 1);
-            // Q rows of this segment, once the last one's products have read theirs
-            if (segs && !wait(&q_empty, (segs - 1) & 1u)) break;
-            for (int r = r0; r < 256; r += 8) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (r < it.nrows) {
-                    const int row = start_row + r, tok = row / p.gq;
-                    v = *reinterpret_cast<const uint4*>(p.q + int64_t(s.q_start + tok) * p.q_t +
-                                                        int64_t(it.head * p.gq + row - tok * p.gq) * p.q_h + 8 * c);
-                }
-                sts128(sbase + Q_OFF + (r >> 7) * TILE + tile_off(r & 127, c), v);
-            }
-            publish(&q_full);
             bool ok = true;
             for (int j = 0; j < steps; ++j, ++kc) {
                 const uint32_t st = kc & 1u, ph = ((kc >> 1) & 1u) ^ 1u;
@@ -303,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
         if (warp == 12) {              // the whole warp walks along, so that addresses stay in uniform registers
             constexpr uint32_t idesc_qk = tc_idesc_f16(128, 128);
             constexpr uint32_t idesc_pv = tc_idesc_f16(128, 128) | (1u << 16);   // B MN-major
-            uint32_t kc = 0, segs = 0, pc[2] = {0u, 0u};
+            uint32_t kc = 0, sc[2] = {0u, 0u}, pc[2] = {0u, 0u};   // steps; segments and steps of each half
             bool ok = true;
             auto qk = [&](int i, uint32_t st) {
                 const uint32_t a = kmajor(sbase + Q_OFF + i * TILE), b = kmajor(sbase + K_OFF + st * TILE);
@@ -321,14 +307,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                 if (elect_one()) tc_commit(bar);
                 __syncwarp();
             };
-            for (int sg = seg0; sg < seg1 && ok; ++sg, ++segs) {
+            for (int sg = seg0; sg < seg1 && ok; ++sg) {
                 const TileSeg it = p.segs[sg];
                 const int steps = (it.blk1 - it.blk0 + 1) >> 1, halves = it.nrows > 128 ? 2 : 1;
-                if (!(ok = wait(&q_full, segs & 1u))) break;
                 if (!(ok = wait(&k_full[kc & 1u], (kc >> 1) & 1u))) break;
-                for (int i = 0; i < halves; ++i) qk(i, kc & 1u);
+                for (int i = 0; i < halves; ++i) {
+                    if (!(ok = wait(&q_full[i], sc[i]++ & 1u))) break;
+                    qk(i, kc & 1u);
+                }
+                if (!ok) break;
                 commit(&k_empty[kc & 1u]);
-                if (steps == 1) commit(&q_empty);
                 for (int j = 0; j < steps && ok; ++j, ++kc) {
                     const uint32_t st = kc & 1u;
                     if (!(ok = wait(&v_full[st], (kc >> 1) & 1u))) break;
@@ -354,7 +342,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                     if (!ok) break;
                     commit(&v_empty[st]);
                     if (j + 1 < steps) commit(&k_empty[(kc + 1) & 1u]);
-                    if (j + 2 == steps) commit(&q_empty);
                 }
             }
             commit(&drain);            // every MMA of this CTA has completed before its tensor memory is freed
@@ -372,13 +359,26 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
         for (int sg = seg0; sg < seg1 && ok; ++sg) {
             const TileSeg it = p.segs[sg];
             if (half * 128 >= it.nrows) continue;
-            const Seq s = p.seqs[it.seq];
-            const int start = s.kv_len - s.q_len, steps = (it.blk1 - it.blk0 + 1) >> 1;
+            const int start = it.start, steps = (it.blk1 - it.blk0 + 1) >> 1;
             const int r = half * 128 + row;                          // row of the segment
             const bool live = r < it.nrows;
             const int arow = it.row0 + (live ? r : it.nrows - 1), tok = arow / p.gq, pos = start + tok;
             const int first_pos = start + (it.row0 + half * 128) / p.gq;
             const int last_pos = start + (it.row0 + min(half * 128 + 127, it.nrows - 1)) / p.gq;
+            // This thread's row of Q (rows past the segment's repeat its last one and are not stored); every
+            // product of this half's last segment is complete (o_full), so its tile is free.
+            const int head = it.head * p.gq + arow - tok * p.gq;
+            {
+                const __half* src = p.q + int64_t(it.q_start + tok) * p.q_t + int64_t(head) * p.q_h;
+                uint4 v[16];
+#pragma unroll
+                for (int c = 0; c < 16; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) sts128(sbase + Q_OFF + half * TILE + tile_off(row, c), v[c]);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[half]);
+            }
             float m = -INFINITY, l = 0.f;                            // m: the maximum that O and l are relative to (log2)
             for (int j = 0; j < steps; ++j, ++sc) {
                 const int key0 = (it.blk0 + 2 * j) * PT;
@@ -445,10 +445,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
             if (!(ok = wait(&o_full[half], oc & 1u))) break;
             ++oc;
             tc_fence_after();
-            const int head = it.head * p.gq + arow - tok * p.gq;
             const float inv = l > 0.f ? 1.0f / l : 0.f;
-            __half* dst = p.out + int64_t(s.q_start + tok) * p.o_t + int64_t(head) * p.o_h;
-            float* prow = p.part + (int64_t(it.part) * 256 + r) * D;
+            __half* dst = p.out + int64_t(it.q_start + tok) * p.o_t + int64_t(head) * p.o_h;
+            float4* prow = reinterpret_cast<float4*>(p.part) + int64_t(it.part) * 32 * 256 + r;
 #pragma unroll
             for (int k = 0; k < 128; k += 32) {
                 float o[32];
@@ -464,14 +463,14 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(prow + k + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        prow[(k + e) * 64] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
             if (live) {
                 if (it.part >= 0)
                     p.part_ml[int64_t(it.part) * 256 + r] = make_float2(m, l);
                 else if (p.lse)
-                    p.lse[int64_t(s.q_start + tok) * p.q_heads + head] =
+                    p.lse[int64_t(it.q_start + tok) * p.q_heads + head] =
                         l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
             }
             tc_fence_before();         // the next segment's first product overwrites O after this half's next p_ready
@@ -485,33 +484,42 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
     }
 }
 
-// Joins the partials of tiles that were cut, in segment order: a warp per row.
+// Joins the partials of tiles that were cut, in segment order.  A CTA takes 32
+// rows, a lane one of them and a warp 16 channels: partials are read as they
+// were written, 512 consecutive bytes per warp and load.
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const Params p, const TileJoin* joins) {
     pdl_wait();
     const TileJoin it = joins[blockIdx.x];
-    const int r = int(blockIdx.y) * 8 + int(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int r = int(blockIdx.y) * 32 + int(threadIdx.x & 31), w = threadIdx.x >> 5;
     if (r >= it.nrows) return;
-    const Seq s = p.seqs[it.seq];
-    const int64_t first = int64_t(it.part0) * 256 + r;
-    float M = -INFINITY;
-    for (int k = lane; k < it.n_parts; k += 32) M = fmaxf(M, p.part_ml[first + k * 256].x);
+    const float2* ml = p.part_ml + int64_t(it.part0) * 256 + r;
+    const float4* part = reinterpret_cast<const float4*>(p.part) + (int64_t(it.part0) * 32 + 4 * w) * 256 + r;
+    float M = -INFINITY, L = 0.f;
+    for (int k = 0; k < it.n_parts; ++k) M = fmaxf(M, ml[k * 256].x);
+    float4 o[4];
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    float L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+    for (int c = 0; c < 4; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
     for (int k = 0; k < it.n_parts; ++k) {
-        const float2 ml = p.part_ml[first + k * 256];
-        const float4 a = *reinterpret_cast<const float4*>(p.part + (first + k * 256) * D + 4 * lane);
-        const float wt = M == -INFINITY ? 0.f : exp2f(ml.x - M);
-        L += wt * ml.y;
-        o.x += wt * a.x; o.y += wt * a.y; o.z += wt * a.z; o.w += wt * a.w;
+        const float2 e = ml[k * 256];
+        const float wt = M == -INFINITY ? 0.f : exp2f(e.x - M);
+        L += wt * e.y;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float4 a = part[(int64_t(k) * 32 + c) * 256];
+            o[c].x += wt * a.x; o[c].y += wt * a.y; o[c].z += wt * a.z; o[c].w += wt * a.w;
+        }
     }
+    const Seq s = p.seqs[it.seq];
     const int row = it.row0 + r, tok = row / p.gq, head = it.head * p.gq + row - tok * p.gq;
     const float inv = L > 0.f ? 1.0f / L : 0.f;
-    *reinterpret_cast<uint2*>(p.out + int64_t(s.q_start + tok) * p.o_t + int64_t(head) * p.o_h + 4 * lane) =
-        make_uint2(pack_f16x2(o.x * inv, o.y * inv), pack_f16x2(o.z * inv, o.w * inv));
-    if (p.lse && lane == 0)
+    __half* dst = p.out + int64_t(s.q_start + tok) * p.o_t + int64_t(head) * p.o_h + 16 * w;
+#pragma unroll
+    for (int c = 0; c < 4; c += 2)
+        *reinterpret_cast<uint4*>(dst + 4 * c) =
+            make_uint4(pack_f16x2(o[c].x * inv, o[c].y * inv), pack_f16x2(o[c].z * inv, o[c].w * inv),
+                       pack_f16x2(o[c + 1].x * inv, o[c + 1].y * inv), pack_f16x2(o[c + 1].z * inv, o[c + 1].w * inv));
+    if (p.lse && w == 0)
         p.lse[int64_t(s.q_start + tok) * p.q_heads + head] = L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
 }
 
@@ -554,7 +562,7 @@ int launch_tiles(const nova_paged_attn_args* a, const nova_paged_plan_info* info
     launch(tc::paged_attn_tile_kernel, dim3(unsigned(s.n_ctas)), dim3(tc::THREADS), tc::SMEM, stream, p);
     if (int rc = check_launch("paged attention")) return rc;
     if (!s.n_joins) return NOVA_OK;
-    launch(tc::paged_attn_join_kernel, dim3(unsigned(s.n_joins), 32), dim3(256), 0, stream, p,
+    launch(tc::paged_attn_join_kernel, dim3(unsigned(s.n_joins), 8), dim3(256), 0, stream, p,
            reinterpret_cast<const TileJoin*>(a->plan + s.joins_off));
     return check_launch("paged attention");
 }

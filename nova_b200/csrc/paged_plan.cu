@@ -160,8 +160,9 @@ void tile_schedule(Builder& b, nova_paged_schedule& s) {
     std::vector<int32_t> ctas{0};
     std::vector<TileJoin> joins;
     s.segs_off = b.at();
-    int64_t segs = 0, rest = total, left = share(rest, 0);   // left: what the current CTA still takes
+    int64_t q_start = 0, segs = 0, rest = total, left = share(rest, 0);   // left: what the current CTA still takes
     for (int64_t i = 0; i < a.seqs; ++i) {
+        q_start += i ? a.q_lens[i - 1] : 0;
         if (few_rows(a, i)) continue;
         for (int64_t h = 0; h < a.kv_heads; ++h)
             for (int64_t r = 0; r < a.q_lens[i] * gq; r += 256) {
@@ -179,7 +180,8 @@ void tile_schedule(Builder& b, nova_paged_schedule& s) {
                     if (steps - take < MIN_STEPS || int64_t(ctas.size()) >= a.sms) take = steps;
                     const int64_t end = std::min(b1, b0 + 2 * take);
                     const bool cut = b0 != blk0 || end != b1;
-                    b.put(TileSeg{int(i), int(h), int(r), int(n), int(b0), int(end), cut ? int(s.n_tile_parts++) : -1, 0});
+                    b.put(TileSeg{int(i), int(h), int(r), int(n), int(b0), int(end), cut ? int(s.n_tile_parts++) : -1, int(q_start), int(a.kv_lens[i] - a.q_lens[i]), int(a.kv_lens[i]),
+                                  int(a.page_off[i]), a.kv_lens[i] % PT ? int(a.tail_out[i]) : 0, 0, 0, 0, 0});
                     ++segs;
                     left -= take + SEG_COST;
                     rest -= take;

@@ -69,8 +69,10 @@ def test_every_row_sees_its_blocks_once(hq, hkv, window):
     sched = p.info.sched[0]
     ctas = p.host[sched.ctas_off:sched.ctas_off + sched.n_ctas + 1].tolist()
     assert ctas == sorted(set(ctas)) and len(ctas) <= 149
-    segs = p.host[sched.segs_off:sched.segs_off + 8 * ctas[-1]].reshape(-1, 8).tolist() if sched.n_ctas else []
-    for seq, head, row0, nrows, b0, b1, part, _ in segs:
+    segs = p.host[sched.segs_off:sched.segs_off + 16 * ctas[-1]].reshape(-1, 16).tolist() if sched.n_ctas else []
+    for seq, head, row0, nrows, b0, b1, part, q_start, start, kv_len, page_off, tail, *_ in segs:
+        assert (q_start, start, kv_len) == (sum(q[:seq]), kv[seq] - q[seq], kv[seq])
+        assert page_off == sum(n // PAGE for n in kv[:seq]) and (not kv_len % PAGE or tail == p.tail_out[seq])
         assert b1 > b0 and 1 <= nrows <= 256
         tiles.setdefault((seq, head, row0, nrows), []).append((b0, b1, part))
     joins = p.host[sched.joins_off:sched.joins_off + 8 * sched.n_joins].reshape(-1, 8).tolist()
