@@ -15,7 +15,6 @@ The repetition rule is that of the reference's ``sample_next`` (src/chat.py:58-6
 
 from __future__ import annotations
 
-from ctypes import byref
 from typing import Mapping, Sequence
 
 import numpy as np
@@ -24,7 +23,7 @@ import torch
 from . import _lib
 
 CHUNK = 2048     # tokens per bias list (one CTA's tokens)
-PROMPT = -32768  # the history's top bit
+_ADJUST = _lib.Entry("nova_adjust_logits", _lib.LogitsArgs, _lib._P)
 
 
 class LogitBias:
@@ -51,6 +50,8 @@ class LogitBias:
         m = len(off)
         self.off, self.token = self.buffer[:m], self.buffer[m:m + n]
         self.value = self.buffer[m + n:].view(torch.float32)
+        at = self.buffer.data_ptr()
+        self._pointers = (at, at + 4 * m, at + 4 * (m + n)) if n else (0, 0, 0)
 
 
 def new_history(rows: int, vocab: int, device: torch.device | str = "cuda") -> torch.Tensor:
@@ -105,51 +106,54 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     none; default: row i has mask i).  What a mask forbids becomes -inf whatever
     it was, NaN included; a row whose mask leaves nothing is all -inf.  ``out``
     may be ``logits``.  Returns a tensor of the logits' type."""
-    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in (torch.float16, torch.float32) \
-            or logits.stride(1) != 1:
+    i, dtype, shape = logits.get_device(), logits.dtype, logits.shape
+    if i < 0 or len(shape) != 2 or (dtype != torch.float16 and dtype != torch.float32) or logits.stride(1) != 1:
         raise ValueError("logits must be CUDA float16 or float32 [rows, vocab] with a contiguous last dimension")
-    rows, vocab = logits.shape
-    dev = logits.device
+    rows, vocab = shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
-    elif out.dtype != logits.dtype or out.shape != logits.shape or out.device != dev or out.stride(1) != 1:
+        out = torch.empty(shape, dtype=dtype, device=logits.device)
+    elif out.dtype != dtype or out.shape != shape or out.get_device() != i or out.stride(1) != 1:
         raise ValueError("out must have the shape, type and device of logits and a contiguous last dimension")
-    a = _lib.LogitsArgs()
-    a.logits, a.logits_stride, a.logits_fp32 = logits.data_ptr(), logits.stride(0), logits.dtype == torch.float32
-    a.out, a.out_stride = out.data_ptr(), out.stride(0)
+    hist = hist_stride = 0
     if history is not None:
-        _check_history(history)
-        if history.shape != logits.shape or history.device != dev:
-            raise ValueError(f"history must be {tuple(logits.shape)} on the logits' device")
-        a.history, a.history_stride = history.data_ptr(), history.stride(0)
+        if history.dtype != torch.int16 or history.shape != shape or history.get_device() != i or history.stride(1) != 1:
+            raise ValueError(f"history must be int16 {tuple(shape)} on the logits' device with a contiguous last dimension")
+        hist, hist_stride = history.data_ptr(), history.stride(0)
+    controls = []
     for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
         if t is None:
+            controls.append(0)
             continue
-        if t.dtype != torch.float32 or tuple(t.shape) != (rows,) or t.device != dev or not t.is_contiguous():
+        if t.dtype != torch.float32 or t.shape != (rows,) or t.get_device() != i or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous float32 [{rows}] on the logits' device")
         if history is None:
             raise ValueError(f"{name} needs a history")
-        setattr(a, name, t.data_ptr())
+        controls.append(t.data_ptr())
+    biases = (0, 0, 0)
     if bias is not None:
-        if (bias.rows, bias.vocab) != (rows, vocab) or bias.buffer.device != dev:
-            raise ValueError(f"bias is for [{bias.rows}, {bias.vocab}] logits, got {tuple(logits.shape)}")
-        if bias.token.numel():
-            a.bias_off, a.bias_token, a.bias_value = bias.off.data_ptr(), bias.token.data_ptr(), bias.value.data_ptr()
+        if bias.rows != rows or bias.vocab != vocab or bias.buffer.get_device() != i:
+            raise ValueError(f"bias is for [{bias.rows}, {bias.vocab}] logits, got {tuple(shape)}")
+        biases = bias._pointers
+    mask = masks = mask_stride = mask_row = 0
     if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] < 1 \
-                or allowed.shape[1] < -(-vocab // 32) or allowed.device != dev or allowed.stride(1) != 1 \
-                or (allowed.shape[0] > 1 and allowed.stride(0) < allowed.shape[1]):
-            raise ValueError(f"allowed must be int32 [masks, {-(-vocab // 32)}] on the logits' device")
-        a.allowed, a.n_masks, a.mask_stride = allowed.data_ptr(), allowed.shape[0], max(allowed.stride(0), allowed.shape[1])
+        words = (vocab + 31) // 32
+        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.get_device() != i:
+            raise ValueError(f"allowed must be int32 [masks, {words}] on the logits' device")
+        masks, width = allowed.shape
+        mask_stride, last = allowed.stride()
+        if masks < 1 or width < words or last != 1 or (masks > 1 and mask_stride < width):
+            raise ValueError(f"allowed must be int32 [masks, {words}] with rows of their own, got {tuple(allowed.shape)}")
+        mask, mask_stride = allowed.data_ptr(), max(mask_stride, width)
         if allowed_row is not None:
-            if allowed_row.dtype != torch.int32 or tuple(allowed_row.shape) != (rows,) or allowed_row.device != dev \
+            if allowed_row.dtype != torch.int32 or allowed_row.shape != (rows,) or allowed_row.get_device() != i \
                     or not allowed_row.is_contiguous():
                 raise ValueError(f"allowed_row must be contiguous int32 [{rows}] on the logits' device")
-            a.allowed_row = allowed_row.data_ptr()
-        elif allowed.shape[0] != rows:
-            raise ValueError(f"{allowed.shape[0]} masks for {rows} rows need allowed_row")
+            mask_row = allowed_row.data_ptr()
+        elif masks != rows:
+            raise ValueError(f"{masks} masks for {rows} rows need allowed_row")
     elif allowed_row is not None:
         raise ValueError("allowed_row needs allowed")
-    a.rows, a.vocab = rows, vocab
-    _lib.check(_lib.lib().nova_adjust_logits(byref(a), _lib.stream_of(dev)), "nova_adjust_logits")
+    _ADJUST(_ADJUST.pack(logits.data_ptr(), logits.stride(0), dtype == torch.float32, out.data_ptr(), out.stride(0), hist,
+                         hist_stride, *controls, *biases, mask, masks, mask_stride, mask_row, rows, vocab),
+            _lib.raw_stream(i))
     return out

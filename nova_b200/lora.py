@@ -10,7 +10,6 @@ No counterpart in the reference.
 
 from __future__ import annotations
 
-from ctypes import byref
 from typing import Sequence
 
 import numpy as np
@@ -19,6 +18,8 @@ import torch
 from . import _lib
 
 MAX_RANK = 128
+_F16 = torch.float16
+_ADD = _lib.Entry("nova_lora_add", _lib.LoraArgs, _lib._P)
 
 
 class LoraPlan:
@@ -59,6 +60,17 @@ class LoraPlan:
         host = np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), rows.astype(np.int32)])
         self.device = torch.device(device)
         self.buffer = torch.from_numpy(host).to(self.device)
+        self._index = self.buffer.get_device()
+        self._stream = _lib.raw_stream(self._index) if self._index >= 0 else 0
+        self._tiles = self.buffer.data_ptr()
+        self._rows = self._tiles + 16 * self.n_tiles
+
+    def _current(self) -> int:
+        """The current stream; tells the allocator when it is not the plan's own."""
+        stream = _lib.raw_stream(self._index)
+        if stream != self._stream:
+            self.buffer.record_stream(torch.cuda.current_stream(self._index))
+        return stream
 
 
 def lora_add(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan, *,
@@ -71,36 +83,39 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tens
     adapter's rank are not read); ``scaling`` fp32 ``[adapters]``.  ``out`` may be
     ``base``; rows without an adapter are then left alone.  Returns fp16
     ``[tokens, N]``."""
-    _lib.require_cuda(x, base, a, b, scaling, out, names=("x", "base", "a", "b", "scaling", "out"))
+    i = plan._index
+    if i < 0:
+        raise ValueError("the plan is not on a CUDA device")
     for t, name in ((x, "x"), (base, "base"), (a, "a"), (b, "b")):
-        if t.dtype != torch.float16 or t.device != x.device:
-            raise ValueError(f"{name} must be float16 on the device of x, got {t.dtype} on {t.device}")
-    if x.dim() != 2 or base.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        if t.dtype != _F16 or t.get_device() != i:
+            raise ValueError(f"{name} must be float16 on the plan's CUDA device, got {t.dtype} on {t.device}")
+    if x.dim() != 2 or base.dim() != 2 or a.dim() != 3:
         raise ValueError("x and base must be 2-D, a and b 3-D")
     tokens, k = x.shape
-    n, adapters, r = base.shape[1], a.shape[0], a.shape[1]
-    if base.shape[0] != tokens or tokens != plan.tokens or plan.buffer.device != x.device:
+    n = base.shape[1]
+    adapters, r, _ = a.shape
+    if base.shape[0] != tokens or tokens != plan.tokens:
         raise ValueError(f"x {tuple(x.shape)}, base {tuple(base.shape)} and the plan's {plan.tokens} rows do not match")
-    if tuple(a.shape) != (adapters, r, k) or tuple(b.shape) != (adapters, n, r) or adapters != plan.adapters:
+    if a.shape[2] != k or b.shape != (adapters, n, r) or adapters != plan.adapters:
         raise ValueError(f"a {tuple(a.shape)} / b {tuple(b.shape)} do not match K={k}, N={n}, {plan.adapters} adapters")
     if plan.max_rank > r:
         raise ValueError(f"the plan has rank {plan.max_rank}, the weights hold {r}")
-    if not a.is_contiguous() or not b.is_contiguous() or x.stride(1) != 1 or base.stride(1) != 1:
+    x_stride, x_last = x.stride()
+    base_stride, base_last = base.stride()
+    if not a.is_contiguous() or not b.is_contiguous() or x_last != 1 or base_last != 1:
         raise ValueError("a and b must be contiguous, x and base have a contiguous last dimension")
-    if scaling is not None and (scaling.dtype != torch.float32 or tuple(scaling.shape) != (adapters,)
-                                or scaling.device != x.device or not scaling.is_contiguous()):
-        raise ValueError(f"scaling must be contiguous float32 [{adapters}]")
+    if scaling is not None and (scaling.dtype != torch.float32 or scaling.shape != (adapters,)
+                                or scaling.get_device() != i or not scaling.is_contiguous()):
+        raise ValueError(f"scaling must be contiguous float32 [{adapters}] on the plan's device")
     if out is None:
-        out = torch.empty((tokens, n), dtype=torch.float16, device=x.device)
-    elif out.dtype != torch.float16 or tuple(out.shape) != (tokens, n) or out.device != x.device or out.stride(1) != 1:
-        raise ValueError(f"out must be float16 [{tokens}, {n}] with a contiguous last dimension")
-    args = _lib.LoraArgs()
-    args.x, args.x_stride = x.data_ptr(), x.stride(0) if tokens > 1 else k
-    args.base, args.base_stride = base.data_ptr(), base.stride(0) if tokens > 1 else n
-    args.out, args.out_stride = out.data_ptr(), out.stride(0) if tokens > 1 else n
-    args.a, args.b, args.scaling = a.data_ptr(), b.data_ptr(), _lib.ptr(scaling)
-    args.tiles, args.rows = plan.buffer.data_ptr(), plan.buffer.data_ptr() + 16 * plan.n_tiles
-    args.n_tiles, args.tile_rows, args.tokens = plan.n_tiles, plan.tile_rows, tokens
-    args.k, args.n, args.adapters, args.max_rank = k, n, adapters, r
-    _lib.check(_lib.lib().nova_lora_add(byref(args), _lib.stream_of(x.device)), "nova_lora_add")
+        out, out_stride = torch.empty((tokens, n), dtype=_F16, device=x.device), n
+    else:
+        if out.dtype != _F16 or out.shape != (tokens, n) or out.get_device() != i or out.stride(1) != 1:
+            raise ValueError(f"out must be float16 [{tokens}, {n}] with a contiguous last dimension")
+        out_stride = out.stride(0)
+    if tokens == 1:                      # a single row's stride says nothing
+        x_stride, base_stride, out_stride = k, n, n
+    _ADD(_ADD.pack(x.data_ptr(), x_stride, base.data_ptr(), base_stride, out.data_ptr(), out_stride, a.data_ptr(),
+                   b.data_ptr(), 0 if scaling is None else scaling.data_ptr(), plan._tiles, plan._rows, plan.n_tiles,
+                   plan.tile_rows, tokens, k, n, adapters, r), plan._current())
     return out

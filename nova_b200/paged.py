@@ -25,7 +25,7 @@ The reference has no counterpart: its caches share one length over the batch
 from __future__ import annotations
 
 import itertools
-from ctypes import byref
+from ctypes import addressof, byref
 from typing import Sequence
 
 import numpy as np
@@ -35,6 +35,9 @@ from . import _lib
 
 PAGE = 64
 HEAD_DIM = 128
+_F16 = torch.float16
+_APPEND = _lib.Entry("nova_paged_append", _lib.PagedAppendArgs, _lib._P, _lib._P)
+_ATTEND = _lib.Entry("nova_paged_attention", _lib.PagedAttnArgs, _lib._P, _lib._P)
 
 
 def _i64(values, name: str) -> np.ndarray:
@@ -109,14 +112,19 @@ class PagePlan:
         self.host = buf[:int(self.info.ints)]
         self.buffer = torch.from_numpy(self.host).to(self.device)
         self.workspace = torch.zeros(int(self.info.workspace_bytes), dtype=torch.uint8, device=self.device)
-        self._stream = _lib.stream_of(self.device) if self.device.type == "cuda" else 0
+        self._index = self.buffer.get_device()                    # -1: on the host, for inspection only
+        self._stream = _lib.raw_stream(self._index) if self._index >= 0 else 0
+        self._info, self._buffer = addressof(self.info), self.buffer.data_ptr()
+        self._workspace, self._workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
 
-    def _on(self, stream: int) -> None:
-        """Tell the allocator when a stream other than the plan's own uses its buffers."""
+    def _current(self) -> int:
+        """The current stream; tells the allocator when it is not the plan's own."""
+        stream = _lib.raw_stream(self._index)
         if stream != self._stream:
-            current = torch.cuda.current_stream(self.device)
+            current = torch.cuda.current_stream(self._index)
             self.buffer.record_stream(current)
             self.workspace.record_stream(current)
+        return stream
 
     def check_errors(self) -> None:
         """Raises RuntimeError when a bounded wait of an attention launch with
@@ -127,20 +135,23 @@ class PagePlan:
             raise RuntimeError(f"paged attention: a bounded wait gave up (code {v.value})")
 
 
-def _cache(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan) -> None:
+def _cache(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan) -> tuple[int, int]:
+    """Checks one layer's storage against the plan -> (pages, tail buffers)."""
     h = plan.num_kv_heads
-    if codes.dtype != torch.uint8 or codes.dim() != 5 or tuple(codes.shape[1:]) != (h, 2, PAGE, HEAD_DIM):
-        raise ValueError(f"codes must be uint8 [pages, {h}, 2, {PAGE}, {HEAD_DIM}], got {codes.dtype} {tuple(codes.shape)}")
-    if scales.dtype != torch.float16 or tuple(scales.shape) != (codes.shape[0], h, 4, HEAD_DIM):
-        raise ValueError(f"scales must be float16 [{codes.shape[0]}, {h}, 4, {HEAD_DIM}], got {scales.dtype} "
+    cs, ts = codes.shape, tails.shape
+    if codes.dtype != torch.uint8 or len(cs) != 5 or cs[1:] != (h, 2, PAGE, HEAD_DIM):
+        raise ValueError(f"codes must be uint8 [pages, {h}, 2, {PAGE}, {HEAD_DIM}], got {codes.dtype} {tuple(cs)}")
+    if scales.dtype != _F16 or scales.shape != (cs[0], h, 4, HEAD_DIM):
+        raise ValueError(f"scales must be float16 [{cs[0]}, {h}, 4, {HEAD_DIM}], got {scales.dtype} "
                          f"{tuple(scales.shape)}")
-    if tails.dtype != torch.float16 or tails.dim() != 5 or tuple(tails.shape[1:]) != (h, 2, PAGE, HEAD_DIM):
-        raise ValueError(f"tails must be float16 [buffers, {h}, 2, {PAGE}, {HEAD_DIM}], got {tails.dtype} "
-                         f"{tuple(tails.shape)}")
+    if tails.dtype != _F16 or len(ts) != 5 or ts[1:] != cs[1:]:
+        raise ValueError(f"tails must be float16 [buffers, {h}, 2, {PAGE}, {HEAD_DIM}], got {tails.dtype} {tuple(ts)}")
     if not (codes.is_contiguous() and scales.is_contiguous() and tails.is_contiguous()):
         raise ValueError("codes, scales and tails must be contiguous")
-    if not (codes.device == scales.device == tails.device == plan.buffer.device) or not codes.is_cuda:
+    i = plan._index
+    if i < 0 or codes.get_device() != i or scales.get_device() != i or tails.get_device() != i:
         raise ValueError("codes, scales, tails and the plan must be on one CUDA device")
+    return cs[0], ts[0]
 
 
 def qkv_append(qkv: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan, *,
@@ -156,40 +167,38 @@ def qkv_append(qkv: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tai
     128]``; None: none), in fp32 and rounded once.  K and V of a page that fills
     are quantized from its 64 tokens, the others stay in ``tails``.  Returns the
     queries, fp16 ``[tokens, H_q, 128]``."""
-    hq, hkv = plan.num_q_heads, plan.num_kv_heads
-    _cache(codes, scales, tails, plan)
-    if qkv.dtype != torch.float16 or tuple(qkv.shape) != (plan.tokens, (hq + 2 * hkv) * HEAD_DIM):
+    hq, hkv, i = plan.num_q_heads, plan.num_kv_heads, plan._index
+    pages, buffers = _cache(codes, scales, tails, plan)
+    shape = (plan.tokens, hq, HEAD_DIM)
+    if qkv.dtype != _F16 or qkv.shape != (plan.tokens, (hq + 2 * hkv) * HEAD_DIM):
         raise ValueError(f"qkv must be float16 [{plan.tokens}, {(hq + 2 * hkv) * HEAD_DIM}], got {qkv.dtype} "
                          f"{tuple(qkv.shape)}")
-    if qkv.device != codes.device or qkv.stride(1) != 1:
+    qkv_stride, last = qkv.stride()
+    if qkv.get_device() != i or last != 1:
         raise ValueError("qkv must be on the cache's device, with a contiguous last dimension")
     for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        if t is not None and (t.dtype != torch.float16 or tuple(t.shape) != (HEAD_DIM,) or t.device != qkv.device
-                              or not t.is_contiguous()):
+        if t is not None and (t.dtype != _F16 or t.shape != (HEAD_DIM,) or t.get_device() != i or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float16 [{HEAD_DIM}] on the cache's device")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
+    rope_len = 0
     if cos is not None:
+        rope_len = cos.shape[0]
         for t, name in ((cos, "cos"), (sin, "sin")):
-            if t.dtype != torch.float16 or t.dim() != 2 or t.shape[1] != HEAD_DIM or t.shape != cos.shape \
-                    or t.device != qkv.device or not t.is_contiguous():
+            if t.dtype != _F16 or t.shape != (rope_len, HEAD_DIM) or t.get_device() != i or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous float16 [rope_len, {HEAD_DIM}] on the cache's device")
     if out is None:
-        out = torch.empty(plan.tokens, hq, HEAD_DIM, dtype=torch.float16, device=qkv.device)
-    elif (out.dtype != torch.float16 or tuple(out.shape) != (plan.tokens, hq, HEAD_DIM) or out.device != qkv.device
-          or out.stride(2) != 1 or out.stride(1) != HEAD_DIM):
-        raise ValueError(f"out must be float16 [{plan.tokens}, {hq}, {HEAD_DIM}] with contiguous rows")
-    a = _lib.PagedAppendArgs()
-    a.qkv, a.qkv_stride = qkv.data_ptr(), qkv.stride(0)
-    a.q_norm_weight, a.k_norm_weight, a.eps = _lib.ptr(q_norm_weight), _lib.ptr(k_norm_weight), float(eps)
-    if cos is not None:
-        a.cos, a.sin, a.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    a.q_out, a.q_t_stride = out.data_ptr(), out.stride(0)
-    a.codes, a.scales, a.tails = codes.data_ptr(), scales.data_ptr(), tails.data_ptr()
-    a.num_pages, a.num_tails, a.plan = codes.shape[0], tails.shape[0], plan.buffer.data_ptr()
-    stream = _lib.stream_of(qkv.device)
-    plan._on(stream)
-    _lib.check(_lib.lib().nova_paged_append(byref(a), byref(plan.info), stream), "nova_paged_append")
+        out, out_stride = torch.empty(shape, dtype=_F16, device=qkv.device), hq * HEAD_DIM
+    else:
+        if (out.dtype != _F16 or out.shape != shape or out.get_device() != i or out.stride(2) != 1
+                or out.stride(1) != HEAD_DIM):
+            raise ValueError(f"out must be float16 {shape} with contiguous rows")
+        out_stride = out.stride(0)
+    _APPEND(_APPEND.pack(qkv.data_ptr(), qkv_stride, 0 if q_norm_weight is None else q_norm_weight.data_ptr(),
+                         0 if k_norm_weight is None else k_norm_weight.data_ptr(), eps,
+                         0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), rope_len,
+                         out.data_ptr(), out_stride, codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages,
+                         buffers, plan._buffer), plan._info, plan._current())
     return out
 
 
@@ -198,14 +207,14 @@ def paged_read(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, p
     """The cached K and V of positions ``[read_from, kv_len)`` of every request of
     the plan, as the values they stand for: two fp16 ``[rows, H_kv, 128]``
     tensors, requests one after another."""
-    _cache(codes, scales, tails, plan)
-    kv = torch.empty(2, plan.read_rows, plan.num_kv_heads, HEAD_DIM, dtype=torch.float16, device=codes.device)
-    k, v = kv.unbind(0)
-    stream = _lib.stream_of(codes.device)
-    plan._on(stream)
-    _lib.check(_lib.lib().nova_paged_read(codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), codes.shape[0],
-                                          tails.shape[0], plan.buffer.data_ptr(), byref(plan.info), k.data_ptr(),
-                                          v.data_ptr(), stream), "nova_paged_read")
+    pages, buffers = _cache(codes, scales, tails, plan)
+    shape = (plan.read_rows, plan.num_kv_heads, HEAD_DIM)
+    k = torch.empty(shape, dtype=_F16, device=codes.device)
+    v = torch.empty(shape, dtype=_F16, device=codes.device)
+    rc = _lib.lib().nova_paged_read(codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages, buffers, plan._buffer,
+                                    plan._info, k.data_ptr(), v.data_ptr(), plan._current())
+    if rc:
+        _lib.check(rc, "nova_paged_read")
     return k, v
 
 
@@ -220,32 +229,26 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     ``scale``: of the scores (default ``128 ** -0.5``).  ``lse_out``: fp32
     ``[tokens, H_q]``, log-sum-exp of the scaled scores.  Returns fp16
     ``[tokens, H_q, 128]``."""
-    hq = plan.num_q_heads
-    _cache(codes, scales, tails, plan)
-    shape = (plan.tokens, hq, HEAD_DIM)
-    if q.dtype != torch.float16 or tuple(q.shape) != shape or q.device != codes.device or q.stride(2) != 1:
+    pages, buffers = _cache(codes, scales, tails, plan)
+    shape, i = (plan.tokens, plan.num_q_heads, HEAD_DIM), plan._index
+    if q.dtype != _F16 or q.shape != shape or q.get_device() != i or q.stride(2) != 1:
         raise ValueError(f"q must be float16 {shape} on the cache's device with a contiguous last dimension, got "
                          f"{q.dtype} {tuple(q.shape)}")
     if window not in plan.windows:
         raise ValueError(f"window {window} is not one of the plan's {plan.windows}")
     if out is None:
-        out = torch.empty(shape, dtype=torch.float16, device=q.device)
-    elif out.dtype != torch.float16 or tuple(out.shape) != shape or out.device != q.device or out.stride(2) != 1:
+        out = torch.empty(shape, dtype=_F16, device=q.device)
+    elif out.dtype != _F16 or out.shape != shape or out.get_device() != i or out.stride(2) != 1:
         raise ValueError(f"out must be float16 {shape} with a contiguous last dimension")
-    if lse_out is not None and (lse_out.dtype != torch.float32 or tuple(lse_out.shape) != shape[:2]
-                                or lse_out.device != q.device or not lse_out.is_contiguous()):
+    if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.shape != shape[:2]
+                                or lse_out.get_device() != i or not lse_out.is_contiguous()):
         raise ValueError(f"lse_out must be contiguous float32 {shape[:2]}")
-    a = _lib.PagedAttnArgs()
-    a.q, a.q_t_stride, a.q_h_stride = q.data_ptr(), q.stride(0), q.stride(1)
-    a.codes, a.scales, a.tails = codes.data_ptr(), scales.data_ptr(), tails.data_ptr()
-    a.num_pages, a.num_tails = codes.shape[0], tails.shape[0]
-    a.out, a.o_t_stride, a.o_h_stride = out.data_ptr(), out.stride(0), out.stride(1)
-    a.lse, a.scale = _lib.ptr(lse_out), HEAD_DIM ** -0.5 if scale is None else float(scale)
-    a.plan, a.workspace, a.workspace_bytes = plan.buffer.data_ptr(), plan.workspace.data_ptr(), plan.workspace.numel()
-    a.sched = plan.windows.index(window)
-    stream = _lib.stream_of(q.device)
-    plan._on(stream)
-    _lib.check(_lib.lib().nova_paged_attention(byref(a), byref(plan.info), stream), "nova_paged_attention")
+    q_t, q_h, _ = q.stride()
+    o_t, o_h, _ = out.stride()
+    _ATTEND(_ATTEND.pack(q.data_ptr(), q_t, q_h, codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages, buffers,
+                         out.data_ptr(), o_t, o_h, 0 if lse_out is None else lse_out.data_ptr(),
+                         HEAD_DIM ** -0.5 if scale is None else scale, plan._buffer, plan._workspace,
+                         plan._workspace_bytes, plan.windows.index(window)), plan._info, plan._current())
     return out
 
 
