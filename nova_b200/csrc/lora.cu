@@ -5,9 +5,9 @@
 // its adapter: memory at any length, and for single tokens the latency of the
 // chain x A^T -> h -> h B^T.  So one launch does both products: a cluster of 8
 // CTAs takes a tile of up to 16 or 64 rows, each CTA an eighth of K for the
-// first product; the partial sums (rows x rank, fp32) are exchanged through
-// distributed shared memory, added in CTA order, and each CTA then has all of
-// h for its eighth of N.  h is rounded to fp16 for the second product (2^-11
+// first product; of the partial sums (rows x rank, fp32) each CTA adds an
+// eighth, in CTA order, through distributed shared memory and hands the result
+// to all, and each then has all of h for its eighth of N.  h is rounded to fp16 for the second product (2^-11
 // of the adapter's term, which is added to base in fp32 before the one rounding
 // of the result).  Fragments of mma.sync m16n8k16 are read straight from
 // global memory: the contraction index is permuted so that a lane's operand
@@ -46,7 +46,7 @@ __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
 // RT: rank tiles of 8 (rank <= 8 RT).  MT: row tiles of 16.
 template <int RT, int MT>
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) lora_add_kernel(const Params p) {
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lora_add_kernel(const Params p) {
     constexpr int R = 8 * RT, TM = 16 * MT, KS = WARPS / MT;   // KS warps share a row tile's part of K
     constexpr int HP = R + 8;                                  // padded row of h
     extern __shared__ __align__(16) uint8_t smem[];
@@ -84,7 +84,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) lora_
         float acc[RT][4];
 #pragma unroll
         for (int j = 0; j < RT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        constexpr int U = RT <= 2 ? 4 : 1;
+        constexpr int U = RT <= 2 ? 4 : RT <= 8 ? 2 : 1;   // 128 registers hold so many chunks in flight
 #pragma unroll U
         for (int c = k0 + ks; c < k1; c += KS) {
             const int k = c * 32;
@@ -112,62 +112,94 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) lora_
         for (int w = 1; w < KS; ++w) s += red[w * TM * R + i];
         red[i] = s;
     }
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const float scale = p.scaling ? p.scaling[adapter] : 1.f;
-    for (int i = threadIdx.x; i < TM * R; i += THREADS) {
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < CLUSTER; ++w) s += cluster.map_shared_rank(red, w)[i];
-        hs[(i / R) * HP + i % R] = __float2half_rn(s * scale);
-    }
-    cluster.sync();     // hs is complete, and nobody reads this CTA's sums any more
-
-    // ---- out = base + h B^T over this CTA's part of N
+    // ---- out = base + h B^T over this CTA's part of N: 32 columns a warp, B read once for all rows of the tile.
+    // What the first product does not change is requested now, so that it arrives during the exchange.
     constexpr int S = RT / 2;                // steps of 16 along the rank
-    uint32_t hf[S][4];
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-        const uint2 lo = *reinterpret_cast<const uint2*>(hs + (mt * 16 + g) * HP + 16 * s + 4 * t);
-        const uint2 hi = *reinterpret_cast<const uint2*>(hs + (mt * 16 + g + 8) * HP + 16 * s + 4 * t);
-        hf[s][0] = lo.x; hf[s][1] = hi.x; hf[s][2] = lo.y; hf[s][3] = hi.y;
-    }
-    const int ra = row_of[mt * 16 + g], rb = row_of[mt * 16 + g + 8];
     const __half* bw = p.b + int64_t(adapter) * p.n * p.max_rank + 4 * t;
-    for (int nb = nb0 + ks; nb < nb1; nb += KS) {
+    uint4 ba[MT], bb[MT];
+    uint2 w[4][S];
+    auto load = [&](int nb) {
         const int n0 = nb * 32, col = n0 + 8 * t;
         const bool in = col < p.n;
-        const uint4 ba = in && ra >= 0 ? *reinterpret_cast<const uint4*>(p.base + ra * p.base_stride + col) : zero4();
-        const uint4 bb = in && rb >= 0 ? *reinterpret_cast<const uint4*>(p.base + rb * p.base_stride + col) : zero4();
-        float acc[4][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int ra = row_of[m * 16 + g], rb = row_of[m * 16 + g + 8];
+            ba[m] = in && ra >= 0 ? *reinterpret_cast<const uint4*>(p.base + ra * p.base_stride + col) : zero4();
+            bb[m] = in && rb >= 0 ? *reinterpret_cast<const uint4*>(p.base + rb * p.base_stride + col) : zero4();
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
             const int c = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const int left = rank - (16 * s + 4 * t);      // entries of this rank that the lane's four hold
-                uint2 w = make_uint2(0u, 0u);
-                if (left > 0 && c < p.n) w = *reinterpret_cast<const uint2*>(bw + int64_t(c) * p.max_rank + 16 * s);
-                if (left < 4) {
-                    w.x = left >= 2 ? w.x : (left == 1 ? w.x & 0xFFFFu : 0u);
-                    w.y = left == 3 ? w.y & 0xFFFFu : 0u;
-                }
-                mma_16816(acc[j], hf[s][0], hf[s][1], hf[s][2], hf[s][3], w.x, w.y);
+                w[j][s] = make_uint2(0u, 0u);
+                if (rank > 16 * s + 4 * t && c < p.n) w[j][s] = *reinterpret_cast<const uint2*>(bw + int64_t(c) * p.max_rank + 16 * s);
             }
         }
-        if (!in) continue;
-        const uint32_t wa[4] = {ba.x, ba.y, ba.z, ba.w}, wb[4] = {bb.x, bb.y, bb.z, bb.w};
-        uint32_t oa[4], ob[4];
+    };
+    int nb = nb0 + warp;
+    if (nb < nb1) load(nb);
+
+    // ---- the clusters' partial sums: CTA i adds the i-th eighth of h, in CTA order, and hands it to every CTA
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const float scale = p.scaling ? p.scaling[adapter] : 1.f;
+    constexpr int SHARE = TM * R / CLUSTER / 2;      // pairs of elements
+    for (int i = threadIdx.x; i < SHARE; i += THREADS) {
+        const int at = cr * SHARE + i;
+        float2 v[CLUSTER];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&wa[j]));
-            const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&wb[j]));
-            oa[j] = pack_f16x2(fa.x + acc[j][0], fa.y + acc[j][1]);
-            ob[j] = pack_f16x2(fb.x + acc[j][2], fb.y + acc[j][3]);
+        for (int k = 0; k < CLUSTER; ++k) v[k] = reinterpret_cast<const float2*>(cluster.map_shared_rank(red, k))[at];
+        float2 s = v[0];
+#pragma unroll
+        for (int k = 1; k < CLUSTER; ++k) s = make_float2(s.x + v[k].x, s.y + v[k].y);
+        const __half2 h = __floats2half2_rn(s.x * scale, s.y * scale);
+        const int off = (2 * at / R) * HP + 2 * at % R;
+#pragma unroll
+        for (int k = 0; k < CLUSTER; ++k) *reinterpret_cast<__half2*>(cluster.map_shared_rank(hs, k) + off) = h;
+    }
+    cluster.sync();                          // h is complete everywhere; no CTA reads or writes another's memory from here
+
+    for (; nb < nb1; nb += WARPS) {
+        const int col = nb * 32 + 8 * t;
+        const bool in = col < p.n;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int left = rank - (16 * s + 4 * t);          // entries of this rank that the lane's four hold
+            if (left >= 4) continue;
+            const uint32_t mx = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u, my = left == 3 ? 0xFFFFu : 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j][s].x &= mx;
+                w[j][s].y &= my;
+            }
         }
-        if (ra >= 0) *reinterpret_cast<uint4*>(p.out + ra * p.out_stride + col) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
-        if (rb >= 0) *reinterpret_cast<uint4*>(p.out + rb * p.out_stride + col) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float acc[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const uint2 lo = *reinterpret_cast<const uint2*>(hs + (m * 16 + g) * HP + 16 * s + 4 * t);
+                const uint2 hi = *reinterpret_cast<const uint2*>(hs + (m * 16 + g + 8) * HP + 16 * s + 4 * t);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_16816(acc[j], lo.x, hi.x, lo.y, hi.y, w[j][s].x, w[j][s].y);
+            }
+            const uint32_t wa[4] = {ba[m].x, ba[m].y, ba[m].z, ba[m].w}, wb[4] = {bb[m].x, bb[m].y, bb[m].z, bb[m].w};
+            uint32_t oa[4], ob[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&wa[j]));
+                const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&wb[j]));
+                oa[j] = pack_f16x2(fa.x + acc[j][0], fa.y + acc[j][1]);
+                ob[j] = pack_f16x2(fb.x + acc[j][2], fb.y + acc[j][3]);
+            }
+            const int ra = row_of[m * 16 + g], rb = row_of[m * 16 + g + 8];
+            if (in && ra >= 0) *reinterpret_cast<uint4*>(p.out + ra * p.out_stride + col) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
+            if (in && rb >= 0) *reinterpret_cast<uint4*>(p.out + rb * p.out_stride + col) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+        }
+        if (nb + WARPS < nb1) load(nb + WARPS);
     }
 }
 

@@ -50,8 +50,9 @@ class LoraPlan:
         rows = np.argsort(of_row, kind="stable")
         values, first, n = np.unique(of_row[rows], return_index=True, return_counts=True)
         busy = n[values >= 0]
-        # 64-row tiles read an adapter's weights once per 64 rows; single tokens would leave them empty
-        self.tile_rows = 64 if len(busy) and busy.max() > 32 else 16
+        # 64-row tiles read an adapter's weights once per 64 rows; where they are too few for a GPU's SMs (8 CTAs
+        # each), or mostly empty, 16-row ones spread the work further
+        self.tile_rows = 64 if (-(-busy // 64)).sum() >= 16 and busy.mean() > 32 else 16
         tiles = []
         for v, f, m in zip(values.tolist(), first.tolist(), n.tolist()):
             r = int(rank[v]) if v >= 0 else 0

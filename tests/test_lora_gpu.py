@@ -53,6 +53,10 @@ CASES = [
     ([33, 100], [0, 1], [128, 77], 776, 200, 128),
     ([5, 90], [0, -1], [7], 4096, 2560, 16),
     ([300], [3], [8, 8, 8, 31], 264, 96, 40),
+    ([900, 77, 300], [0, 1, 2], [16, 9, 64], 136, 328, 64),
+    ([1000, 60], [0, 1], [128, 100], 96, 40, 128),
+    ([1030, 1], [1, 0], [8, 13], 72, 64, 16),
+    ([1100], [0], [30], 40, 104, 32),
     ([64, 64], [0, 1], [0, 16], 512, 256, 16),
 ]
 
@@ -130,12 +134,13 @@ def test_plan_gathers_rows_by_adapter():
     tiles = p.buffer[:4 * p.n_tiles].view(-1, 4).tolist()
     rows = p.buffer[4 * p.n_tiles:].tolist()
     of_row = np.repeat(which, tokens).tolist()
-    assert sorted(rows) == list(range(46)) and p.tile_rows == 64 and p.max_rank == 16
+    assert sorted(rows) == list(range(46)) and p.tile_rows == 16 and p.max_rank == 16
     for adapter, rank, first, n in tiles:
         assert 1 <= n <= p.tile_rows and rank == (ranks[adapter] if adapter >= 0 else 0)
         assert all(of_row[r] == adapter for r in rows[first:first + n])
     assert sum(t[3] for t in tiles) == 46
     assert LoraPlan([1] * 40, [0] * 20 + [1] * 20, [8, 8], device="cpu").tile_rows == 16
+    assert LoraPlan([700, 500], [0, 1], [8, 8], device="cpu").tile_rows == 64
 
 
 @pytest.mark.parametrize("args,message", [
