@@ -53,23 +53,28 @@ struct alignas(16) Vec {
     T v[VEC];
 };
 
+// Biases of a CTA's tokens up to this many go from lane to lane: each lane holds
+// one, and a warp takes those of its own tokens.  More go through shared memory.
+constexpr int FEW_BIASES = 64;
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) {
-    __shared__ __align__(16) float bias[CHUNK];
-    const int row = blockIdx.y;
+    __shared__ __align__(16) float bias_s[CHUNK];
+    const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31;
     const T* src = reinterpret_cast<const T*>(p.logits) + row * p.lstride;
     T* dst = reinterpret_cast<T*>(p.out) + row * p.ostride;
     const int16_t* hist = p.history ? p.history + row * p.hstride : nullptr;
     // Tokens before the row that its first vector would cover, and whether every pointer agrees on it.
-    const uintptr_t lead = hist ? reinterpret_cast<uintptr_t>(hist) / 2 % VEC : reinterpret_cast<uintptr_t>(src) / sizeof(T) % VEC;
+    const int lead = int(hist ? reinterpret_cast<uintptr_t>(hist) / 2 % VEC : reinterpret_cast<uintptr_t>(src) / sizeof(T) % VEC);
     const bool vec = (reinterpret_cast<uintptr_t>(src) - lead * sizeof(T)) % 16 == 0 &&
                      (reinterpret_cast<uintptr_t>(dst) - lead * sizeof(T)) % 16 == 0;
-    const int base = int(blockIdx.x) * CHUNK - int(lead);      // first token of this CTA
+    const int base = chunk * CHUNK - lead;                     // first token of this CTA
     if (base >= p.vocab) return;
     const int t0 = base + int(threadIdx.x) * VEC;
     const bool whole = vec && t0 >= 0 && t0 + VEC <= p.vocab;
     pdl_wait();
 
+    // loads that nothing waits for, all in flight
     Vec<T> x;
     Vec<int16_t> h;
 #pragma unroll
@@ -90,50 +95,69 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
                 if (hist) h.v[i] = hist[t0 + i];
             }
     }
-    // 8 mask bits of this thread's tokens (all set: no mask).
-    uint32_t keep = 0xFFu;
-    if (p.allowed) {
-        const int which = p.allowed_row ? p.allowed_row[row] : row;
-        if (which >= p.n_masks) {
-            keep = 0u;
-        } else if (which >= 0) {
-            const uint32_t* m = p.allowed + which * p.mask_stride;
-            const int f = max(t0, 0), words = (p.vocab + 31) / 32, w = f >> 5;
-            const uint32_t lo = w < words ? m[w] : 0u;
-            const uint32_t hi = (f & 31) > 32 - VEC && w + 1 < words ? m[w + 1] : 0u;
-            keep = __funnelshift_r(lo, hi, f & 31) << (f - t0);
-        }
+    int e0 = 0, e1 = 0;       // biases of this CTA's tokens: they lie in its list and, with a lead, in the one before
+    if (p.bias_off) {
+        const int* off = p.bias_off + int64_t(row) * p.chunks;
+        e0 = off[min(max(chunk - (lead > 0), 0), p.chunks)];
+        e1 = off[min(chunk + 1, p.chunks)];
     }
+    const int which = !p.allowed ? -1 : p.allowed_row ? p.allowed_row[row] : row;
     const float rep = p.repetition ? p.repetition[row] : 1.f;
     const float freq = p.frequency ? p.frequency[row] : 0.f;
     const float pres = p.presence ? p.presence[row] : 0.f;
-    // This CTA's biases: its tokens lie in bias lists blockIdx.x - 1 and blockIdx.x.
-    bool biased = false;
-    if (p.bias_off) {
-        const int* off = p.bias_off + int64_t(row) * p.chunks;
-        const int e0 = off[max(int(blockIdx.x) - (lead > 0), 0)], e1 = off[min(int(blockIdx.x) + 1, p.chunks)];
-        biased = e1 > e0;
-        if (biased) {
+    // 8 mask bits of this thread's tokens (all set: no mask)
+    uint32_t keep = 0xFFu;
+    if (which >= p.n_masks) {
+        keep = 0u;
+    } else if (which >= 0) {
+        const uint32_t* m = p.allowed + which * p.mask_stride;
+        const int f = max(t0, 0), words = (p.vocab + 31) / 32, w = f >> 5;
+        const uint32_t lo = w < words ? m[w] : 0u;
+        const uint32_t hi = (f & 31) > 32 - VEC && w + 1 < words ? m[w + 1] : 0u;
+        keep = __funnelshift_r(lo, hi, f & 31) << (f - t0);
+    }
+    float b[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) bias[i * THREADS + threadIdx.x] = 0.f;
-            __syncthreads();
-            for (int e = e0 + threadIdx.x; e < e1; e += THREADS) {
-                const int at = p.bias_token[e] - base;
-                if (at >= 0 && at < CHUNK) bias[at] = p.bias_value[e];
+    for (int i = 0; i < VEC; ++i) b[i] = 0.f;
+    const int count = e1 - e0;                                 // the same in the whole CTA
+    if (count > 0 && count <= FEW_BIASES) {
+        for (int e = e0; e < e1; e += 32) {
+            const bool have = e + lane < e1;
+            const int token = have ? p.bias_token[e + lane] : -1;
+            const float value = have ? p.bias_value[e + lane] : 0.f;
+            const int first = t0 - lane * VEC;                 // this warp's first token
+            unsigned mine = __ballot_sync(0xffffffffu, have && token >= first && token < first + 32 * VEC);
+            for (; mine; mine &= mine - 1) {
+                const int l = __ffs(mine) - 1, k = __shfl_sync(0xffffffffu, token, l) - t0;
+                const float v = __shfl_sync(0xffffffffu, value, l);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) b[i] = k == i ? v : b[i];
             }
-            __syncthreads();
         }
+    } else if (count > 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) bias_s[i * THREADS + threadIdx.x] = 0.f;
+        __syncthreads();
+        for (int e = e0 + threadIdx.x; e < e1; e += THREADS) {
+            const int at = p.bias_token[e] - base;
+            if (at >= 0 && at < CHUNK) bias_s[at] = p.bias_value[e];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) b[i] = bias_s[int(threadIdx.x) * VEC + i];
     }
     Vec<T> y;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         float v = to_float<T>(x.v[i]);
         const int hi = h.v[i];
-        if (hi) v = v > 0.f ? div_rn(v, rep) : v * rep;
-        const int times = hi & 0x7FFF;
-        v -= freq * float(times);
-        v -= times ? pres : 0.f;
-        if (biased) v += bias[int(threadIdx.x) * VEC + i];
+        if (hi) {
+            const int times = hi & 0x7FFF;
+            v = v > 0.f ? div_rn(v, rep) : v * rep;
+            v -= freq * float(times);
+            v -= times ? pres : 0.f;
+        }
+        v += b[i];
         y.v[i] = from_float<T>((keep >> i) & 1u ? v : -INFINITY);
     }
     if (whole) {
@@ -217,10 +241,8 @@ extern "C" int nova_adjust_logits(const nova_logits_args* a, void* stream) {
     p.vocab = int(a->vocab);
     p.chunks = int((a->vocab + CHUNK - 1) / CHUNK);
     const dim3 grid(unsigned((a->vocab + VEC - 1 + CHUNK - 1) / CHUNK), unsigned(a->rows));
-    if (a->logits_fp32)
-        launch(adjust_logits_kernel<float>, grid, dim3(THREADS), 0, static_cast<cudaStream_t>(stream), p);
-    else
-        launch(adjust_logits_kernel<__half>, grid, dim3(THREADS), 0, static_cast<cudaStream_t>(stream), p);
+    launch(a->logits_fp32 ? adjust_logits_kernel<float> : adjust_logits_kernel<__half>, grid, dim3(THREADS), 0,
+           static_cast<cudaStream_t>(stream), p);
     return check_launch("adjust logits");
 }
 

@@ -13,7 +13,8 @@ namespace nova {
 namespace paged {
 
 constexpr int THREADS = 256;
-constexpr int PAIRS = 64;       // (token, query head) rows per CTA of the q part
+constexpr int QH = 4;           // query heads of one token that a half warp takes
+constexpr int QITEMS = 16;      // such items per CTA of the q part
 
 struct AppendParams {
     const __half* qkv;
@@ -28,12 +29,9 @@ struct AppendParams {
     uint8_t* codes;
     __half* scales;
     __half* tails;
-    const Seq* seqs;
-    const int* pages;
     const int* pos;
     const Block* blocks;
-    int64_t tokens;
-    int n_write, q_heads, kv_heads;
+    int tokens, n_write, q_heads, kv_heads;
     int q_ctas;
 };
 
@@ -67,30 +65,26 @@ __device__ __forceinline__ Row8 pack(const float (&x)[8]) {
     return r;
 }
 
-// RMSNorm (w != NULL) and RoPE (cos != NULL) of one row held by a half warp,
+// RMSNorm (norm; w: the weights) and RoPE (rope) of one row held by a half warp,
 // in fp32 and rounded to fp16 once: the reference rounds after the norm, after
 // the weight and after each rotation product, which costs half a unit in the
 // last place each time and nothing here needs its bits.
-__device__ __forceinline__ Row8 norm_rope_row(const Row8& in, const __half* w, const __half* cos, const __half* sin,
-                                              int64_t pos, float eps, int c) {
+__device__ __forceinline__ Row8 norm_rope_row(const Row8& in, bool norm, const float (&w)[8], bool rope,
+                                              const float (&cs)[8], const float (&sn)[8], float eps) {
     float x[8];
     unpack(in, x);
-    if (w) {
+    if (norm) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        const float r = rsqrt_ieee(ss * (1.0f / D) + eps);
-        float g[8];
-        unpack(load_row(w, c), g);
+        const float r = rsqrtf(ss * (1.0f / D) + eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= r * g[i];
+        for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
     }
-    if (cos) {
-        float cs[8], sn[8], y[8];
-        unpack(load_row(cos + pos * D, c), cs);
-        unpack(load_row(sin + pos * D, c), sn);
+    if (rope) {
+        float y[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             y[i] = x[i] * cs[i] - x[i + 4] * sn[i];
@@ -102,6 +96,18 @@ __device__ __forceinline__ Row8 norm_rope_row(const Row8& in, const __half* w, c
     return pack(x);
 }
 
+// Code of a value: rint((v - low) / step) of the framework's quantizer, bit for
+// bit.  The quotient by the reciprocal is within 4e-5 of the divided one (it is
+// at most 255), so only one that close to a tie is divided; adding 1.5 * 2^23
+// rounds to the nearest even integer and leaves it in the low mantissa bits.
+__device__ __forceinline__ uint32_t code_of(float v, float low, float step, float inv) {
+    constexpr float MAGIC = 12582912.0f;
+    const float d = v - low, q = d * inv;
+    float t = __fadd_rn(q, MAGIC);
+    if (fabsf(q - __fadd_rn(t, -MAGIC)) > 0.4999f) t = __fadd_rn(div_rn(d, step), MAGIC);
+    return __float_as_uint(t) & 0xFFu;
+}
+
 __device__ __forceinline__ uint32_t hmin2u(uint32_t a, uint32_t b) {
     __half2 r = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&r);
@@ -111,65 +117,77 @@ __device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
     return *reinterpret_cast<uint32_t*>(&r);
 }
 
-// CTAs [0, q_ctas): 64 (token, query head) rows each.  The others: K or V of
+// CTAs [0, q_ctas): 16 groups of 4 query heads of a token each.  The others: K or V of
 // one (touched block, KV head).  A block that the step completes is held in
 // registers (4 tokens x 8 channels a thread), its minimum and maximum per
 // channel go through shared memory once, and codes leave as 4-byte pieces of
 // 128-byte rows; a block that stays open only gets its new rows.
-__global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(THREADS, 4) paged_append_kernel(const AppendParams p) {
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 15, part = warp * 2 + (lane >> 4);
+    const Row8 zero{make_uint2(0u, 0u), make_uint2(0u, 0u)};
     if (int(blockIdx.x) < p.q_ctas) {
-        const int64_t base = int64_t(blockIdx.x) * PAIRS, n = p.tokens * p.q_heads;
-        Row8 r[4];
-        int64_t tok[4];
-        int head[4];
+        const int groups = (p.q_heads + QH - 1) / QH, n = p.tokens * groups;
+        const int at = int(blockIdx.x) * QITEMS + part, use = min(at, n - 1);   // past the end: the last one, unstored
+        const int tok = use / groups, h0 = (use - tok * groups) * QH;
+        const __half* src = p.qkv + tok * p.qkv_stride + h0 * D;
+        Row8 r[QH];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t at = min(base + i * 16 + part, n - 1);   // a row past the end repeats the last one, unstored
-            tok[i] = at / p.q_heads;
-            head[i] = int(at - tok[i] * p.q_heads);
-            r[i] = load_row(p.qkv + tok[i] * p.qkv_stride + head[i] * D, c);
-        }
+        for (int i = 0; i < QH; ++i) r[i] = h0 + i < p.q_heads ? load_row(src + i * D, c) : zero;
+        float w[8], cs[8], sn[8];
+        unpack(p.wq ? load_row(p.wq, c) : zero, w);
+        const int64_t pos = p.cos ? int64_t(p.pos[tok]) * D : 0;
+        unpack(p.cos ? load_row(p.cos + pos, c) : zero, cs);
+        unpack(p.cos ? load_row(p.sin + pos, c) : zero, sn);
+        __half* dst = p.q + tok * p.q_stride + h0 * D;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            r[i] = norm_rope_row(r[i], p.wq, p.cos, p.sin, p.cos ? p.pos[tok[i]] : 0, p.eps, c);
-            if (base + i * 16 + part < n) store_row(p.q + tok[i] * p.q_stride + head[i] * D, c, r[i]);
+        for (int i = 0; i < QH; ++i) {
+            const Row8 y = norm_rope_row(r[i], p.wq, w, p.cos, cs, sn, p.eps);
+            if (at < n && h0 + i < p.q_heads) store_row(dst + i * D, c, y);
         }
         return;
     }
     const int item = (blockIdx.x - p.q_ctas) / (2 * p.kv_heads), hj = (blockIdx.x - p.q_ctas) % (2 * p.kv_heads);
     const int head = hj >> 1, j = hj & 1;
     const Block blk = p.blocks[item];
-    const Seq s = p.seqs[blk.seq];
-    const int first = s.kv_len - s.q_len, b0 = blk.blk * PT;
-    const bool closes = b0 + PT <= s.kv_len;
-    const __half* src = p.qkv + (p.q_heads + j * p.kv_heads + head) * int64_t(D);
-    const __half* old = p.tails + half_off(s.tail_in, p.kv_heads, head, j);
-    Row8 r[4];
+    const int b0 = blk.blk * PT;
+    const bool closes = blk.page >= 0;
+    const __half* src = p.qkv + (p.q_heads + j * p.kv_heads + head) * int64_t(D) + int64_t(blk.row - blk.first) * p.qkv_stride;
+    const __half* old = p.tails + half_off(blk.tail_in, p.kv_heads, head, j);
+    Row8 r[4], cs[4], sn[4];
+    bool fresh[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int slot = i * 16 + part, pos = b0 + slot;
-        r[i] = Row8{make_uint2(0u, 0u), make_uint2(0u, 0u)};
-        if (pos >= first && pos < s.kv_len) r[i] = load_row(src + int64_t(s.q_start + pos - first) * p.qkv_stride, c);
-        else if (closes) r[i] = load_row(old + slot * D, c);   // pos < first: the open page's token
+        fresh[i] = pos >= blk.first && pos < blk.kv_len;
+        r[i] = cs[i] = sn[i] = zero;
+        if (fresh[i]) {
+            r[i] = load_row(src + int64_t(pos) * p.qkv_stride, c);
+            if (j == 0 && p.cos) {
+                cs[i] = load_row(p.cos + int64_t(pos) * D, c);
+                sn[i] = load_row(p.sin + int64_t(pos) * D, c);
+            }
+        } else if (closes) {                                   // before `first`: the open page's token
+            r[i] = load_row(old + slot * D, c);
+        }
     }
     if (j == 0) {
+        float w[8], cf[8], sf[8];
+        unpack(p.wk ? load_row(p.wk, c) : zero, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int pos = b0 + i * 16 + part;
-            const bool fresh = pos >= first && pos < s.kv_len;
-            const Row8 y = norm_rope_row(r[i], p.wk, p.cos, p.sin, fresh ? pos : first, p.eps, c);
-            if (fresh) r[i] = y;
+            if (!__any_sync(0xffffffffu, fresh[i])) continue;
+            unpack(cs[i], cf);
+            unpack(sn[i], sf);
+            const Row8 y = norm_rope_row(r[i], p.wk, w, p.cos, cf, sf, p.eps);
+            if (fresh[i]) r[i] = y;
         }
     }
     if (!closes) {
-        __half* dst = p.tails + half_off(s.tail_out, p.kv_heads, head, j);
+        __half* dst = p.tails + half_off(blk.tail_out, p.kv_heads, head, j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int slot = i * 16 + part, pos = b0 + slot;
-            if (pos >= first && pos < s.kv_len) store_row(dst + slot * D, c, r[i]);
-        }
+        for (int i = 0; i < 4; ++i)
+            if (fresh[i]) store_row(dst + (i * 16 + part) * D, c, r[i]);
         return;
     }
     __shared__ __align__(8) uint32_t lims[8][2][D / 2];   // per warp: minima, maxima of each channel pair
@@ -211,7 +229,10 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendParam
         step[2 * k] = fmaxf(div_rn(b.x - a.x, 255.0f), 1e-8f);
         step[2 * k + 1] = fmaxf(div_rn(b.y - a.y, 255.0f), 1e-8f);
     }
-    const int page = p.pages[s.page_off + blk.blk];
+    const int page = blk.page;
+    float inv[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) inv[k] = div_rn(1.0f, step[k]);
     uint8_t* codes = p.codes + half_off(page, p.kv_heads, head, j);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -219,10 +240,7 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendParam
         unpack(r[i], x);
         uint32_t w[2] = {0u, 0u};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float v = fminf(fmaxf(rintf(div_rn(x[k] - low[k], step[k])), 0.0f), 255.0f);
-            w[k >> 2] |= uint32_t(v) << (8 * (k & 3));
-        }
+        for (int k = 0; k < 8; ++k) w[k >> 2] |= code_of(x[k], low[k], step[k], inv[k]) << (8 * (k & 3));
         uint8_t* row = codes + (i * 16 + part) * D;
         *reinterpret_cast<uint32_t*>(row + 4 * c) = w[0];
         *reinterpret_cast<uint32_t*>(row + 64 + 4 * c) = w[1];
@@ -236,40 +254,41 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendParam
 
 // K or V of one (block, KV head) as fp16 rows.
 __global__ void __launch_bounds__(THREADS)
-    paged_read_kernel(const uint8_t* codes, const __half* scales, const __half* tails, const Seq* seqs,
-                      const int* pages, const Block* blocks, int kv_heads, __half* k_out, __half* v_out) {
+    paged_read_kernel(const uint8_t* codes, const __half* scales, const __half* tails, const Block* blocks, int kv_heads,
+                      __half* k_out, __half* v_out) {
     pdl_wait();
     const int lane = threadIdx.x & 31, c = lane & 15, part = (threadIdx.x >> 5) * 2 + (lane >> 4);
     const int item = blockIdx.x / (2 * kv_heads), hj = blockIdx.x % (2 * kv_heads), head = hj >> 1, j = hj & 1;
     const Block blk = blocks[item];
-    const Seq s = seqs[blk.seq];
-    const int b0 = blk.blk * PT, from = blk.pad;
-    __half* out = (j ? v_out : k_out) + head * D;
+    const int b0 = blk.blk * PT, from = blk.first - b0;
     const int64_t stride = int64_t(kv_heads) * D;
-    if (b0 + PT > s.kv_len) {
-        const __half* src = tails + half_off(s.tail_out, kv_heads, head, j);
+    __half* out = (j ? v_out : k_out) + head * D + int64_t(blk.row - blk.first + b0) * stride;   // of the block's slot 0
+    if (blk.page < 0) {
+        const __half* src = tails + half_off(blk.tail_out, kv_heads, head, j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int slot = i * 16 + part;
-            if (slot >= from && b0 + slot < s.kv_len)
-                store_row(out + (int64_t(blk.row) + slot - from) * stride, c, load_row(src + slot * D, c));
+            if (slot >= from && b0 + slot < blk.kv_len) store_row(out + slot * stride, c, load_row(src + slot * D, c));
         }
         return;
     }
-    const int page = pages[s.page_off + blk.blk];
-    const uint8_t* src = codes + half_off(page, kv_heads, head, j);
-    const __half* sc = scales + ((int64_t(page) * kv_heads + head) * 4 + 2 * j) * D;
+    const uint8_t* src = codes + half_off(blk.page, kv_heads, head, j);
+    const __half* sc = scales + ((int64_t(blk.page) * kv_heads + head) * 4 + 2 * j) * D;
     const Row8 mn = load_row(sc, c), st = load_row(sc + D, c);
+    uint32_t a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a[i] = *reinterpret_cast<const uint32_t*>(src + (i * 16 + part) * D + 4 * c);
+        b[i] = *reinterpret_cast<const uint32_t*>(src + (i * 16 + part) * D + 64 + 4 * c);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int slot = i * 16 + part;
         if (slot < from) continue;
-        const uint32_t a = *reinterpret_cast<const uint32_t*>(src + slot * D + 4 * c);
-        const uint32_t b = *reinterpret_cast<const uint32_t*>(src + slot * D + 64 + 4 * c);
         Row8 r;   // fp16(code * step + min), one rounding
-        r.lo = make_uint2(hfma2(u8x2_lo_to_f16x2(a), st.lo.x, mn.lo.x), hfma2(u8x2_hi_to_f16x2(a), st.lo.y, mn.lo.y));
-        r.hi = make_uint2(hfma2(u8x2_lo_to_f16x2(b), st.hi.x, mn.hi.x), hfma2(u8x2_hi_to_f16x2(b), st.hi.y, mn.hi.y));
-        store_row(out + (int64_t(blk.row) + slot - from) * stride, c, r);
+        r.lo = make_uint2(hfma2(u8x2_lo_to_f16x2(a[i]), st.lo.x, mn.lo.x), hfma2(u8x2_hi_to_f16x2(a[i]), st.lo.y, mn.lo.y));
+        r.hi = make_uint2(hfma2(u8x2_lo_to_f16x2(b[i]), st.hi.x, mn.hi.x), hfma2(u8x2_hi_to_f16x2(b[i]), st.hi.y, mn.hi.y));
+        store_row(out + slot * stride, c, r);
     }
 }
 
@@ -329,15 +348,13 @@ extern "C" int nova_paged_append(const nova_paged_append_args* a, const nova_pag
     p.codes = static_cast<uint8_t*>(a->codes);
     p.scales = static_cast<__half*>(a->scales);
     p.tails = static_cast<__half*>(a->tails);
-    p.seqs = reinterpret_cast<const Seq*>(a->plan + info->seq_off);
-    p.pages = a->plan + info->page_off;
     p.pos = a->plan + info->pos_off;
     p.blocks = reinterpret_cast<const Block*>(a->plan + info->write_off);
-    p.tokens = info->tokens;
+    p.tokens = int(info->tokens);
     p.n_write = int(info->n_write);
     p.q_heads = int(info->q_heads);
     p.kv_heads = int(info->kv_heads);
-    const int64_t q_ctas = (info->tokens * info->q_heads + PAIRS - 1) / PAIRS;
+    const int64_t q_ctas = (info->tokens * ((info->q_heads + QH - 1) / QH) + QITEMS - 1) / QITEMS;
     const int64_t grid = q_ctas + info->n_write * 2 * info->kv_heads;
     if (grid >= (1ll << 31)) return fail(NOVA_ERR_UNSUPPORTED, "paged append: too many tokens in one step");
     p.q_ctas = int(q_ctas);
@@ -357,7 +374,6 @@ extern "C" int nova_paged_read(const void* codes, const void* scales, const void
     if (grid >= (1ll << 31)) return fail(NOVA_ERR_UNSUPPORTED, "paged read: too many rows in one call");
     launch(paged_read_kernel, dim3(unsigned(grid)), dim3(THREADS), 0, static_cast<cudaStream_t>(stream),
            static_cast<const uint8_t*>(codes), static_cast<const __half*>(scales), static_cast<const __half*>(tails),
-           reinterpret_cast<const Seq*>(plan + info->seq_off), static_cast<const int*>(plan + info->page_off),
            reinterpret_cast<const Block*>(plan + info->read_off), int(info->kv_heads), static_cast<__half*>(k_out),
            static_cast<__half*>(v_out));
     return check_launch("paged read");

@@ -16,6 +16,7 @@ struct Seq {                    // one request
 };
 struct RowsItem {               // few query rows x a range of 64-token blocks
     int seq, row0, nrows, blk0, blk1, part0, split, n_splits;
+    int q_start, start, kv_len, page_off, tail, pad0, pad1, pad2;   // the request's: position of its first new token, ...
 };
 struct TileSeg {                // many query rows (up to 256) x a range of blocks; part < 0: the whole tile
     int seq, head, row0, nrows, blk0, blk1, part, q_start;
@@ -25,7 +26,8 @@ struct TileJoin {               // a tile whose segments left partials
     int seq, head, row0, nrows, part0, n_parts, pad0, pad1;
 };
 struct Block {                  // one 64-token block of a request (write and read lists)
-    int seq, blk, row, pad;     // row: read list only, the output row of the block's first copied position
+    int blk, first, kv_len, row;         // row: token row of position `first`, the first new (written) or copied (read) one
+    int tail_in, tail_out, page, pad;    // page: -1 while the block is open
 };
 
 constexpr int ROWS_MAX = 16;    // query rows of one KV head that the few-rows kernel takes per tile

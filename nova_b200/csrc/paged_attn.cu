@@ -43,7 +43,6 @@ struct Params {
     __half* out;
     int64_t o_t, o_h;
     float* lse;
-    const Seq* seqs;
     const int* pages;
     const RowsItem* items;
     int* err;
@@ -124,13 +123,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
     pdl_wait();
 
     const RowsItem it = p.items[blockIdx.x];
-    const Seq s = p.seqs[it.seq];
-    const int start = s.kv_len - s.q_len;
-    const int n_full = s.kv_len / PT;      // blocks past this one are the open page
+    const int start = it.start;
+    const int n_full = it.kv_len / PT;      // blocks past this one are the open page
 
     auto issue = [&](int blk, int j) {     // one lane: K (j = 0) or V half of a page
         uint64_t* bar = j ? bar_v : bar_k;
-        const int64_t ph = int64_t(p.pages[s.page_off + blk]) * p.kv_heads + head;
+        const int64_t ph = int64_t(p.pages[it.page_off + blk]) * p.kv_heads + head;
         mbar_arrive_expect_tx(bar, TX_HALF);
         tma_load_2d(stage + j * 8192, &tm, 0, int((ph * 2 + j) * PT), bar);
         bulk_g2s(stage + SC + j * 512, p.scales + (ph * 4 + 2 * j) * D, 512, bar);
@@ -155,7 +153,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
         const int r = HL ? (g & 3) : n * 8 + g;
         if (r < it.nrows) {
             const int row = it.row0 + r, tok = row / p.gq;
-            const __half* qp = p.q + int64_t(s.q_start + tok) * p.q_t + int64_t(head * p.gq + row - tok * p.gq) * p.q_h + 32 * t;
+            const __half* qp = p.q + int64_t(it.q_start + tok) * p.q_t + int64_t(head * p.gq + row - tok * p.gq) * p.q_h + 32 * t;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * i);
@@ -309,10 +307,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
     // The open page, 16 fp16 tokens at a time (one tile per warp), by the item that holds its block.
     if (ok && it.blk1 > n_full && it.blk0 <= n_full) {
         const int r0 = 16 * warp + g, base = n_full * PT;
-        if (base + 16 * warp < s.kv_len) {
-            const __half* tk = p.tails + half_off(s.tail_out, p.kv_heads, head, 0);
+        if (base + 16 * warp < it.kv_len) {
+            const __half* tk = p.tails + half_off(it.tail, p.kv_heads, head, 0);
             const __half* tv = tk + HALF_ROW;
-            const bool live0 = base + r0 < s.kv_len, live1 = base + r0 + 8 < s.kv_len;
+            const bool live0 = base + r0 < it.kv_len, live1 = base + r0 + 8 < it.kv_len;
             float x[NC][2];
             {
                 uint32_t k0[16], k1[16];
@@ -345,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-                const bool in = base + tok[k] < s.kv_len;   // a slot that holds no token may hold anything
+                const bool in = base + tok[k] < it.kv_len;   // a slot that holds no token may hold anything
                 const uint4 a = in ? *reinterpret_cast<const uint4*>(tv + tok[k] * D + 16 * g) : z;
                 const uint4 b = in ? *reinterpret_cast<const uint4*>(tv + tok[k] * D + 16 * g + 8) : z;
                 v[k][0] = a.x; v[k][1] = a.y; v[k][2] = a.z; v[k][3] = a.w;
@@ -399,9 +397,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
         const int row = it.row0 + r, tok = row / p.gq, qh = head * p.gq + row - tok * p.gq;
         const float inv = L > 0.f ? 1.0f / L : 0.f;
         const uint2 h = make_uint2(pack_f16x2(o.x * inv, o.y * inv), pack_f16x2(o.z * inv, o.w * inv));
-        *reinterpret_cast<uint2*>(p.out + int64_t(s.q_start + tok) * p.o_t + int64_t(qh) * p.o_h + d0) = h;
+        *reinterpret_cast<uint2*>(p.out + int64_t(it.q_start + tok) * p.o_t + int64_t(qh) * p.o_h + d0) = h;
         if (p.lse && lane == 0)
-            p.lse[int64_t(s.q_start + tok) * p.q_heads + qh] =
+            p.lse[int64_t(it.q_start + tok) * p.q_heads + qh] =
                 L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
     };
     const int64_t slot = (int64_t(it.part0) * p.kv_heads + head * int64_t(it.n_splits));
@@ -524,7 +522,6 @@ extern "C" int nova_paged_attention(const nova_paged_attn_args* a, const nova_pa
     p.o_t = a->o_t_stride;
     p.o_h = a->o_h_stride;
     p.lse = static_cast<float*>(a->lse);
-    p.seqs = reinterpret_cast<const Seq*>(a->plan + info->seq_off);
     p.pages = a->plan + info->page_off;
     p.items = reinterpret_cast<const RowsItem*>(a->plan + s.rows_off);
     p.q_heads = int(info->q_heads);

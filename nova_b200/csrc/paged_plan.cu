@@ -97,10 +97,13 @@ void seen_blocks(const nova_paged_plan_args& a, int64_t i, int64_t row0, int64_t
 // per 256 rows in the tensor-core kernel.
 bool few_rows(const nova_paged_plan_args& a, int64_t i) { return a.q_lens[i] * (a.q_heads / a.kv_heads) <= ROWS_MAX; }
 
-// Work list of the few-rows kernel: every tile's blocks cut into splits.
-// A split is at least one block per warp (4); enough of them that the resident
-// CTAs (3 per SM) are filled about four times over, which evens out ragged
-// lengths; and at most 32 per tile, so that joining them stays short.
+// Work list of the few-rows kernel: every tile's blocks cut into splits of at
+// least one block per warp (4), at most 32 per tile so that joining them stays
+// short.  A CTA costs a few blocks' time to start and to join, so where splits
+// of up to 48 blocks let all CTAs be resident at once (3 per SM) the smallest
+// such size is taken; 16 requests of 8191 tokens: 70 us, 76 in splits of 16.
+// Beyond that about four times as many CTAs as are resident even out ragged
+// lengths (32 requests of 8000 to 32768 tokens: 225 us, 260 in one wave).
 void rows_schedule(Builder& b, nova_paged_schedule& s) {
     const nova_paged_plan_args& a = b.a;
     const int64_t gq = a.q_heads / a.kv_heads;
@@ -108,16 +111,26 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
     for (int64_t i = 0; i < a.seqs; ++i)
         if (few_rows(a, i)) most = std::max(most, a.q_lens[i] * gq);
     s.rows_per_tile = most <= 4 ? 4 : most <= 8 ? 8 : ROWS_MAX;
+    std::vector<int64_t> tiles;                // blocks of each tile
     for (int64_t i = 0; i < a.seqs; ++i)
         for (int64_t r = 0; few_rows(a, i) && r < a.q_lens[i] * gq; r += s.rows_per_tile) {
             int64_t b0, b1;
             seen_blocks(a, i, r, std::min(s.rows_per_tile, a.q_lens[i] * gq - r), s.window, &b0, &b1);
+            tiles.push_back(b1 - b0);
             total += b1 - b0;
         }
-    int64_t chunk = std::max<int64_t>(4, total * a.kv_heads / (a.sms * 3 * 4) / 4 * 4);
+    const int64_t resident = a.sms * 3;
+    int64_t chunk = 4;
+    for (; chunk <= 48; chunk += 4) {
+        int64_t ctas = 0;
+        for (int64_t n : tiles) ctas += (n + chunk - 1) / chunk * a.kv_heads;
+        if (ctas <= resident) break;
+    }
+    if (chunk > 48) chunk = std::max<int64_t>(16, total * a.kv_heads / (resident * 4) / 4 * 4);
     s.rows_off = b.at();
     int64_t& parts = s.n_parts;
-    for (int64_t i = 0; i < a.seqs; ++i)
+    int64_t q_start = 0;
+    for (int64_t i = 0; i < a.seqs; q_start += a.q_lens[i++])
         for (int64_t r = 0; few_rows(a, i) && r < a.q_lens[i] * gq; r += s.rows_per_tile) {
             const int64_t n = std::min(s.rows_per_tile, a.q_lens[i] * gq - r);
             int64_t b0, b1;
@@ -126,7 +139,9 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
             const int64_t splits = (b1 - b0 + c - 1) / c;
             for (int64_t k = 0; k < splits; ++k) {
                 RowsItem it{int(i), int(r), int(n), int(b0 + k * c), int(std::min(b1, b0 + (k + 1) * c)),
-                            splits > 1 ? int(parts) : -1, int(k), int(splits)};
+                            splits > 1 ? int(parts) : -1, int(k), int(splits), int(q_start),
+                            int(a.kv_lens[i] - a.q_lens[i]), int(a.kv_lens[i]), int(a.page_off[i]),
+                            a.kv_lens[i] % PT ? int(a.tail_out[i]) : 0, 0, 0, 0};
                 b.put(it);
                 ++s.n_rows;
             }
@@ -240,21 +255,23 @@ extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, i
         for (int64_t i = 0; i < a.seqs; ++i)
             for (int64_t j = a.kv_lens[i] - a.q_lens[i]; j < a.kv_lens[i]; ++j) b.v.push_back(int32_t(j));
         info->write_off = b.at();
-        for (int64_t i = 0; i < a.seqs; ++i)
-            if (a.q_lens[i])
-                for (int64_t g = (a.kv_lens[i] - a.q_lens[i]) / PT; g * PT < a.kv_lens[i]; ++g) {
-                    b.put(Block{int(i), int(g), 0, 0});
-                    ++info->n_write;
-                }
+        int64_t row = 0;
+        auto block = [&](int64_t i, int64_t g, int64_t first, int64_t out_row) {
+            const int64_t kv = a.kv_lens[i], start = kv - a.q_lens[i];
+            const bool full = (g + 1) * PT <= kv;
+            return Block{int(g), int(first), int(kv), int(out_row), start % PT ? int(a.tail_in[i]) : 0,
+                         kv % PT ? int(a.tail_out[i]) : 0, full ? int(a.pages[a.page_off[i] + g]) : -1, 0};
+        };
+        for (int64_t i = 0; i < a.seqs; row += a.q_lens[i++]) {
+            const int64_t start = a.kv_lens[i] - a.q_lens[i];
+            for (int64_t g = start / PT; a.q_lens[i] && g * PT < a.kv_lens[i]; ++g, ++info->n_write)
+                b.put(block(i, g, start, row));
+        }
         info->read_off = b.at();
         for (int64_t i = 0; i < a.seqs; ++i) {
-            const int64_t from = a.read_from ? a.read_from[i] : (a.kv_lens[i] - a.q_lens[i]) / PT * PT;
-            for (int64_t g = from / PT; from < a.kv_lens[i] && g * PT < a.kv_lens[i]; ++g) {
-                const int64_t first = std::max(from, g * PT);
-                b.put(Block{int(i), int(g), int(info->read_rows), int(first - g * PT)});
-                info->read_rows += std::min((g + 1) * PT, a.kv_lens[i]) - first;
-                ++info->n_read;
-            }
+            const int64_t kv = a.kv_lens[i], from = a.read_from ? a.read_from[i] : (kv - a.q_lens[i]) / PT * PT;
+            for (int64_t g = from / PT; from < kv && g * PT < kv; ++g, ++info->n_read) b.put(block(i, g, from, info->read_rows));
+            info->read_rows += kv - from;
         }
         info->n_windows = a.n_windows;
         for (int64_t w = 0; w < a.n_windows; ++w) {

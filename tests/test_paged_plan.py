@@ -24,7 +24,7 @@ def make(q, kv, hq=8, hkv=2, **kw):
 
 def rows_items(plan, w=0):
     s = plan.info.sched[w]
-    return plan.host[s.rows_off:s.rows_off + 8 * s.n_rows].reshape(-1, 8)
+    return plan.host[s.rows_off:s.rows_off + 16 * s.n_rows].reshape(-1, 16)
 
 
 def test_records_and_lists():
@@ -35,20 +35,24 @@ def test_records_and_lists():
     assert p.tokens == 106
     pos = p.host[i.pos_off:i.pos_off + 106]
     assert pos.tolist() == [*range(5), 129, *range(200, 300)]
-    write = p.host[i.write_off:i.write_off + 4 * i.n_write].reshape(-1, 4)
-    assert write[:, :2].tolist() == [[0, 0], [1, 2], [3, 3], [3, 4]]
+    write = p.host[i.write_off:i.write_off + 8 * i.n_write].reshape(-1, 8)
+    # block, first new position, length, its token row, tail before and after, page (-1: stays open)
+    assert write[:, :7].tolist() == [[0, 0, 5, 0, 0, 0, -1], [2, 129, 130, 5, 2, 2, -1], [3, 200, 300, 6, 6, 7, 6],
+                                     [4, 200, 300, 6, 6, 7, -1]]
     assert p.read_rows == 5 + 2 + 0 + (300 - 192)
 
 
 def test_read_from():
     p = make([1, 1, 1], [200, 70, 1], read_from=[0, 70, 0])
     i = p.info
-    read = p.host[i.read_off:i.read_off + 4 * i.n_read].reshape(-1, 4)
+    read = p.host[i.read_off:i.read_off + 8 * i.n_read].reshape(-1, 8)
     assert p.read_rows == 201
-    assert read.tolist() == [[0, 0, 0, 0], [0, 1, 64, 0], [0, 2, 128, 0], [0, 3, 192, 0], [2, 0, 200, 0]]
+    # block, first copied position, length, its output row
+    assert read[:, :4].tolist() == [[0, 0, 200, 0], [1, 0, 200, 0], [2, 0, 200, 0], [3, 0, 200, 0], [0, 0, 1, 200]]
     p = make([1], [200], read_from=[100])
-    read = p.host[p.info.read_off:p.info.read_off + 4 * p.info.n_read].reshape(-1, 4)
-    assert p.read_rows == 100 and read.tolist() == [[0, 1, 0, 36], [0, 2, 28, 0], [0, 3, 92, 0]]
+    read = p.host[p.info.read_off:p.info.read_off + 8 * p.info.n_read].reshape(-1, 8)
+    assert p.read_rows == 100
+    assert read[:, :4].tolist() == [[1, 100, 200, 0], [2, 100, 200, 0], [3, 100, 200, 0]]
 
 
 @pytest.mark.parametrize("window", [0, 1, 63, 200])
@@ -61,7 +65,9 @@ def test_every_row_sees_its_blocks_once(hq, hkv, window):
     p = make(q, kv, hq, hkv, windows=(window,))
     gq = hq // hkv
     seen = {}
-    for seq, row0, nrows, b0, b1, part0, split, n in rows_items(p).tolist():
+    for seq, row0, nrows, b0, b1, part0, split, n, q_start, start, kv_len, page_off, tail, *_ in rows_items(p).tolist():
+        assert (q_start, start, kv_len) == (sum(q[:seq]), kv[seq] - q[seq], kv[seq])
+        assert page_off == sum(n // PAGE for n in kv[:seq]) and (not kv_len % PAGE or tail == p.tail_out[seq])
         assert 0 <= split < n and (part0 < 0) == (n == 1) and b1 > b0 and nrows >= 1
         for r in range(row0, row0 + nrows):
             seen.setdefault((seq, r), []).extend(range(b0, b1))
