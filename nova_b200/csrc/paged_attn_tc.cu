@@ -356,29 +356,36 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
         const uint32_t s_addr = tmem + S_COL + half * 128 + lanes, o_addr = tmem + O_COL + half * 128 + lanes;
         uint32_t sc = 0, oc = 0;       // steps and segments of this half so far
         bool ok = true;
-        for (int sg = seg0; sg < seg1 && ok; ++sg) {
+        // First of the segments from sg on that has rows in this half.
+        auto next_seg = [&](int sg) {
+            while (sg < seg1 && p.segs[sg].nrows <= half * 128) ++sg;
+            return sg;
+        };
+        // This thread's row of a segment's Q into shared memory (rows past the segment's repeat its last one and are
+        // not stored).  Called when every score of this half's last segment is complete, so its tile is free.
+        auto load_q = [&](const TileSeg& it) {
+            const int arow = it.row0 + min(half * 128 + row, it.nrows - 1), tok = arow / p.gq;
+            const __half* src = p.q + int64_t(it.q_start + tok) * p.q_t + int64_t(it.head * p.gq + arow - tok * p.gq) * p.q_h;
+            uint4 v[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) sts128(sbase + Q_OFF + half * TILE + tile_off(row, c), v[c]);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[half]);
+        };
+        int sg = next_seg(seg0);
+        if (sg < seg1) load_q(p.segs[sg]);
+        while (sg < seg1 && ok) {
             const TileSeg it = p.segs[sg];
-            if (half * 128 >= it.nrows) continue;
             const int start = it.start, steps = (it.blk1 - it.blk0 + 1) >> 1;
             const int r = half * 128 + row;                          // row of the segment
             const bool live = r < it.nrows;
             const int arow = it.row0 + (live ? r : it.nrows - 1), tok = arow / p.gq, pos = start + tok;
+            const int head = it.head * p.gq + arow - tok * p.gq;
             const int first_pos = start + (it.row0 + half * 128) / p.gq;
             const int last_pos = start + (it.row0 + min(half * 128 + 127, it.nrows - 1)) / p.gq;
-            // This thread's row of Q (rows past the segment's repeat its last one and are not stored); every
-            // product of this half's last segment is complete (o_full), so its tile is free.
-            const int head = it.head * p.gq + arow - tok * p.gq;
-            {
-                const __half* src = p.q + int64_t(it.q_start + tok) * p.q_t + int64_t(head) * p.q_h;
-                uint4 v[16];
-#pragma unroll
-                for (int c = 0; c < 16; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-#pragma unroll
-                for (int c = 0; c < 16; ++c) sts128(sbase + Q_OFF + half * TILE + tile_off(row, c), v[c]);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[half]);
-            }
             float m = -INFINITY, l = 0.f;                            // m: the maximum that O and l are relative to (log2)
             for (int j = 0; j < steps; ++j, ++sc) {
                 const int key0 = (it.blk0 + 2 * j) * PT;
@@ -442,6 +449,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                 if (lane == 0) mbar_arrive(&p_ready[half]);
             }
             if (!ok) break;
+            // the next segment's Q: its first scores are computed while this one's result is stored
+            sg = next_seg(sg + 1);
+            if (sg < seg1) load_q(p.segs[sg]);
             if (!(ok = wait(&o_full[half], oc & 1u))) break;
             ++oc;
             tc_fence_after();

@@ -92,10 +92,12 @@ void seen_blocks(const nova_paged_plan_args& a, int64_t i, int64_t row0, int64_t
     *b1 = last / PT + 1;
 }
 
-// Which kernel takes request i: one tile of the few-rows kernel holds 16 query
-// rows of a KV head; more would read the cache once per 16 rows there, and once
-// per 256 rows in the tensor-core kernel.
-bool few_rows(const nova_paged_plan_args& a, int64_t i) { return a.q_lens[i] * (a.q_heads / a.kv_heads) <= ROWS_MAX; }
+// Which kernel takes request i.  A tile of the few-rows kernel holds 16 query
+// rows of a KV head, the tensor-core kernel's 256; the first starts and joins
+// faster, the second reads the cache once.  16 requests of up to 4000 tokens:
+// 32 rows each 67 us there, 97 us here; one of 8192 tokens, 64 rows: 48 and 36.
+constexpr int64_t FEW_ROWS = 2 * ROWS_MAX;
+bool few_rows(const nova_paged_plan_args& a, int64_t i) { return a.q_lens[i] * (a.q_heads / a.kv_heads) <= FEW_ROWS; }
 
 // Work list of the few-rows kernel: every tile's blocks cut into splits of at
 // least one block per warp (4), at most 32 per tile so that joining them stays
@@ -151,64 +153,84 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
 
 // Segments of the tensor-core kernel: the steps (128 keys) of all 256-row tiles
 // in a row, request by request and head by head so that neighbouring CTAs read
-// the same cache, cut into equal shares.  A segment costs about SEG_COST steps
-// besides its own (Q, the first loads, the result), and none is shorter than
-// MIN_STEPS unless its tile is.
-constexpr int64_t SEG_COST = 2, MIN_STEPS = 4;
+// the same cache, cut so that no CTA takes more than a share; the smallest share
+// that the SMs can hold is searched.  A segment costs about SEG_COST steps
+// besides its own (its result, the pipeline's fill), and a tile is not cut into
+// pieces below MIN_STEPS.
+constexpr int64_t SEG_COST = 3, MIN_STEPS = 3;
+
+struct Tile {
+    int64_t seq, head, row0, nrows, b0, b1, q_start;
+};
+
+// Deals the tiles' steps out to CTAs of `share` each -> how many it takes.
+// emit(tile, first block, end, new CTA).
+template <typename Emit>
+int64_t deal(const std::vector<Tile>& tiles, int64_t share, Emit&& emit) {
+    int64_t ctas = 1, left = share;
+    bool fresh = true;                         // nothing in this CTA yet
+    for (const Tile& t : tiles)
+        for (int64_t b0 = t.b0; b0 < t.b1;) {
+            const int64_t steps = (t.b1 - b0 + 1) / 2, room = left - SEG_COST;
+            int64_t take = std::min(steps, room);
+            if (take < steps) take = std::min(take, steps - MIN_STEPS);
+            if (take < std::min(steps, MIN_STEPS)) {
+                if (!fresh) {
+                    ++ctas;
+                    left = share;
+                    fresh = true;
+                    continue;
+                }
+                take = steps;                  // a share too small for any cut: the whole tile
+            }
+            const int64_t end = std::min(t.b1, b0 + 2 * take);
+            emit(t, b0, end, fresh);
+            left -= take + SEG_COST;
+            b0 = end;
+            fresh = false;
+        }
+    return ctas - fresh;
+}
 
 void tile_schedule(Builder& b, nova_paged_schedule& s) {
     const nova_paged_plan_args& a = b.a;
     const int64_t gq = a.q_heads / a.kv_heads;
-    int64_t total = 0;
-    for (int64_t i = 0; i < a.seqs; ++i)
-        for (int64_t r = 0; !few_rows(a, i) && r < a.q_lens[i] * gq; r += 256) {
-            int64_t b0, b1;
-            seen_blocks(a, i, r, std::min<int64_t>(256, a.q_lens[i] * gq - r), s.window, &b0, &b1);
-            total += ((b1 - b0 + 1) / 2 + SEG_COST) * a.kv_heads;
-        }
-    if (!total) return;
-    // What a CTA takes of the rest: an even share of it, recomputed per CTA since cuts are uneven.
-    auto share = [&](int64_t rest, int64_t started) {
-        const int64_t n = std::max<int64_t>(1, a.sms - started);
-        return std::max((rest + n - 1) / n, MIN_STEPS + SEG_COST);
-    };
-    std::vector<int32_t> ctas{0};
+    std::vector<Tile> tiles;
+    int64_t q_start = 0, total = 0;
+    for (int64_t i = 0; i < a.seqs; q_start += a.q_lens[i++])
+        for (int64_t h = 0; !few_rows(a, i) && h < a.kv_heads; ++h)
+            for (int64_t r = 0; r < a.q_lens[i] * gq; r += 256) {
+                Tile t{i, h, r, std::min<int64_t>(256, a.q_lens[i] * gq - r), 0, 0, q_start};
+                seen_blocks(a, i, r, t.nrows, s.window, &t.b0, &t.b1);
+                total += (t.b1 - t.b0 + 1) / 2 + SEG_COST;
+                tiles.push_back(t);
+            }
+    if (tiles.empty()) return;
+    auto none = [](const Tile&, int64_t, int64_t, bool) {};
+    int64_t lo = std::max((total + a.sms - 1) / a.sms, MIN_STEPS + SEG_COST), hi = lo;
+    while (deal(tiles, hi, none) > a.sms) hi *= 2;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (deal(tiles, mid, none) <= a.sms) hi = mid;
+        else lo = mid + 1;
+    }
+    std::vector<int32_t> ctas;
     std::vector<TileJoin> joins;
     s.segs_off = b.at();
-    int64_t q_start = 0, segs = 0, rest = total, left = share(rest, 0);   // left: what the current CTA still takes
-    for (int64_t i = 0; i < a.seqs; ++i) {
-        q_start += i ? a.q_lens[i - 1] : 0;
-        if (few_rows(a, i)) continue;
-        for (int64_t h = 0; h < a.kv_heads; ++h)
-            for (int64_t r = 0; r < a.q_lens[i] * gq; r += 256) {
-                const int64_t n = std::min<int64_t>(256, a.q_lens[i] * gq - r);
-                int64_t b0, b1;
-                seen_blocks(a, i, r, n, s.window, &b0, &b1);
-                const int64_t first_part = s.n_tile_parts, blk0 = b0;
-                while (b0 < b1) {
-                    if (left < MIN_STEPS + SEG_COST && int64_t(ctas.size()) < a.sms) {   // the next CTA
-                        if (ctas.back() != segs) ctas.push_back(int32_t(segs));
-                        left = share(rest, int64_t(ctas.size()) - 1);
-                    }
-                    const int64_t steps = (b1 - b0 + 1) / 2;
-                    int64_t take = std::min(steps, std::max(left - SEG_COST, MIN_STEPS));
-                    if (steps - take < MIN_STEPS || int64_t(ctas.size()) >= a.sms) take = steps;
-                    const int64_t end = std::min(b1, b0 + 2 * take);
-                    const bool cut = b0 != blk0 || end != b1;
-                    b.put(TileSeg{int(i), int(h), int(r), int(n), int(b0), int(end), cut ? int(s.n_tile_parts++) : -1, int(q_start), int(a.kv_lens[i] - a.q_lens[i]), int(a.kv_lens[i]),
-                                  int(a.page_off[i]), a.kv_lens[i] % PT ? int(a.tail_out[i]) : 0, 0, 0, 0, 0});
-                    ++segs;
-                    left -= take + SEG_COST;
-                    rest -= take;
-                    b0 = end;
-                }
-                rest -= SEG_COST;
-                if (s.n_tile_parts > first_part)
-                    joins.push_back(TileJoin{int(i), int(h), int(r), int(n), int(first_part),
-                                             int(s.n_tile_parts - first_part), 0, 0});
-            }
-    }
-    if (ctas.back() != segs) ctas.push_back(int32_t(segs));
+    int64_t segs = 0;
+    deal(tiles, hi, [&](const Tile& t, int64_t b0, int64_t end, bool fresh) {
+        if (fresh) ctas.push_back(int32_t(segs));
+        const bool cut = b0 != t.b0 || end != t.b1;
+        if (cut && b0 == t.b0)
+            joins.push_back(TileJoin{int(t.seq), int(t.head), int(t.row0), int(t.nrows), int(s.n_tile_parts), 0, 0, 0});
+        if (cut) ++joins.back().n_parts;
+        b.put(TileSeg{int(t.seq), int(t.head), int(t.row0), int(t.nrows), int(b0), int(end),
+                      cut ? int(s.n_tile_parts++) : -1, int(t.q_start), int(a.kv_lens[t.seq] - a.q_lens[t.seq]),
+                      int(a.kv_lens[t.seq]), int(a.page_off[t.seq]), a.kv_lens[t.seq] % PT ? int(a.tail_out[t.seq]) : 0,
+                      0, 0, 0, 0});
+        ++segs;
+    });
+    ctas.push_back(int32_t(segs));
     s.n_ctas = int64_t(ctas.size()) - 1;
     s.ctas_off = b.at();
     b.v.insert(b.v.end(), ctas.begin(), ctas.end());
