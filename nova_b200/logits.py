@@ -92,6 +92,14 @@ def add_generated(history: torch.Tensor, tokens: torch.Tensor, offsets: torch.Te
     _history_add(history, tokens, offsets, False)
 
 
+def _control(t: torch.Tensor, name: str, rows: int, device: int, history: torch.Tensor | None) -> int:
+    if t.dtype != torch.float32 or t.shape != (rows,) or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float32 [{rows}] on the logits' device")
+    if history is None:
+        raise ValueError(f"{name} needs a history")
+    return t.data_ptr()
+
+
 def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
                   repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
                   presence: torch.Tensor | None = None, bias: LogitBias | None = None,
@@ -111,7 +119,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         raise ValueError("logits must be CUDA float16 or float32 [rows, vocab] with a contiguous last dimension")
     rows, vocab = shape
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=logits.device)
+        out = torch.empty_strided(shape, (vocab, 1), dtype=dtype, device=logits.device)
     elif out.dtype != dtype or out.shape != shape or out.get_device() != i or out.stride(1) != 1:
         raise ValueError("out must have the shape, type and device of logits and a contiguous last dimension")
     hist = hist_stride = 0
@@ -119,16 +127,13 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         if history.dtype != torch.int16 or history.shape != shape or history.get_device() != i or history.stride(1) != 1:
             raise ValueError(f"history must be int16 {tuple(shape)} on the logits' device with a contiguous last dimension")
         hist, hist_stride = history.data_ptr(), history.stride(0)
-    controls = []
-    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-        if t is None:
-            controls.append(0)
-            continue
-        if t.dtype != torch.float32 or t.shape != (rows,) or t.get_device() != i or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous float32 [{rows}] on the logits' device")
-        if history is None:
-            raise ValueError(f"{name} needs a history")
-        controls.append(t.data_ptr())
+    rep = freq = pres = 0
+    if repetition is not None:
+        rep = _control(repetition, "repetition", rows, i, history)
+    if frequency is not None:
+        freq = _control(frequency, "frequency", rows, i, history)
+    if presence is not None:
+        pres = _control(presence, "presence", rows, i, history)
     biases = (0, 0, 0)
     if bias is not None:
         if bias.rows != rows or bias.vocab != vocab or bias.buffer.get_device() != i:
@@ -154,6 +159,6 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     elif allowed_row is not None:
         raise ValueError("allowed_row needs allowed")
     _ADJUST(_ADJUST.pack(logits.data_ptr(), logits.stride(0), dtype == torch.float32, out.data_ptr(), out.stride(0), hist,
-                         hist_stride, *controls, *biases, mask, masks, mask_stride, mask_row, rows, vocab),
+                         hist_stride, rep, freq, pres, *biases, mask, masks, mask_stride, mask_row, rows, vocab),
             _lib.raw_stream(i))
     return out

@@ -109,7 +109,7 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tens
                                 or scaling.get_device() != i or not scaling.is_contiguous()):
         raise ValueError(f"scaling must be contiguous float32 [{adapters}] on the plan's device")
     if out is None:
-        out, out_stride = torch.empty((tokens, n), dtype=_F16, device=x.device), n
+        out, out_stride = torch.empty_strided((tokens, n), (n, 1), dtype=_F16, device=x.device), n
     else:
         if out.dtype != _F16 or out.shape != (tokens, n) or out.get_device() != i or out.stride(1) != 1:
             raise ValueError(f"out must be float16 [{tokens}, {n}] with a contiguous last dimension")

@@ -36,6 +36,8 @@ from . import _lib
 PAGE = 64
 HEAD_DIM = 128
 _F16 = torch.float16
+_SCALE = HEAD_DIM ** -0.5
+_TILE = (2, PAGE, HEAD_DIM)
 _APPEND = _lib.Entry("nova_paged_append", _lib.PagedAppendArgs, _lib._P, _lib._P)
 _ATTEND = _lib.Entry("nova_paged_attention", _lib.PagedAttnArgs, _lib._P, _lib._P)
 
@@ -114,6 +116,8 @@ class PagePlan:
         self.workspace = torch.zeros(int(self.info.workspace_bytes), dtype=torch.uint8, device=self.device)
         self._index = self.buffer.get_device()                    # -1: on the host, for inspection only
         self._stream = _lib.raw_stream(self._index) if self._index >= 0 else 0
+        self._q_shape = (self.tokens, self.num_q_heads, HEAD_DIM)
+        self._sched = {w: n for n, w in enumerate(windows)}
         self._info, self._buffer = addressof(self.info), self.buffer.data_ptr()
         self._workspace, self._workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
 
@@ -137,21 +141,20 @@ class PagePlan:
 
 def _cache(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan) -> tuple[int, int]:
     """Checks one layer's storage against the plan -> (pages, tail buffers)."""
-    h = plan.num_kv_heads
-    cs, ts = codes.shape, tails.shape
-    if codes.dtype != torch.uint8 or len(cs) != 5 or cs[1:] != (h, 2, PAGE, HEAD_DIM):
-        raise ValueError(f"codes must be uint8 [pages, {h}, 2, {PAGE}, {HEAD_DIM}], got {codes.dtype} {tuple(cs)}")
-    if scales.dtype != _F16 or scales.shape != (cs[0], h, 4, HEAD_DIM):
-        raise ValueError(f"scales must be float16 [{cs[0]}, {h}, 4, {HEAD_DIM}], got {scales.dtype} "
-                         f"{tuple(scales.shape)}")
-    if tails.dtype != _F16 or len(ts) != 5 or ts[1:] != cs[1:]:
-        raise ValueError(f"tails must be float16 [buffers, {h}, 2, {PAGE}, {HEAD_DIM}], got {tails.dtype} {tuple(ts)}")
+    h, i = plan.num_kv_heads, plan._index
+    pages, buffers = codes.shape[0], tails.shape[0]
+    if codes.dtype != torch.uint8 or codes.shape != (pages, h, *_TILE):
+        raise ValueError(f"codes must be uint8 [pages, {h}, 2, {PAGE}, {HEAD_DIM}], got {codes.dtype} {tuple(codes.shape)}")
+    if scales.dtype != _F16 or scales.shape != (pages, h, 4, HEAD_DIM):
+        raise ValueError(f"scales must be float16 [{pages}, {h}, 4, {HEAD_DIM}], got {scales.dtype} {tuple(scales.shape)}")
+    if tails.dtype != _F16 or tails.shape != (buffers, h, *_TILE):
+        raise ValueError(f"tails must be float16 [buffers, {h}, 2, {PAGE}, {HEAD_DIM}], got {tails.dtype} "
+                         f"{tuple(tails.shape)}")
     if not (codes.is_contiguous() and scales.is_contiguous() and tails.is_contiguous()):
         raise ValueError("codes, scales and tails must be contiguous")
-    i = plan._index
     if i < 0 or codes.get_device() != i or scales.get_device() != i or tails.get_device() != i:
         raise ValueError("codes, scales, tails and the plan must be on one CUDA device")
-    return cs[0], ts[0]
+    return pages, buffers
 
 
 def qkv_append(qkv: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan, *,
@@ -169,7 +172,7 @@ def qkv_append(qkv: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tai
     queries, fp16 ``[tokens, H_q, 128]``."""
     hq, hkv, i = plan.num_q_heads, plan.num_kv_heads, plan._index
     pages, buffers = _cache(codes, scales, tails, plan)
-    shape = (plan.tokens, hq, HEAD_DIM)
+    shape = plan._q_shape
     if qkv.dtype != _F16 or qkv.shape != (plan.tokens, (hq + 2 * hkv) * HEAD_DIM):
         raise ValueError(f"qkv must be float16 [{plan.tokens}, {(hq + 2 * hkv) * HEAD_DIM}], got {qkv.dtype} "
                          f"{tuple(qkv.shape)}")
@@ -188,7 +191,8 @@ def qkv_append(qkv: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tai
             if t.dtype != _F16 or t.shape != (rope_len, HEAD_DIM) or t.get_device() != i or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous float16 [rope_len, {HEAD_DIM}] on the cache's device")
     if out is None:
-        out, out_stride = torch.empty(shape, dtype=_F16, device=qkv.device), hq * HEAD_DIM
+        out_stride = hq * HEAD_DIM
+        out = torch.empty_strided(shape, (out_stride, HEAD_DIM, 1), dtype=_F16, device=qkv.device)
     else:
         if (out.dtype != _F16 or out.shape != shape or out.get_device() != i or out.stride(2) != 1
                 or out.stride(1) != HEAD_DIM):
@@ -209,8 +213,8 @@ def paged_read(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, p
     tensors, requests one after another."""
     pages, buffers = _cache(codes, scales, tails, plan)
     shape = (plan.read_rows, plan.num_kv_heads, HEAD_DIM)
-    k = torch.empty(shape, dtype=_F16, device=codes.device)
-    v = torch.empty(shape, dtype=_F16, device=codes.device)
+    k = torch.empty_strided(shape, (plan.num_kv_heads * HEAD_DIM, HEAD_DIM, 1), dtype=_F16, device=codes.device)
+    v = torch.empty_like(k)
     rc = _lib.lib().nova_paged_read(codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages, buffers, plan._buffer,
                                     plan._info, k.data_ptr(), v.data_ptr(), plan._current())
     if rc:
@@ -230,25 +234,29 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     ``[tokens, H_q]``, log-sum-exp of the scaled scores.  Returns fp16
     ``[tokens, H_q, 128]``."""
     pages, buffers = _cache(codes, scales, tails, plan)
-    shape, i = (plan.tokens, plan.num_q_heads, HEAD_DIM), plan._index
-    if q.dtype != _F16 or q.shape != shape or q.get_device() != i or q.stride(2) != 1:
-        raise ValueError(f"q must be float16 {shape} on the cache's device with a contiguous last dimension, got "
-                         f"{q.dtype} {tuple(q.shape)}")
-    if window not in plan.windows:
+    shape, i = plan._q_shape, plan._index
+    if q.dtype != _F16 or q.shape != shape or q.get_device() != i:
+        raise ValueError(f"q must be float16 {shape} on the cache's device, got {q.dtype} {tuple(q.shape)}")
+    sched = plan._sched.get(window)
+    if sched is None:
         raise ValueError(f"window {window} is not one of the plan's {plan.windows}")
+    q_t, q_h, q_d = q.stride()
     if out is None:
-        out = torch.empty(shape, dtype=_F16, device=q.device)
-    elif out.dtype != _F16 or out.shape != shape or out.get_device() != i or out.stride(2) != 1:
-        raise ValueError(f"out must be float16 {shape} with a contiguous last dimension")
-    if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.shape != shape[:2]
-                                or lse_out.get_device() != i or not lse_out.is_contiguous()):
-        raise ValueError(f"lse_out must be contiguous float32 {shape[:2]}")
-    q_t, q_h, _ = q.stride()
-    o_t, o_h, _ = out.stride()
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=_F16, device=q.device)
+    elif out.dtype != _F16 or out.shape != shape or out.get_device() != i:
+        raise ValueError(f"out must be float16 {shape} on the cache's device")
+    o_t, o_h, o_d = out.stride()
+    if q_d != 1 or o_d != 1:
+        raise ValueError("q and out need a contiguous last dimension")
+    lse = 0
+    if lse_out is not None:
+        if (lse_out.dtype != torch.float32 or lse_out.shape != shape[:2] or lse_out.get_device() != i
+                or not lse_out.is_contiguous()):
+            raise ValueError(f"lse_out must be contiguous float32 {shape[:2]}")
+        lse = lse_out.data_ptr()
     _ATTEND(_ATTEND.pack(q.data_ptr(), q_t, q_h, codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages, buffers,
-                         out.data_ptr(), o_t, o_h, 0 if lse_out is None else lse_out.data_ptr(),
-                         HEAD_DIM ** -0.5 if scale is None else scale, plan._buffer, plan._workspace,
-                         plan._workspace_bytes, plan.windows.index(window)), plan._info, plan._current())
+                         out.data_ptr(), o_t, o_h, lse, _SCALE if scale is None else scale, plan._buffer, plan._workspace,
+                         plan._workspace_bytes, sched), plan._info, plan._current())
     return out
 
 
