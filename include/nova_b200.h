@@ -720,8 +720,13 @@ typedef struct nova_lora_args {
     const int32_t* tiles;     /* device                                          */
     const int32_t* rows;      /* device                                          */
     int64_t n_tiles, tile_rows, tokens, k, n, adapters, max_rank;
+    int64_t top_rank;         /* the largest rank in tiles                       */
+    void* workspace;          /* nova_lora_workspace_bytes()                     */
+    int64_t workspace_bytes;
 } nova_lora_args;
 
+/* Workspace of nova_lora_add (0 for 16-row tiles); needs no initialisation. */
+NOVA_API int nova_lora_workspace_bytes(int64_t n_tiles, int64_t tile_rows, int64_t top_rank, int64_t* bytes);
 NOVA_API int nova_lora_add(const nova_lora_args* args, void* stream);
 
 /*

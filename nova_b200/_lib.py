@@ -171,6 +171,7 @@ class LoraArgs(ctypes.Structure):
         ("x", _P), ("x_stride", _I), ("base", _P), ("base_stride", _I), ("out", _P), ("out_stride", _I),
         ("a", _P), ("b", _P), ("scaling", _P), ("tiles", _P), ("rows", _P),
         ("n_tiles", _I), ("tile_rows", _I), ("tokens", _I), ("k", _I), ("n", _I), ("adapters", _I), ("max_rank", _I),
+        ("top_rank", _I), ("workspace", _P), ("workspace_bytes", _I),
     ]
 
 
@@ -226,6 +227,7 @@ _SIGNATURES: dict[str, list] = {
     "nova_paged_read": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P],
     "nova_paged_attention": [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(PagedPlanInfo), _P],
     "nova_paged_attention_read_error": [_P, ctypes.POINTER(_i)],
+    "nova_lora_workspace_bytes": [_I, _I, _I, ctypes.POINTER(_I)],
     "nova_lora_add": [ctypes.POINTER(LoraArgs), _P],
     "nova_adjust_logits": [ctypes.POINTER(LogitsArgs), _P],
     "nova_history_add": [_P, _I, _P, _P, _I, _I, _I, _i, _P],

@@ -3,17 +3,21 @@
 //
 // 2 r (K + N) flops per row against 2 K + 4 N bytes of it and 2 r (K + N) of
 // its adapter: memory at any length, and for single tokens the latency of the
-// chain x A^T -> h -> h B^T.  So one launch does both products: a cluster of 8
-// CTAs takes a tile of up to 16 or 64 rows, each CTA an eighth of K for the
-// first product; of the partial sums (rows x rank, fp32) each CTA adds an
-// eighth, in CTA order, through distributed shared memory and hands the result
-// to all, and each then has all of h for its eighth of N.  h is rounded to fp16 for the second product (2^-11
-// of the adapter's term, which is added to base in fp32 before the one rounding
-// of the result).  Fragments of mma.sync m16n8k16 are read straight from
-// global memory: the contraction index is permuted so that a lane's operand
-// registers are 16 (x, A) or 8 (B) consecutive bytes, and the columns of four
-// neighbouring tiles are dealt so that a lane's results are 16 consecutive
-// bytes of base and out.
+// chain x A^T -> h -> h B^T.  The first product is split over K between the 8
+// CTAs of a cluster; of the partial sums (rows x rank, fp32) each CTA adds an
+// eighth, in CTA order, through distributed shared memory.  h is rounded to
+// fp16 for the second product (2^-11 of the adapter's term, which is added to
+// base in fp32 before the one rounding of the result).
+//   * few rows (16-row tiles): one launch; the clusters hand h to all of their
+//     CTAs, each of which goes on with an eighth of N;
+//   * many (64-row tiles): h goes through memory and a second launch takes the
+//     columns.  As one launch a cluster held its 8 CTAs for the whole of N, and
+//     37 of them did not fit the GPU at once: 93 us against 69 for 1.7k rows of
+//     19456 columns at rank 64.
+// Fragments of mma.sync m16n8k16 are read straight from global memory: the
+// contraction index is permuted so that a lane's operand registers are 16 (x, A)
+// or 8 (B) consecutive bytes, and the columns of four neighbouring tiles are
+// dealt so that a lane's results are 16 consecutive bytes of base and out.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -39,90 +43,97 @@ struct Params {
     const float* scaling;
     const int4* tiles;
     const int* rows;
+    __half* h;                   // 64-row tiles: the first product, [tile][64][R]
     int k, n, max_rank, copy;    // copy: rows without an adapter are copied (out is not base)
 };
+
+// The rank that the kernels are built for: what h has room for.
+inline int64_t rank_tile(int64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
 // RT: rank tiles of 8 (rank <= 8 RT).  MT: row tiles of 16.
 template <int RT, int MT>
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lora_add_kernel(const Params p) {
-    constexpr int R = 8 * RT, TM = 16 * MT, KS = WARPS / MT;   // KS warps share a row tile's part of K
-    constexpr int HP = R + 8;                                  // padded row of h
-    extern __shared__ __align__(16) uint8_t smem[];
-    float* red = reinterpret_cast<float*>(smem);               // [KS][TM][R], then this CTA's sums in [0]
-    __half* hs = reinterpret_cast<__half*>(red + KS * TM * R); // [TM][HP]
-    __shared__ int row_of[TM];
+struct Shape {
+    static constexpr int R = 8 * RT, TM = 16 * MT, KS = WARPS / MT;   // KS warps share a row tile's part of K
+    static constexpr int HP = R + 16;                                 // padded row of h: its reads hit all banks
+    static constexpr int RED = KS * TM * R * 4, H = TM * HP * 2;      // bytes of partial sums, of h
+};
 
+// This CTA's part of x A^T for a tile, fp32 sums over its warps in red[0 .. TM * R).
+template <int RT, int MT>
+__device__ __forceinline__ void shrink(const Params& p, int adapter, int rank, const int* row_of, float* red, int cr) {
+    using S = Shape<RT, MT>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int cr = int(blockIdx.x) % CLUSTER;
-    pdl_wait();
-    const int4 tile = p.tiles[blockIdx.x / CLUSTER];
-    const int adapter = tile.x, rank = tile.y, count = tile.w;
-    if (threadIdx.x < TM) row_of[threadIdx.x] = int(threadIdx.x) < count ? p.rows[tile.z + threadIdx.x] : -1;
-    __syncthreads();
-    const int n32 = (p.n + 31) / 32, nb0 = cr * n32 / CLUSTER, nb1 = (cr + 1) * n32 / CLUSTER;
-
-    if (adapter < 0) {      // the whole cluster has this tile: nobody waits below
-        if (p.copy)
-            for (int r = warp; r < count; r += WARPS)
-                for (int c = nb0 * 32 + lane * 8; c < min(nb1 * 32, p.n); c += 256)
-                    *reinterpret_cast<uint4*>(p.out + row_of[r] * p.out_stride + c) =
-                        *reinterpret_cast<const uint4*>(p.base + row_of[r] * p.base_stride + c);
-        return;
-    }
-
-    // ---- h = x A^T over this CTA's part of K
     const int mt = warp % MT, ks = warp / MT;
-    {
-        const int nk = (p.k + 31) / 32;
-        const int k0 = cr * nk / CLUSTER, k1 = (cr + 1) * nk / CLUSTER;
-        const int ra = row_of[mt * 16 + g], rb = row_of[mt * 16 + g + 8];
-        const __half* xa = ra >= 0 ? p.x + ra * p.x_stride + 8 * t : nullptr;
-        const __half* xb = rb >= 0 ? p.x + rb * p.x_stride + 8 * t : nullptr;
-        const __half* aw = p.a + int64_t(adapter) * p.max_rank * p.k + 8 * t;
-        float acc[RT][4];
+    const int nk = (p.k + 31) / 32;
+    const int k0 = cr * nk / CLUSTER, k1 = (cr + 1) * nk / CLUSTER;
+    const int ra = row_of[mt * 16 + g], rb = row_of[mt * 16 + g + 8];
+    const __half* xa = ra >= 0 ? p.x + ra * p.x_stride + 8 * t : nullptr;
+    const __half* xb = rb >= 0 ? p.x + rb * p.x_stride + 8 * t : nullptr;
+    const __half* aw = p.a + int64_t(adapter) * p.max_rank * p.k + 8 * t;
+    float acc[RT][4];
 #pragma unroll
-        for (int j = 0; j < RT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        constexpr int U = RT <= 2 ? 4 : RT <= 8 ? 2 : 1;   // 128 registers hold so many chunks in flight
+    for (int j = 0; j < RT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    constexpr int U = RT <= 2 ? 4 : RT <= 8 ? 2 : 1;   // 128 registers hold so many chunks in flight
 #pragma unroll U
-        for (int c = k0 + ks; c < k1; c += KS) {
-            const int k = c * 32;
-            const bool in = k + 8 * t < p.k;
-            const uint4 va = in && xa ? *reinterpret_cast<const uint4*>(xa + k) : zero4();
-            const uint4 vb = in && xb ? *reinterpret_cast<const uint4*>(xb + k) : zero4();
-#pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                const uint4 w = in && 8 * j + g < rank ? *reinterpret_cast<const uint4*>(aw + int64_t(8 * j + g) * p.k + k) : zero4();
-                mma_16816(acc[j], va.x, vb.x, va.y, vb.y, w.x, w.y);
-                mma_16816(acc[j], va.z, vb.z, va.w, vb.w, w.z, w.w);
-            }
-        }
-        float* dst = red + (ks * TM + mt * 16) * R;
+    for (int c = k0 + ks; c < k1; c += S::KS) {
+        const int k = c * 32;
+        const bool in = k + 8 * t < p.k;
+        const uint4 va = in && xa ? *reinterpret_cast<const uint4*>(xa + k) : zero4();
+        const uint4 vb = in && xb ? *reinterpret_cast<const uint4*>(xb + k) : zero4();
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
-            *reinterpret_cast<float2*>(dst + g * R + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-            *reinterpret_cast<float2*>(dst + (g + 8) * R + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+            const uint4 w = in && 8 * j + g < rank ? *reinterpret_cast<const uint4*>(aw + int64_t(8 * j + g) * p.k + k) : zero4();
+            mma_16816(acc[j], va.x, vb.x, va.y, vb.y, w.x, w.y);
+            mma_16816(acc[j], va.z, vb.z, va.w, vb.w, w.z, w.w);
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < TM * R; i += THREADS) {
-        float s = red[i];
+    float* dst = red + (ks * S::TM + mt * 16) * S::R;
 #pragma unroll
-        for (int w = 1; w < KS; ++w) s += red[w * TM * R + i];
-        red[i] = s;
+    for (int j = 0; j < RT; ++j) {
+        *reinterpret_cast<float2*>(dst + g * S::R + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2*>(dst + (g + 8) * S::R + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
     }
-    // ---- out = base + h B^T over this CTA's part of N: 32 columns a warp, B read once for all rows of the tile.
-    // What the first product does not change is requested now, so that it arrives during the exchange.
-    constexpr int S = RT / 2;                // steps of 16 along the rank
-    const __half* bw = p.b + int64_t(adapter) * p.n * p.max_rank + 4 * t;
-    uint4 ba[MT], bb[MT];
+    __syncthreads();
+    for (int i = threadIdx.x; i < S::TM * S::R; i += THREADS) {
+        float v = red[i];
+#pragma unroll
+        for (int w = 1; w < S::KS; ++w) v += red[w * S::TM * S::R + i];
+        red[i] = v;
+    }
+}
+
+// CTA i of the cluster adds the i-th eighth of h over all CTAs, in CTA order, and
+// hands each pair of elements to put(row, column, pair).
+template <int RT, int MT, typename Put>
+__device__ __forceinline__ void gather(cg::cluster_group& cluster, float* red, int cr, float scale, Put&& put) {
+    using S = Shape<RT, MT>;
+    constexpr int SHARE = S::TM * S::R / CLUSTER / 2;
+    for (int i = threadIdx.x; i < SHARE; i += THREADS) {
+        const int at = cr * SHARE + i;
+        float2 v[CLUSTER];
+#pragma unroll
+        for (int k = 0; k < CLUSTER; ++k) v[k] = reinterpret_cast<const float2*>(cluster.map_shared_rank(red, k))[at];
+        float2 s = v[0];
+#pragma unroll
+        for (int k = 1; k < CLUSTER; ++k) s = make_float2(s.x + v[k].x, s.y + v[k].y);
+        put(2 * at / S::R, 2 * at % S::R, __floats2half2_rn(s.x * scale, s.y * scale));
+    }
+}
+
+// 32 columns of the second product for MW row tiles of 16, B in registers once.
+template <int RT, int MW>
+struct Columns {
+    static constexpr int S = RT / 2;           // steps of 16 along the rank
+    uint4 ba[MW], bb[MW];
     uint2 w[4][S];
-    auto load = [&](int nb) {
+
+    __device__ __forceinline__ void load(const Params& p, const __half* bw, int rank, const int* row_of, int nb, int g, int t) {
         const int n0 = nb * 32, col = n0 + 8 * t;
         const bool in = col < p.n;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < MW; ++m) {
             const int ra = row_of[m * 16 + g], rb = row_of[m * 16 + g + 8];
             ba[m] = in && ra >= 0 ? *reinterpret_cast<const uint4*>(p.base + ra * p.base_stride + col) : zero4();
             bb[m] = in && rb >= 0 ? *reinterpret_cast<const uint4*>(p.base + rb * p.base_stride + col) : zero4();
@@ -133,34 +144,15 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 w[j][s] = make_uint2(0u, 0u);
-                if (rank > 16 * s + 4 * t && c < p.n) w[j][s] = *reinterpret_cast<const uint2*>(bw + int64_t(c) * p.max_rank + 16 * s);
+                if (rank > 16 * s + 4 * t && c < p.n)
+                    w[j][s] = *reinterpret_cast<const uint2*>(bw + int64_t(c) * p.max_rank + 16 * s + 4 * t);
             }
         }
-    };
-    int nb = nb0 + warp;
-    if (nb < nb1) load(nb);
-
-    // ---- the clusters' partial sums: CTA i adds the i-th eighth of h, in CTA order, and hands it to every CTA
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const float scale = p.scaling ? p.scaling[adapter] : 1.f;
-    constexpr int SHARE = TM * R / CLUSTER / 2;      // pairs of elements
-    for (int i = threadIdx.x; i < SHARE; i += THREADS) {
-        const int at = cr * SHARE + i;
-        float2 v[CLUSTER];
-#pragma unroll
-        for (int k = 0; k < CLUSTER; ++k) v[k] = reinterpret_cast<const float2*>(cluster.map_shared_rank(red, k))[at];
-        float2 s = v[0];
-#pragma unroll
-        for (int k = 1; k < CLUSTER; ++k) s = make_float2(s.x + v[k].x, s.y + v[k].y);
-        const __half2 h = __floats2half2_rn(s.x * scale, s.y * scale);
-        const int off = (2 * at / R) * HP + 2 * at % R;
-#pragma unroll
-        for (int k = 0; k < CLUSTER; ++k) *reinterpret_cast<__half2*>(cluster.map_shared_rank(hs, k) + off) = h;
     }
-    cluster.sync();                          // h is complete everywhere; no CTA reads or writes another's memory from here
 
-    for (; nb < nb1; nb += WARPS) {
+    // hs: the first row tile's h, rows of hp elements.
+    __device__ __forceinline__ void finish(const Params& p, const __half* hs, int hp, int rank, const int* row_of, int nb, int g,
+                                           int t) {
         const int col = nb * 32 + 8 * t;
         const bool in = col < p.n;
 #pragma unroll
@@ -175,14 +167,14 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
             }
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < MW; ++m) {
             float acc[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const uint2 lo = *reinterpret_cast<const uint2*>(hs + (m * 16 + g) * HP + 16 * s + 4 * t);
-                const uint2 hi = *reinterpret_cast<const uint2*>(hs + (m * 16 + g + 8) * HP + 16 * s + 4 * t);
+                const uint2 lo = *reinterpret_cast<const uint2*>(hs + (m * 16 + g) * hp + 16 * s + 4 * t);
+                const uint2 hi = *reinterpret_cast<const uint2*>(hs + (m * 16 + g + 8) * hp + 16 * s + 4 * t);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) mma_16816(acc[j], lo.x, hi.x, lo.y, hi.y, w[j][s].x, w[j][s].y);
             }
@@ -199,23 +191,140 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
             if (in && ra >= 0) *reinterpret_cast<uint4*>(p.out + ra * p.out_stride + col) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
             if (in && rb >= 0) *reinterpret_cast<uint4*>(p.out + rb * p.out_stride + col) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
         }
-        if (nb + WARPS < nb1) load(nb + WARPS);
+    }
+};
+
+// Columns [c0, c1) of the rows without an adapter.
+__device__ __forceinline__ void copy_rows(const Params& p, const int* row_of, int count, int c0, int c1) {
+    for (int r = threadIdx.x >> 5; r < count; r += WARPS)
+        for (int c = c0 + int(threadIdx.x & 31) * 8; c < min(c1, p.n); c += 256)
+            *reinterpret_cast<uint4*>(p.out + row_of[r] * p.out_stride + c) =
+                *reinterpret_cast<const uint4*>(p.base + row_of[r] * p.base_stride + c);
+}
+
+__device__ __forceinline__ int4 tile_rows(const Params& p, int tile, int tm, int* row_of) {
+    const int4 t = p.tiles[tile];
+    if (int(threadIdx.x) < tm) row_of[threadIdx.x] = int(threadIdx.x) < t.w ? p.rows[t.z + threadIdx.x] : -1;
+    __syncthreads();
+    return t;
+}
+
+// Both products of a 16-row tile in one launch (single tokens, few rows).
+template <int RT>
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lora_add_kernel(const Params p) {
+    using S = Shape<RT, 1>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* red = reinterpret_cast<float*>(smem);
+    __half* hs = reinterpret_cast<__half*>(smem + S::RED);
+    __shared__ int row_of[S::TM];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int cr = int(blockIdx.x) % CLUSTER;
+    pdl_wait();
+    const int4 tile = tile_rows(p, blockIdx.x / CLUSTER, S::TM, row_of);
+    const int n32 = (p.n + 31) / 32, nb0 = cr * n32 / CLUSTER, nb1 = (cr + 1) * n32 / CLUSTER;
+    if (tile.x < 0) {       // the whole cluster has this tile: nobody waits below
+        if (p.copy) copy_rows(p, row_of, tile.w, nb0 * 32, nb1 * 32);
+        return;
+    }
+    shrink<RT, 1>(p, tile.x, tile.y, row_of, red, cr);
+    // what the first product does not change is requested now, so that it arrives during the exchange
+    const __half* bw = p.b + int64_t(tile.x) * p.n * p.max_rank;
+    Columns<RT, 1> c;
+    int nb = nb0 + warp;
+    if (nb < nb1) c.load(p, bw, tile.y, row_of, nb, g, t);
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    gather<RT, 1>(cluster, red, cr, p.scaling ? p.scaling[tile.x] : 1.f, [&](int row, int col, __half2 h) {
+#pragma unroll
+        for (int k = 0; k < CLUSTER; ++k) *reinterpret_cast<__half2*>(cluster.map_shared_rank(hs, k) + row * S::HP + col) = h;
+    });
+    cluster.sync();         // h is complete everywhere; no CTA reads or writes another's memory from here
+    for (; nb < nb1; nb += WARPS) {
+        c.finish(p, hs, S::HP, tile.y, row_of, nb, g, t);
+        if (nb + WARPS < nb1) c.load(p, bw, tile.y, row_of, nb + WARPS, g, t);
     }
 }
 
-template <int RT, int MT>
-int run(const Params& p, int64_t tiles, cudaStream_t stream) {
-    constexpr int R = 8 * RT, TM = 16 * MT, KS = WARPS / MT;
-    constexpr int bytes = KS * TM * R * 4 + TM * (R + 8) * 2;
-    static bool ready[kMaxDevices];        // shared-memory limit raised on this device
-    const int dev = current_device();
-    if (dev < 0 || dev >= kMaxDevices || !ready[dev]) {
-        if (cudaFuncSetAttribute(reinterpret_cast<const void*>(&lora_add_kernel<RT, MT>),
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-            return check_launch("lora add");
-        if (dev >= 0 && dev < kMaxDevices) ready[dev] = true;
+// The first product of 64-row tiles -> h (fp16 [tile][64][R]) in the workspace.
+template <int RT>
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lora_shrink_kernel(const Params p) {
+    using S = Shape<RT, 4>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* red = reinterpret_cast<float*>(smem);
+    __shared__ int row_of[S::TM];
+    const int cr = int(blockIdx.x) % CLUSTER, at = blockIdx.x / CLUSTER;
+    pdl_wait();
+    const int4 tile = tile_rows(p, at, S::TM, row_of);
+    if (tile.x < 0) return;
+    shrink<RT, 4>(p, tile.x, tile.y, row_of, red, cr);
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    __half* h_out = p.h + int64_t(at) * S::TM * S::R;
+    gather<RT, 4>(cluster, red, cr, p.scaling ? p.scaling[tile.x] : 1.f,
+                  [&](int row, int col, __half2 h) { *reinterpret_cast<__half2*>(h_out + row * S::R + col) = h; });
+    cluster.sync();         // the others have read this CTA's sums
+}
+
+// The second product of 64-row tiles: COLS columns of a tile per CTA, a warp 32
+// rows x 32 columns at a time.
+constexpr int COLS = 512;
+
+template <int RT>
+__global__ void __launch_bounds__(THREADS, RT <= 8 ? 3 : 2) lora_expand_kernel(const Params p) {
+    using S = Shape<RT, 4>;
+    __shared__ __align__(16) __half hs[S::TM * S::HP];
+    __shared__ int row_of[S::TM];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    pdl_wait();
+    const int4 tile = tile_rows(p, blockIdx.y, S::TM, row_of);
+    const int c0 = int(blockIdx.x) * COLS, c1 = min(c0 + COLS, p.n);
+    if (tile.x < 0) {
+        if (p.copy) copy_rows(p, row_of, tile.w, c0, c1);
+        return;
     }
-    launch(lora_add_kernel<RT, MT>, dim3(unsigned(tiles * CLUSTER)), dim3(THREADS), bytes, stream, p);
+    const int* rows = row_of + (warp & 1) * 32;
+    const __half* bw = p.b + int64_t(tile.x) * p.n * p.max_rank;
+    Columns<RT, 2> c;
+    int nb = c0 / 32 + (warp >> 1);
+    const int nb1 = (c1 + 31) / 32;
+    if (nb < nb1) c.load(p, bw, tile.y, rows, nb, g, t);
+    const uint4* h_in = reinterpret_cast<const uint4*>(p.h + int64_t(blockIdx.y) * S::TM * S::R);
+    for (int i = threadIdx.x; i < S::TM * S::R / 8; i += THREADS)
+        *reinterpret_cast<uint4*>(hs + i / RT * S::HP + i % RT * 8) = h_in[i];
+    __syncthreads();
+    for (; nb < nb1; nb += WARPS / 2) {
+        c.finish(p, hs + (warp & 1) * 32 * S::HP, S::HP, tile.y, rows, nb, g, t);
+        if (nb + WARPS / 2 < nb1) c.load(p, bw, tile.y, rows, nb + WARPS / 2, g, t);
+    }
+}
+
+// Raises a kernel's shared-memory limit, once per device.
+template <typename K>
+int allow_smem(K kernel, int bytes, bool (&ready)[kMaxDevices]) {
+    const int dev = current_device();
+    if (dev >= 0 && dev < kMaxDevices && ready[dev]) return NOVA_OK;
+    if (cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+        cudaSuccess)
+        return check_launch("lora add");
+    if (dev >= 0 && dev < kMaxDevices) ready[dev] = true;
+    return NOVA_OK;
+}
+
+template <int RT>
+int run(const Params& p, int64_t tiles, bool wide, cudaStream_t stream) {
+    static bool ready[2][kMaxDevices];
+    const dim3 grid(unsigned(tiles * CLUSTER)), block(THREADS);
+    if (!wide) {
+        constexpr int bytes = Shape<RT, 1>::RED + Shape<RT, 1>::H;
+        if (int rc = allow_smem(&lora_add_kernel<RT>, bytes, ready[0])) return rc;
+        launch(lora_add_kernel<RT>, grid, block, bytes, stream, p);
+        return check_launch("lora add");
+    }
+    constexpr int bytes = Shape<RT, 4>::RED;
+    if (int rc = allow_smem(&lora_shrink_kernel<RT>, bytes, ready[1])) return rc;
+    launch(lora_shrink_kernel<RT>, grid, block, bytes, stream, p);
+    if (int rc = check_launch("lora add")) return rc;
+    launch(lora_expand_kernel<RT>, dim3(unsigned((p.n + COLS - 1) / COLS), unsigned(tiles)), block, 0, stream, p);
     return check_launch("lora add");
 }
 
@@ -235,12 +344,14 @@ extern "C" int nova_lora_add(const nova_lora_args* a, void* stream) {
         return fail(NOVA_ERR_INVALID, "lora add: k=%lld and n=%lld must be multiples of 8", (long long)a->k, (long long)a->n);
     if (a->adapters < 0 || (a->adapters && (a->max_rank < 8 || a->max_rank % 8 || a->max_rank > 128)))
         return fail(NOVA_ERR_UNSUPPORTED, "lora add: max_rank %lld must be a multiple of 8 up to 128", (long long)a->max_rank);
+    if (a->top_rank < 0 || a->top_rank > a->max_rank)
+        return fail(NOVA_ERR_INVALID, "lora add: top_rank %lld above max_rank %lld", (long long)a->top_rank, (long long)a->max_rank);
     if (!a->base || !a->out || !a->tiles || !a->rows || (a->adapters && (!a->x || !a->a || !a->b)))
         return fail(NOVA_ERR_INVALID, "lora add: NULL pointer");
     if (a->x_stride < a->k || a->base_stride < a->n || a->out_stride < a->n)
         return fail(NOVA_ERR_INVALID, "lora add: row strides below the row length");
     auto off = [](const void* p, int64_t al) { return reinterpret_cast<uintptr_t>(p) % al != 0; };
-    if (off(a->x, 16) || off(a->base, 16) || off(a->out, 16) || off(a->a, 16) || off(a->b, 16) || off(a->tiles, 16) ||
+    if (off(a->x, 16) || off(a->base, 16) || off(a->out, 16) || off(a->a, 16) || off(a->b, 16) || off(a->tiles, 16) || off(a->workspace, 16) ||
         a->x_stride % 8 || a->base_stride % 8 || a->out_stride % 8)
         return fail(NOVA_ERR_ALIGN, "lora add: pointers need 16-byte alignment, strides multiples of 8");
     Params p{};
@@ -259,11 +370,21 @@ extern "C" int nova_lora_add(const nova_lora_args* a, void* stream) {
     p.n = int(a->n);
     p.max_rank = int(a->max_rank);
     p.copy = a->out != a->base;
-    const int rt = a->max_rank <= 16 ? 2 : a->max_rank <= 32 ? 4 : a->max_rank <= 64 ? 8 : 16;
+    p.h = static_cast<__half*>(a->workspace);
+    const bool wide = a->tile_rows == 64;
+    const int64_t r = rank_tile(a->top_rank);
+    if (wide && a->adapters && (!a->workspace || a->workspace_bytes < a->n_tiles * 64 * r * 2))
+        return fail(NOVA_ERR_INVALID, "lora add: workspace of %lld bytes, %lld are needed", (long long)a->workspace_bytes,
+                    (long long)(a->n_tiles * 64 * r * 2));
+    if (wide && a->n_tiles > 65535) return fail(NOVA_ERR_UNSUPPORTED, "lora add: %lld tiles", (long long)a->n_tiles);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->tile_rows == 16)
-        return rt == 2 ? run<2, 1>(p, a->n_tiles, s) : rt == 4 ? run<4, 1>(p, a->n_tiles, s)
-             : rt == 8 ? run<8, 1>(p, a->n_tiles, s) : run<16, 1>(p, a->n_tiles, s);
-    return rt == 2 ? run<2, 4>(p, a->n_tiles, s) : rt == 4 ? run<4, 4>(p, a->n_tiles, s)
-         : rt == 8 ? run<8, 4>(p, a->n_tiles, s) : run<16, 4>(p, a->n_tiles, s);
+    return r == 16 ? run<2>(p, a->n_tiles, wide, s) : r == 32 ? run<4>(p, a->n_tiles, wide, s)
+         : r == 64 ? run<8>(p, a->n_tiles, wide, s) : run<16>(p, a->n_tiles, wide, s);
+}
+
+extern "C" int nova_lora_workspace_bytes(int64_t n_tiles, int64_t tile_rows, int64_t top_rank, int64_t* bytes) {
+    if (!bytes || n_tiles < 0 || top_rank < 0 || top_rank > 128)
+        return fail(NOVA_ERR_INVALID, "lora workspace: tiles=%lld, top_rank=%lld", (long long)n_tiles, (long long)top_rank);
+    *bytes = tile_rows == 64 ? n_tiles * 64 * lora::rank_tile(top_rank) * 2 : 0;
+    return NOVA_OK;
 }
