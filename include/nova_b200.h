@@ -600,10 +600,14 @@ typedef struct nova_paged_plan_args {
     int64_t windows[NOVA_PAGED_MAX_WINDOWS];
 } nova_paged_plan_args;
 
+typedef struct nova_paged_rows {
+    int64_t off, n, rows_per_tile;             /* work items of few query rows   */
+    int64_t n_parts;                           /* partial results of split items */
+} nova_paged_rows;
+
 typedef struct nova_paged_schedule {
     int64_t window;
-    int64_t rows_off, n_rows, rows_per_tile;   /* work items of few query rows   */
-    int64_t n_parts;                           /* partial results of split items */
+    nova_paged_rows rows[2];                   /* up to 4 rows per KV head; more */
     int64_t segs_off, ctas_off, n_ctas;        /* segments of many query rows    */
     int64_t joins_off, n_joins, n_tile_parts;  /* tiles cut between CTAs         */
 } nova_paged_schedule;

@@ -126,10 +126,16 @@ class PagedPlanArgs(ctypes.Structure):
     ]
 
 
+class PagedRows(ctypes.Structure):
+    """Mirror of ``nova_paged_rows``."""
+
+    _fields_ = [("off", _I), ("n", _I), ("rows_per_tile", _I), ("n_parts", _I)]
+
+
 class PagedSchedule(ctypes.Structure):
     """Mirror of ``nova_paged_schedule``."""
 
-    _fields_ = [("window", _I), ("rows_off", _I), ("n_rows", _I), ("rows_per_tile", _I), ("n_parts", _I),
+    _fields_ = [("window", _I), ("rows", PagedRows * 2),
                 ("segs_off", _I), ("ctas_off", _I), ("n_ctas", _I), ("joins_off", _I), ("n_joins", _I), ("n_tile_parts", _I)]
 
 

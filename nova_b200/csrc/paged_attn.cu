@@ -469,7 +469,7 @@ namespace {
 
 typedef void (*RowsKernel)(const rows::Params, const CUtensorMap);
 
-int launch_rows(const rows::Params& p, const CUtensorMap& tm, const nova_paged_schedule& s, cudaStream_t stream) {
+int launch_rows(const rows::Params& p, const CUtensorMap& tm, const nova_paged_rows& s, cudaStream_t stream) {
     static const RowsKernel kernels[3] = {rows::paged_attn_rows_kernel<1, true>, rows::paged_attn_rows_kernel<1, false>,
                                           rows::paged_attn_rows_kernel<2, false>};
     static bool ready[kMaxDevices][3];     // shared-memory limit raised on this device
@@ -481,7 +481,7 @@ int launch_rows(const rows::Params& p, const CUtensorMap& tm, const nova_paged_s
             return check_launch("paged attention");
         if (dev >= 0 && dev < kMaxDevices) ready[dev][which] = true;
     }
-    launch(kernels[which], dim3(unsigned(s.n_rows), unsigned(p.kv_heads)), dim3(rows::THREADS), rows::SMEM, stream, p, tm);
+    launch(kernels[which], dim3(unsigned(s.n), unsigned(p.kv_heads)), dim3(rows::THREADS), rows::SMEM, stream, p, tm);
     return check_launch("paged attention");
 }
 
@@ -509,9 +509,10 @@ extern "C" int nova_paged_attention(const nova_paged_attn_args* a, const nova_pa
         return fail(NOVA_ERR_UNSUPPORTED, "paged attention: %lld pages of %lld heads exceed 2^31 code rows",
                     (long long)a->num_pages, (long long)info->kv_heads);
     const nova_paged_schedule& s = info->sched[a->sched];
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (s.n_ctas)
-        if (int rc = launch_tiles(a, info, s, static_cast<cudaStream_t>(stream))) return rc;
-    if (!s.n_rows) return NOVA_OK;
+        if (int rc = launch_tiles(a, info, s, st)) return rc;
+    if (!s.rows[0].n && !s.rows[1].n) return NOVA_OK;
     rows::Params p{};
     p.q = static_cast<const __half*>(a->q);
     p.q_t = a->q_t_stride;
@@ -523,21 +524,28 @@ extern "C" int nova_paged_attention(const nova_paged_attn_args* a, const nova_pa
     p.o_h = a->o_h_stride;
     p.lse = static_cast<float*>(a->lse);
     p.pages = a->plan + info->page_off;
-    p.items = reinterpret_cast<const RowsItem*>(a->plan + s.rows_off);
     p.q_heads = int(info->q_heads);
     p.kv_heads = int(info->kv_heads);
     p.gq = p.q_heads / p.kv_heads;
     p.window = int(s.window);
-    p.tile_rows = int(s.rows_per_tile);
     p.scale_log2 = float(a->scale * 1.4426950408889634);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     p.err = reinterpret_cast<int*>(ws);
-    p.counters = reinterpret_cast<unsigned*>(ws + WS_HEAD);
-    p.part = reinterpret_cast<float*>(ws + WS_HEAD + ws_counters(s.n_parts, info->kv_heads));
     CUtensorMap tm{};
     if (a->num_pages > 0)
         if (int rc = make_tmap_u8_rows128(&tm, a->codes, uint64_t(code_rows), PT)) return rc;
-    return launch_rows(p, tm, s, static_cast<cudaStream_t>(stream));
+    int64_t counters = WS_HEAD, part = WS_HEAD + ws_counters(s, info->kv_heads);
+    for (const nova_paged_rows& list : s.rows) {
+        p.items = reinterpret_cast<const RowsItem*>(a->plan + list.off);
+        p.tile_rows = int(list.rows_per_tile);
+        p.counters = reinterpret_cast<unsigned*>(ws + counters);
+        p.part = reinterpret_cast<float*>(ws + part);
+        if (list.n)
+            if (int rc = launch_rows(p, tm, list, st)) return rc;
+        counters += list.n_parts * info->kv_heads * 4;
+        part += ws_list(list, info->kv_heads);
+    }
+    return NOVA_OK;
 }
 
 extern "C" int nova_paged_attention_read_error(void* workspace, int* host_value) {

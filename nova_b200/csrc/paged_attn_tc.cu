@@ -554,7 +554,7 @@ int launch_tiles(const nova_paged_attn_args* a, const nova_paged_plan_info* info
     p.cta_first = a->plan + s.ctas_off;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     p.err = reinterpret_cast<int*>(ws);
-    p.part = reinterpret_cast<float*>(ws + ws_rows_bytes(s.n_parts, info->kv_heads, s.rows_per_tile));
+    p.part = reinterpret_cast<float*>(ws + ws_rows_bytes(s, info->kv_heads));
     p.part_ml = reinterpret_cast<float2*>(p.part + s.n_tile_parts * 256 * D);
     p.q_heads = int(info->q_heads);
     p.kv_heads = int(info->kv_heads);

@@ -99,25 +99,27 @@ void seen_blocks(const nova_paged_plan_args& a, int64_t i, int64_t row0, int64_t
 constexpr int64_t FEW_ROWS = 2 * ROWS_MAX;
 bool few_rows(const nova_paged_plan_args& a, int64_t i) { return a.q_lens[i] * (a.q_heads / a.kv_heads) <= FEW_ROWS; }
 
-// Work list of the few-rows kernel: every tile's blocks cut into splits of at
+// Work lists of the few-rows kernel: requests of up to 4 rows, whose tiles keep
+// the weights' low parts at no cost, and of more.  Every tile's blocks are cut into splits of at
 // least one block per warp (4), at most 32 per tile so that joining them stays
 // short.  A CTA costs a few blocks' time to start and to join, so where splits
 // of up to 48 blocks let all CTAs be resident at once (3 per SM) the smallest
 // such size is taken; 16 requests of 8191 tokens: 70 us, 76 in splits of 16.
 // Beyond that about four times as many CTAs as are resident even out ragged
 // lengths (32 requests of 8000 to 32768 tokens: 225 us, 260 in one wave).
-void rows_schedule(Builder& b, nova_paged_schedule& s) {
+void rows_schedule(Builder& b, const nova_paged_schedule& s, bool more, nova_paged_rows& list) {
     const nova_paged_plan_args& a = b.a;
     const int64_t gq = a.q_heads / a.kv_heads;
+    auto mine = [&](int64_t i) { return few_rows(a, i) && (a.q_lens[i] * gq > 4) == more; };
     int64_t most = 0, total = 0;
     for (int64_t i = 0; i < a.seqs; ++i)
-        if (few_rows(a, i)) most = std::max(most, a.q_lens[i] * gq);
-    s.rows_per_tile = most <= 4 ? 4 : most <= 8 ? 8 : ROWS_MAX;
+        if (mine(i)) most = std::max(most, a.q_lens[i] * gq);
+    list.rows_per_tile = !more ? 4 : most <= 8 ? 8 : ROWS_MAX;
     std::vector<int64_t> tiles;                // blocks of each tile
     for (int64_t i = 0; i < a.seqs; ++i)
-        for (int64_t r = 0; few_rows(a, i) && r < a.q_lens[i] * gq; r += s.rows_per_tile) {
+        for (int64_t r = 0; mine(i) && r < a.q_lens[i] * gq; r += list.rows_per_tile) {
             int64_t b0, b1;
-            seen_blocks(a, i, r, std::min(s.rows_per_tile, a.q_lens[i] * gq - r), s.window, &b0, &b1);
+            seen_blocks(a, i, r, std::min(list.rows_per_tile, a.q_lens[i] * gq - r), s.window, &b0, &b1);
             tiles.push_back(b1 - b0);
             total += b1 - b0;
         }
@@ -129,25 +131,24 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
         if (ctas <= resident) break;
     }
     if (chunk > 48) chunk = std::max<int64_t>(16, total * a.kv_heads / (resident * 4) / 4 * 4);
-    s.rows_off = b.at();
-    int64_t& parts = s.n_parts;
+    list.off = b.at();
     int64_t q_start = 0;
     for (int64_t i = 0; i < a.seqs; q_start += a.q_lens[i++])
-        for (int64_t r = 0; few_rows(a, i) && r < a.q_lens[i] * gq; r += s.rows_per_tile) {
-            const int64_t n = std::min(s.rows_per_tile, a.q_lens[i] * gq - r);
+        for (int64_t r = 0; mine(i) && r < a.q_lens[i] * gq; r += list.rows_per_tile) {
+            const int64_t n = std::min(list.rows_per_tile, a.q_lens[i] * gq - r);
             int64_t b0, b1;
             seen_blocks(a, i, r, n, s.window, &b0, &b1);
             const int64_t c = std::max(chunk, ((b1 - b0 + 31) / 32 + 3) / 4 * 4);
             const int64_t splits = (b1 - b0 + c - 1) / c;
             for (int64_t k = 0; k < splits; ++k) {
                 RowsItem it{int(i), int(r), int(n), int(b0 + k * c), int(std::min(b1, b0 + (k + 1) * c)),
-                            splits > 1 ? int(parts) : -1, int(k), int(splits), int(q_start),
+                            splits > 1 ? int(list.n_parts) : -1, int(k), int(splits), int(q_start),
                             int(a.kv_lens[i] - a.q_lens[i]), int(a.kv_lens[i]), int(a.page_off[i]),
                             a.kv_lens[i] % PT ? int(a.tail_out[i]) : 0, 0, 0, 0};
                 b.put(it);
-                ++s.n_rows;
+                ++list.n;
             }
-            if (splits > 1) parts += splits;
+            if (splits > 1) list.n_parts += splits;
         }
 }
 
@@ -157,7 +158,7 @@ void rows_schedule(Builder& b, nova_paged_schedule& s) {
 // that the SMs can hold is searched.  A segment costs about SEG_COST steps
 // besides its own (its result, the pipeline's fill), and a tile is not cut into
 // pieces below MIN_STEPS.
-constexpr int64_t SEG_COST = 3, MIN_STEPS = 3;
+constexpr int64_t SEG_COST = 4, MIN_STEPS = 3;
 
 struct Tile {
     int64_t seq, head, row0, nrows, b0, b1, q_start;
@@ -299,9 +300,10 @@ extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, i
         for (int64_t w = 0; w < a.n_windows; ++w) {
             nova_paged_schedule& s = info->sched[w];
             s.window = a.windows[w];
-            rows_schedule(b, s);
+            rows_schedule(b, s, false, s.rows[0]);
+            rows_schedule(b, s, true, s.rows[1]);
             tile_schedule(b, s);
-            const int64_t bytes = ws_rows_bytes(s.n_parts, a.kv_heads, s.rows_per_tile) + s.n_tile_parts * 256 * (D + 2) * 4;
+            const int64_t bytes = ws_rows_bytes(s, a.kv_heads) + s.n_tile_parts * 256 * (D + 2) * 4;
             info->workspace_bytes = std::max(info->workspace_bytes, bytes);
         }
         info->ints = int64_t(b.v.size());

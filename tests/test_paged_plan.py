@@ -23,8 +23,7 @@ def make(q, kv, hq=8, hkv=2, **kw):
 
 
 def rows_items(plan, w=0):
-    s = plan.info.sched[w]
-    return plan.host[s.rows_off:s.rows_off + 16 * s.n_rows].reshape(-1, 16)
+    return np.concatenate([plan.host[r.off:r.off + 16 * r.n].reshape(-1, 16) for r in plan.info.sched[w].rows])
 
 
 def test_records_and_lists():
