@@ -49,7 +49,7 @@ class State:
         return torch.cat([x, self.tails[self.tail_out[i], head, j, :n % PAGE].double()])
 
 
-def attention(s: State, window=0, scale=D ** -0.5):
+def attention(s: State, window=0, scale=D ** -0.5, device="cpu"):
     """(out, bound on the kernel's error, lse, bound on its error), 64 bits.
 
     The kernel rounds each weight to fp16 (2^-11 of it at most; a weight below
@@ -62,15 +62,16 @@ def attention(s: State, window=0, scale=D ** -0.5):
     lse = torch.full(s.q.shape[:2], -float("inf"), dtype=torch.float64)
     lse_bound = torch.zeros(s.q.shape[:2], dtype=torch.float64)
     t0, gq = 0, s.hq // s.hkv
+    out, bound, lse, lse_bound = (t.to(device) for t in (out, bound, lse, lse_bound))
     for i, (m, n) in enumerate(zip(s.q_lens, s.kv_lens)):
         if not m:
             continue
-        behind = torch.arange(n - m, n)[:, None] - torch.arange(n)[None]
+        behind = torch.arange(n - m, n, device=device)[:, None] - torch.arange(n, device=device)[None]
         hide = (behind < 0) | ((behind >= window) if window else torch.zeros_like(behind, dtype=torch.bool))
         for h in range(s.hkv):
-            k, v = s.values(i, h, 0), s.values(i, h, 1)
+            k, v = s.values(i, h, 0).to(device), s.values(i, h, 1).to(device)
             for e in range(h * gq, (h + 1) * gq):
-                q = s.q[t0:t0 + m, e].double()
+                q = s.q[t0:t0 + m, e].to(device).double()
                 a = (q @ k.t() * scale).masked_fill(hide, -float("inf"))
                 size = (q.abs() @ k.abs().t() * scale).masked_fill(hide, 0.0).amax(1, keepdim=True)
                 p = torch.softmax(a, 1)
@@ -82,7 +83,7 @@ def attention(s: State, window=0, scale=D ** -0.5):
                 lse[t0:t0 + m, e] = torch.logsumexp(a, 1)
                 lse_bound[t0:t0 + m, e] = (err + n * 2.0 ** -24)[:, 0] + 2.0 ** -22 * (1 + lse[t0:t0 + m, e].abs())
         t0 += m
-    return out, bound, lse, lse_bound
+    return out.cpu(), bound.cpu(), lse.cpu(), lse_bound.cpu()
 
 
 def norm_rope(x, w, cos, sin, eps):
