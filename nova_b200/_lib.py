@@ -8,7 +8,6 @@ missing, or the tensors are not on a CUDA device, the calls raise.
 from __future__ import annotations
 
 import ctypes
-import struct
 from pathlib import Path
 
 import torch
@@ -323,36 +322,21 @@ def stream_of(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def raw_stream(index: int) -> int:
-    """Handle of the current stream of CUDA device ``index``, without building a
-    ``torch.cuda.Stream`` (about 4 us)."""
-    return torch._C._cuda_getCurrentRawStream(index)
+_fast = None
 
 
-class Entry:
-    """An entry point whose first argument is a struct, called with the struct's
-    bytes: ``entry(entry.pack(*fields), ...)``.  Packing all fields at once takes
-    about a microsecond less than setting them one by one on the ctypes mirror,
-    which is a tenth of a short call."""
-
-    __slots__ = ("name", "pack", "_rest", "_fn")
-
-    def __init__(self, name: str, mirror: type[ctypes.Structure], *rest) -> None:
-        codes = {_P: "q", _I: "q", ctypes.c_double: "d"}
-        layout = struct.Struct("<" + "".join(codes[t] for _, t in mirror._fields_))
-        if layout.size != ctypes.sizeof(mirror):
-            raise TypeError(f"{mirror.__name__} is not made of 8-byte fields")
-        self.name, self.pack, self._rest, self._fn = name, layout.pack, rest, None
-
-    def __call__(self, args: bytes, *rest) -> None:
-        fn = self._fn
-        if fn is None:
-            fn = lib()[self.name]          # a function object of its own, with its own argument types
-            fn.argtypes, fn.restype = [_P, *self._rest], ctypes.c_int
-            self._fn = fn
-        rc = fn(args, *rest)
-        if rc:
-            check(rc, self.name)
+def fast():
+    """The compiled binding of the serving operators, ``nova_b200._fast`` (built
+    with the library by ``python -m nova_b200.build``; there is no other path)."""
+    global _fast
+    if _fast is None:
+        lib()
+        try:
+            from . import _fast as module
+        except ImportError as e:
+            raise RuntimeError(f"nova_b200._fast is not built; run `python -m nova_b200.build` ({e})") from e
+        _fast = module
+    return _fast
 
 
 def available() -> bool:

@@ -2,6 +2,9 @@
 sm_100a with nvcc and links ``nova_b200/libnova_b200.so`` in the source tree
 (the shared object travels with the checkout; nothing goes to site-packages).
 
+The Python binding of the serving operators (``csrc/binding.cpp`` ->
+``nova_b200/_fast.so``) is compiled with the host compiler against this torch.
+
     python -m nova_b200.build            # incremental
     python -m nova_b200.build --force    # rebuild everything
     python -m nova_b200.build --verbose  # show -Xptxas -v register / spill report
@@ -14,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -21,6 +25,7 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 OBJ = PKG / "_build"
 LIB = PKG / "libnova_b200.so"
+FAST = PKG / "_fast.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -62,7 +67,29 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    build_binding(force)
     return LIB
+
+
+def build_binding(force: bool = False) -> Path:
+    """``nova_b200/_fast.so``, linked to the CUDA library beside it."""
+    src = CSRC / "binding.cpp"
+    deps = max(src.stat().st_mtime, (INCLUDE / "nova_b200.h").stat().st_mtime, Path(__file__).stat().st_mtime)
+    if not force and FAST.exists() and FAST.stat().st_mtime >= deps:
+        return FAST
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    includes = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes), str(src),
+           "-o", str(FAST), f"-L{PKG}", "-l:libnova_b200.so", f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+    return FAST
 
 
 def main() -> None:

@@ -23,7 +23,6 @@ import torch
 from . import _lib
 
 CHUNK = 2048     # tokens per bias list (one CTA's tokens)
-_ADJUST = _lib.Entry("nova_adjust_logits", _lib.LogitsArgs, _lib._P)
 
 
 class LogitBias:
@@ -50,8 +49,9 @@ class LogitBias:
         m = len(off)
         self.off, self.token = self.buffer[:m], self.buffer[m:m + n]
         self.value = self.buffer[m + n:].view(torch.float32)
-        at = self.buffer.data_ptr()
-        self._pointers = (at, at + 4 * m, at + 4 * (m + n)) if n else (0, 0, 0)
+        at = self.buffer.data_ptr()           # what csrc/binding.cpp reads; no biases: no pointers
+        self._handle = (self.rows, self.vocab, self.buffer.get_device(),
+                        *((at, at + 4 * m, at + 4 * (m + n)) if n else (0, 0, 0)))
 
 
 def new_history(rows: int, vocab: int, device: torch.device | str = "cuda") -> torch.Tensor:
@@ -92,14 +92,6 @@ def add_generated(history: torch.Tensor, tokens: torch.Tensor, offsets: torch.Te
     _history_add(history, tokens, offsets, False)
 
 
-def _control(t: torch.Tensor, name: str, rows: int, device: int, history: torch.Tensor | None) -> int:
-    if t.dtype != torch.float32 or t.shape != (rows,) or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous float32 [{rows}] on the logits' device")
-    if history is None:
-        raise ValueError(f"{name} needs a history")
-    return t.data_ptr()
-
-
 def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
                   repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
                   presence: torch.Tensor | None = None, bias: LogitBias | None = None,
@@ -114,51 +106,5 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     none; default: row i has mask i).  What a mask forbids becomes -inf whatever
     it was, NaN included; a row whose mask leaves nothing is all -inf.  ``out``
     may be ``logits``.  Returns a tensor of the logits' type."""
-    i, dtype, shape = logits.get_device(), logits.dtype, logits.shape
-    if i < 0 or len(shape) != 2 or (dtype != torch.float16 and dtype != torch.float32) or logits.stride(1) != 1:
-        raise ValueError("logits must be CUDA float16 or float32 [rows, vocab] with a contiguous last dimension")
-    rows, vocab = shape
-    if out is None:
-        out = torch.empty_strided(shape, (vocab, 1), dtype=dtype, device=logits.device)
-    elif out.dtype != dtype or out.shape != shape or out.get_device() != i or out.stride(1) != 1:
-        raise ValueError("out must have the shape, type and device of logits and a contiguous last dimension")
-    hist = hist_stride = 0
-    if history is not None:
-        if history.dtype != torch.int16 or history.shape != shape or history.get_device() != i or history.stride(1) != 1:
-            raise ValueError(f"history must be int16 {tuple(shape)} on the logits' device with a contiguous last dimension")
-        hist, hist_stride = history.data_ptr(), history.stride(0)
-    rep = freq = pres = 0
-    if repetition is not None:
-        rep = _control(repetition, "repetition", rows, i, history)
-    if frequency is not None:
-        freq = _control(frequency, "frequency", rows, i, history)
-    if presence is not None:
-        pres = _control(presence, "presence", rows, i, history)
-    biases = (0, 0, 0)
-    if bias is not None:
-        if bias.rows != rows or bias.vocab != vocab or bias.buffer.get_device() != i:
-            raise ValueError(f"bias is for [{bias.rows}, {bias.vocab}] logits, got {tuple(shape)}")
-        biases = bias._pointers
-    mask = masks = mask_stride = mask_row = 0
-    if allowed is not None:
-        words = (vocab + 31) // 32
-        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.get_device() != i:
-            raise ValueError(f"allowed must be int32 [masks, {words}] on the logits' device")
-        masks, width = allowed.shape
-        mask_stride, last = allowed.stride()
-        if masks < 1 or width < words or last != 1 or (masks > 1 and mask_stride < width):
-            raise ValueError(f"allowed must be int32 [masks, {words}] with rows of their own, got {tuple(allowed.shape)}")
-        mask, mask_stride = allowed.data_ptr(), max(mask_stride, width)
-        if allowed_row is not None:
-            if allowed_row.dtype != torch.int32 or allowed_row.shape != (rows,) or allowed_row.get_device() != i \
-                    or not allowed_row.is_contiguous():
-                raise ValueError(f"allowed_row must be contiguous int32 [{rows}] on the logits' device")
-            mask_row = allowed_row.data_ptr()
-        elif masks != rows:
-            raise ValueError(f"{masks} masks for {rows} rows need allowed_row")
-    elif allowed_row is not None:
-        raise ValueError("allowed_row needs allowed")
-    _ADJUST(_ADJUST.pack(logits.data_ptr(), logits.stride(0), dtype == torch.float32, out.data_ptr(), out.stride(0), hist,
-                         hist_stride, rep, freq, pres, *biases, mask, masks, mask_stride, mask_row, rows, vocab),
-            _lib.raw_stream(i))
-    return out
+    return _lib.fast().adjust_logits(logits, history, repetition, frequency, presence,
+                                     None if bias is None else bias._handle, allowed, allowed_row, out)

@@ -18,8 +18,6 @@ import torch
 from . import _lib
 
 MAX_RANK = 128
-_F16 = torch.float16
-_ADD = _lib.Entry("nova_lora_add", _lib.LoraArgs, _lib._P)
 
 
 class LoraPlan:
@@ -62,23 +60,22 @@ class LoraPlan:
         host = np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), rows.astype(np.int32)])
         self.device = torch.device(device)
         self.buffer = torch.from_numpy(host).to(self.device)
-        self._index = self.buffer.get_device()
-        self._stream = _lib.raw_stream(self._index) if self._index >= 0 else 0
-        self._tiles = self.buffer.data_ptr()
-        self._rows = self._tiles + 16 * self.n_tiles
         need = _lib.ctypes.c_int64(0)
         _lib.call("nova_lora_workspace_bytes", self.n_tiles, self.tile_rows, self.max_rank, _lib.ctypes.byref(need))
         self.workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-        self._workspace = (self.workspace.data_ptr(), need.value)
+        self._handle = 0                      # on the host: for inspection only
+        if self.buffer.is_cuda:               # what csrc/binding.cpp reads (LoraHandle)
+            at = self.buffer.data_ptr()
+            self._fields = (_lib.ctypes.c_int64 * 11)(
+                at, at + 16 * self.n_tiles, self.workspace.data_ptr(), need.value, self.buffer.get_device(),
+                _lib.stream_of(self.buffer.device), self.n_tiles, self.tile_rows, self.tokens, self.adapters, self.max_rank)
+            self._handle = _lib.ctypes.addressof(self._fields)
 
-    def _current(self) -> int:
-        """The current stream; tells the allocator when it is not the plan's own."""
-        stream = _lib.raw_stream(self._index)
-        if stream != self._stream:
-            current = torch.cuda.current_stream(self._index)
-            self.buffer.record_stream(current)
-            self.workspace.record_stream(current)
-        return stream
+    def _on_other_stream(self) -> None:
+        """A stream other than the plan's own uses its buffers: the allocator must know."""
+        current = torch.cuda.current_stream(self.buffer.device)
+        self.buffer.record_stream(current)
+        self.workspace.record_stream(current)
 
 
 def lora_add(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan, *,
@@ -91,39 +88,4 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tens
     adapter's rank are not read); ``scaling`` fp32 ``[adapters]``.  ``out`` may be
     ``base``; rows without an adapter are then left alone.  Returns fp16
     ``[tokens, N]``."""
-    i = plan._index
-    if i < 0:
-        raise ValueError("the plan is not on a CUDA device")
-    for t, name in ((x, "x"), (base, "base"), (a, "a"), (b, "b")):
-        if t.dtype != _F16 or t.get_device() != i:
-            raise ValueError(f"{name} must be float16 on the plan's CUDA device, got {t.dtype} on {t.device}")
-    if x.dim() != 2 or base.dim() != 2 or a.dim() != 3:
-        raise ValueError("x and base must be 2-D, a and b 3-D")
-    tokens, k = x.shape
-    n = base.shape[1]
-    adapters, r, _ = a.shape
-    if base.shape[0] != tokens or tokens != plan.tokens:
-        raise ValueError(f"x {tuple(x.shape)}, base {tuple(base.shape)} and the plan's {plan.tokens} rows do not match")
-    if a.shape[2] != k or b.shape != (adapters, n, r) or adapters != plan.adapters:
-        raise ValueError(f"a {tuple(a.shape)} / b {tuple(b.shape)} do not match K={k}, N={n}, {plan.adapters} adapters")
-    if plan.max_rank > r:
-        raise ValueError(f"the plan has rank {plan.max_rank}, the weights hold {r}")
-    x_stride, x_last = x.stride()
-    base_stride, base_last = base.stride()
-    if not a.is_contiguous() or not b.is_contiguous() or x_last != 1 or base_last != 1:
-        raise ValueError("a and b must be contiguous, x and base have a contiguous last dimension")
-    if scaling is not None and (scaling.dtype != torch.float32 or scaling.shape != (adapters,)
-                                or scaling.get_device() != i or not scaling.is_contiguous()):
-        raise ValueError(f"scaling must be contiguous float32 [{adapters}] on the plan's device")
-    if out is None:
-        out, out_stride = torch.empty_strided((tokens, n), (n, 1), dtype=_F16, device=x.device), n
-    else:
-        if out.dtype != _F16 or out.shape != (tokens, n) or out.get_device() != i or out.stride(1) != 1:
-            raise ValueError(f"out must be float16 [{tokens}, {n}] with a contiguous last dimension")
-        out_stride = out.stride(0)
-    if tokens == 1:                      # a single row's stride says nothing
-        x_stride, base_stride, out_stride = k, n, n
-    _ADD(_ADD.pack(x.data_ptr(), x_stride, base.data_ptr(), base_stride, out.data_ptr(), out_stride, a.data_ptr(),
-                   b.data_ptr(), 0 if scaling is None else scaling.data_ptr(), plan._tiles, plan._rows, plan.n_tiles,
-                   plan.tile_rows, tokens, k, n, adapters, r, plan.max_rank, *plan._workspace), plan._current())
-    return out
+    return _lib.fast().lora_add(x, base, a, b, plan, scaling, out)

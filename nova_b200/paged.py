@@ -35,11 +35,6 @@ from . import _lib
 
 PAGE = 64
 HEAD_DIM = 128
-_F16 = torch.float16
-_SCALE = HEAD_DIM ** -0.5
-_TILE = (2, PAGE, HEAD_DIM)
-_APPEND = _lib.Entry("nova_paged_append", _lib.PagedAppendArgs, _lib._P, _lib._P)
-_ATTEND = _lib.Entry("nova_paged_attention", _lib.PagedAttnArgs, _lib._P, _lib._P)
 
 
 def _i64(values, name: str) -> np.ndarray:
@@ -114,21 +109,18 @@ class PagePlan:
         self.host = buf[:int(self.info.ints)]
         self.buffer = torch.from_numpy(self.host).to(self.device)
         self.workspace = torch.zeros(int(self.info.workspace_bytes), dtype=torch.uint8, device=self.device)
-        self._index = self.buffer.get_device()                    # -1: on the host, for inspection only
-        self._stream = _lib.raw_stream(self._index) if self._index >= 0 else 0
-        self._q_shape = (self.tokens, self.num_q_heads, HEAD_DIM)
-        self._sched = {w: n for n, w in enumerate(windows)}
-        self._info, self._buffer = addressof(self.info), self.buffer.data_ptr()
-        self._workspace, self._workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        self._handle = 0                      # on the host: for inspection only
+        if self.buffer.is_cuda:               # what csrc/binding.cpp reads (PageHandle)
+            self._fields = (_lib.ctypes.c_int64 * 6)(
+                addressof(self.info), self.buffer.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(),
+                self.buffer.get_device(), _lib.stream_of(self.buffer.device))
+            self._handle = addressof(self._fields)
 
-    def _current(self) -> int:
-        """The current stream; tells the allocator when it is not the plan's own."""
-        stream = _lib.raw_stream(self._index)
-        if stream != self._stream:
-            current = torch.cuda.current_stream(self._index)
-            self.buffer.record_stream(current)
-            self.workspace.record_stream(current)
-        return stream
+    def _on_other_stream(self) -> None:
+        """A stream other than the plan's own uses its buffers: the allocator must know."""
+        current = torch.cuda.current_stream(self.buffer.device)
+        self.buffer.record_stream(current)
+        self.workspace.record_stream(current)
 
     def check_errors(self) -> None:
         """Raises RuntimeError when a bounded wait of an attention launch with
@@ -137,24 +129,6 @@ class PagePlan:
         _lib.call("nova_paged_attention_read_error", self.workspace.data_ptr(), byref(v))
         if v.value:
             raise RuntimeError(f"paged attention: a bounded wait gave up (code {v.value})")
-
-
-def _cache(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan) -> tuple[int, int]:
-    """Checks one layer's storage against the plan -> (pages, tail buffers)."""
-    h, i = plan.num_kv_heads, plan._index
-    pages, buffers = codes.shape[0], tails.shape[0]
-    if codes.dtype != torch.uint8 or codes.shape != (pages, h, *_TILE):
-        raise ValueError(f"codes must be uint8 [pages, {h}, 2, {PAGE}, {HEAD_DIM}], got {codes.dtype} {tuple(codes.shape)}")
-    if scales.dtype != _F16 or scales.shape != (pages, h, 4, HEAD_DIM):
-        raise ValueError(f"scales must be float16 [{pages}, {h}, 4, {HEAD_DIM}], got {scales.dtype} {tuple(scales.shape)}")
-    if tails.dtype != _F16 or tails.shape != (buffers, h, *_TILE):
-        raise ValueError(f"tails must be float16 [buffers, {h}, 2, {PAGE}, {HEAD_DIM}], got {tails.dtype} "
-                         f"{tuple(tails.shape)}")
-    if not (codes.is_contiguous() and scales.is_contiguous() and tails.is_contiguous()):
-        raise ValueError("codes, scales and tails must be contiguous")
-    if i < 0 or codes.get_device() != i or scales.get_device() != i or tails.get_device() != i:
-        raise ValueError("codes, scales, tails and the plan must be on one CUDA device")
-    return pages, buffers
 
 
 def qkv_append(qkv: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan, *,
@@ -170,40 +144,7 @@ def qkv_append(qkv: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tai
     128]``; None: none), in fp32 and rounded once.  K and V of a page that fills
     are quantized from its 64 tokens, the others stay in ``tails``.  Returns the
     queries, fp16 ``[tokens, H_q, 128]``."""
-    hq, hkv, i = plan.num_q_heads, plan.num_kv_heads, plan._index
-    pages, buffers = _cache(codes, scales, tails, plan)
-    shape = plan._q_shape
-    if qkv.dtype != _F16 or qkv.shape != (plan.tokens, (hq + 2 * hkv) * HEAD_DIM):
-        raise ValueError(f"qkv must be float16 [{plan.tokens}, {(hq + 2 * hkv) * HEAD_DIM}], got {qkv.dtype} "
-                         f"{tuple(qkv.shape)}")
-    qkv_stride, last = qkv.stride()
-    if qkv.get_device() != i or last != 1:
-        raise ValueError("qkv must be on the cache's device, with a contiguous last dimension")
-    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        if t is not None and (t.dtype != _F16 or t.shape != (HEAD_DIM,) or t.get_device() != i or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float16 [{HEAD_DIM}] on the cache's device")
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin go together")
-    rope_len = 0
-    if cos is not None:
-        rope_len = cos.shape[0]
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            if t.dtype != _F16 or t.shape != (rope_len, HEAD_DIM) or t.get_device() != i or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous float16 [rope_len, {HEAD_DIM}] on the cache's device")
-    if out is None:
-        out_stride = hq * HEAD_DIM
-        out = torch.empty_strided(shape, (out_stride, HEAD_DIM, 1), dtype=_F16, device=qkv.device)
-    else:
-        if (out.dtype != _F16 or out.shape != shape or out.get_device() != i or out.stride(2) != 1
-                or out.stride(1) != HEAD_DIM):
-            raise ValueError(f"out must be float16 {shape} with contiguous rows")
-        out_stride = out.stride(0)
-    _APPEND(_APPEND.pack(qkv.data_ptr(), qkv_stride, 0 if q_norm_weight is None else q_norm_weight.data_ptr(),
-                         0 if k_norm_weight is None else k_norm_weight.data_ptr(), eps,
-                         0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), rope_len,
-                         out.data_ptr(), out_stride, codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages,
-                         buffers, plan._buffer), plan._info, plan._current())
-    return out
+    return _lib.fast().qkv_append(qkv, codes, scales, tails, plan, q_norm_weight, k_norm_weight, eps, cos, sin, out)
 
 
 def paged_read(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan
@@ -211,15 +152,7 @@ def paged_read(codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, p
     """The cached K and V of positions ``[read_from, kv_len)`` of every request of
     the plan, as the values they stand for: two fp16 ``[rows, H_kv, 128]``
     tensors, requests one after another."""
-    pages, buffers = _cache(codes, scales, tails, plan)
-    shape = (plan.read_rows, plan.num_kv_heads, HEAD_DIM)
-    k = torch.empty_strided(shape, (plan.num_kv_heads * HEAD_DIM, HEAD_DIM, 1), dtype=_F16, device=codes.device)
-    v = torch.empty_like(k)
-    rc = _lib.lib().nova_paged_read(codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages, buffers, plan._buffer,
-                                    plan._info, k.data_ptr(), v.data_ptr(), plan._current())
-    if rc:
-        _lib.check(rc, "nova_paged_read")
-    return k, v
+    return _lib.fast().paged_read(codes, scales, tails, plan)
 
 
 def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tails: torch.Tensor, plan: PagePlan, *,
@@ -233,31 +166,7 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     ``scale``: of the scores (default ``128 ** -0.5``).  ``lse_out``: fp32
     ``[tokens, H_q]``, log-sum-exp of the scaled scores.  Returns fp16
     ``[tokens, H_q, 128]``."""
-    pages, buffers = _cache(codes, scales, tails, plan)
-    shape, i = plan._q_shape, plan._index
-    if q.dtype != _F16 or q.shape != shape or q.get_device() != i:
-        raise ValueError(f"q must be float16 {shape} on the cache's device, got {q.dtype} {tuple(q.shape)}")
-    sched = plan._sched.get(window)
-    if sched is None:
-        raise ValueError(f"window {window} is not one of the plan's {plan.windows}")
-    q_t, q_h, q_d = q.stride()
-    if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=_F16, device=q.device)
-    elif out.dtype != _F16 or out.shape != shape or out.get_device() != i:
-        raise ValueError(f"out must be float16 {shape} on the cache's device")
-    o_t, o_h, o_d = out.stride()
-    if q_d != 1 or o_d != 1:
-        raise ValueError("q and out need a contiguous last dimension")
-    lse = 0
-    if lse_out is not None:
-        if (lse_out.dtype != torch.float32 or lse_out.shape != shape[:2] or lse_out.get_device() != i
-                or not lse_out.is_contiguous()):
-            raise ValueError(f"lse_out must be contiguous float32 {shape[:2]}")
-        lse = lse_out.data_ptr()
-    _ATTEND(_ATTEND.pack(q.data_ptr(), q_t, q_h, codes.data_ptr(), scales.data_ptr(), tails.data_ptr(), pages, buffers,
-                         out.data_ptr(), o_t, o_h, lse, _SCALE if scale is None else scale, plan._buffer, plan._workspace,
-                         plan._workspace_bytes, sched), plan._info, plan._current())
-    return out
+    return _lib.fast().paged_attention(q, codes, scales, tails, plan, window, scale, out, lse_out)
 
 
 class PagedKVCache:

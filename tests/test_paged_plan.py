@@ -173,3 +173,30 @@ def test_tail_alternates_when_a_page_opens():
             if (start + n) % PAGE:
                 assert (p.tail_out[0] == tin) == ((start + n) // PAGE == start // PAGE)
         prev = p.tail_out[0]
+
+
+def test_binding_refuses_without_a_gpu():
+    """The compiled binding loads on the CPU and refuses host plans and other objects before anything else."""
+    import torch
+
+    from nova_b200 import _lib
+    from nova_b200.logits import adjust_logits
+    from nova_b200.lora import LoraPlan, lora_add
+    from nova_b200.paged import paged_attention, paged_read
+
+    assert _lib.fast().__name__.endswith("_fast")
+    p, t = make([1], [1]), torch.zeros(1, 8, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="plan is not on a CUDA device"):
+        paged_attention(t, t, t, t, p)
+    with pytest.raises(ValueError, match="plan is not on a CUDA device"):
+        paged_read(t, t, t, p)
+    with pytest.raises(ValueError, match="plan is not on a CUDA device"):
+        lora_add(t, t, t, t, LoraPlan([1], [0], [8], device="cpu"))
+    with pytest.raises(ValueError, match="CUDA"):
+        adjust_logits(t[0])
+    with pytest.raises(ValueError, match="tensor"):
+        adjust_logits(None)
+    with pytest.raises(AttributeError):
+        paged_read(t, t, t, object())
+    with pytest.raises(TypeError):
+        _lib.fast().paged_read(t, t)
