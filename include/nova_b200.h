@@ -620,6 +620,7 @@ typedef struct nova_paged_plan_info {
     int64_t max_page, max_tail;                /* largest page / tail number used */
     int64_t max_pos;          /* largest position of a new token, -1: none       */
     int64_t seq_off, page_off, pos_off;
+    int64_t open_off, n_open;
     int64_t write_off, n_write, read_off, n_read;
     int64_t n_windows;
     nova_paged_schedule sched[NOVA_PAGED_MAX_WINDOWS];

@@ -144,7 +144,7 @@ class PagedPlanInfo(ctypes.Structure):
     _fields_ = [
         ("ints", _I), ("workspace_bytes", _I), ("seqs", _I), ("tokens", _I), ("read_rows", _I), ("q_heads", _I),
         ("kv_heads", _I), ("max_page", _I), ("max_tail", _I), ("max_pos", _I), ("seq_off", _I), ("page_off", _I),
-        ("pos_off", _I), ("write_off", _I), ("n_write", _I), ("read_off", _I), ("n_read", _I), ("n_windows", _I),
+        ("pos_off", _I), ("open_off", _I), ("n_open", _I), ("write_off", _I), ("n_write", _I), ("read_off", _I), ("n_read", _I), ("n_windows", _I),
         ("sched", PagedSchedule * PAGED_MAX_WINDOWS),
     ]
 

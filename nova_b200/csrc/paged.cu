@@ -13,8 +13,8 @@ namespace nova {
 namespace paged {
 
 constexpr int THREADS = 256;
-constexpr int QH = 4;           // query heads of one token that a half warp takes
-constexpr int QITEMS = 16;      // such items per CTA of the q part
+constexpr int RH = 4;           // heads of one token that a half warp takes
+constexpr int ITEMS = 16;       // such items per CTA of the row part
 
 struct AppendParams {
     const __half* qkv;
@@ -30,9 +30,10 @@ struct AppendParams {
     __half* scales;
     __half* tails;
     const int* pos;
+    const OpenToken* open;
     const Block* blocks;
-    int tokens, n_write, q_heads, kv_heads;
-    int q_ctas;
+    int tokens, n_open, n_write, q_heads, kv_heads;
+    int row_ctas;
 };
 
 struct Row8 {                   // channels 4c..4c+3 and 64+4c..64+4c+3 of one row
@@ -73,12 +74,12 @@ __device__ __forceinline__ Row8 norm_rope_row(const Row8& in, bool norm, const f
                                               const float (&cs)[8], const float (&sn)[8], float eps) {
     float x[8];
     unpack(in, x);
+    float ss = 0.f;              // summed whether it is used or not: the other half warp may want its norm
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     if (norm) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         const float r = rsqrtf(ss * (1.0f / D) + eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
@@ -117,41 +118,59 @@ __device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
     return *reinterpret_cast<uint32_t*>(&r);
 }
 
-// CTAs [0, q_ctas): 16 groups of 4 query heads of a token each.  The others: K or V of
-// one (touched block, KV head).  A block that the step completes is held in
-// registers (4 tokens x 8 channels a thread), its minimum and maximum per
+// CTAs [0, row_ctas): 16 groups of 4 heads of a token each, one per half warp:
+// query heads, then K and V heads (of tokens whose page stays open: into its tail
+// buffer).  The others: K or V of one (block that the step completes, KV head),
+// held in registers (4 tokens x 8 channels a thread); its minimum and maximum per
 // channel go through shared memory once, and codes leave as 4-byte pieces of
-// 128-byte rows; a block that stays open only gets its new rows.
+// 128-byte rows.
 __global__ void __launch_bounds__(THREADS, 4) paged_append_kernel(const AppendParams p) {
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 15, part = warp * 2 + (lane >> 4);
     const Row8 zero{make_uint2(0u, 0u), make_uint2(0u, 0u)};
-    if (int(blockIdx.x) < p.q_ctas) {
-        const int groups = (p.q_heads + QH - 1) / QH, n = p.tokens * groups;
-        const int at = int(blockIdx.x) * QITEMS + part, use = min(at, n - 1);   // past the end: the last one, unstored
-        const int tok = use / groups, h0 = (use - tok * groups) * QH;
-        const __half* src = p.qkv + tok * p.qkv_stride + h0 * D;
-        Row8 r[QH];
+    if (int(blockIdx.x) < p.row_ctas) {
+        const int gq = (p.q_heads + RH - 1) / RH, gk = (p.kv_heads + RH - 1) / RH;
+        const int nq = p.tokens * gq, n = nq + p.n_open * 2 * gk;
+        const int at = int(blockIdx.x) * ITEMS + part;
+        const bool live = at < n, query = at < nq;
+        int tok = 0, h0 = 0, pos = 0, kind = 0, tail = 0;                     // kind: Q, K, V
+        if (query) {
+            tok = at / gq;
+            h0 = (at - tok * gq) * RH;
+            pos = p.cos ? p.pos[tok] : 0;
+        } else if (live) {
+            const int o = (at - nq) / (2 * gk), grp = (at - nq) - o * 2 * gk;
+            const OpenToken t = p.open[o];
+            kind = grp < gk ? 1 : 2;
+            h0 = (grp < gk ? grp : grp - gk) * RH;
+            tok = t.row;
+            pos = t.pos;
+            tail = t.tail;
+        }
+        const int heads = query ? p.q_heads : p.kv_heads;
+        const __half* src = p.qkv + tok * p.qkv_stride + (h0 + (kind == 0 ? 0 : p.q_heads + (kind == 1 ? 0 : p.kv_heads))) * D;
+        Row8 r[RH];
 #pragma unroll
-        for (int i = 0; i < QH; ++i) r[i] = h0 + i < p.q_heads ? load_row(src + i * D, c) : zero;
+        for (int i = 0; i < RH; ++i) r[i] = live && h0 + i < heads ? load_row(src + i * D, c) : zero;
+        const __half* wp = kind == 0 ? p.wq : kind == 1 ? p.wk : nullptr;
+        const bool rope = p.cos && kind < 2;
         float w[8], cs[8], sn[8];
-        unpack(p.wq ? load_row(p.wq, c) : zero, w);
-        const int64_t pos = p.cos ? int64_t(p.pos[tok]) * D : 0;
-        unpack(p.cos ? load_row(p.cos + pos, c) : zero, cs);
-        unpack(p.cos ? load_row(p.sin + pos, c) : zero, sn);
-        __half* dst = p.q + tok * p.q_stride + h0 * D;
+        unpack(wp ? load_row(wp, c) : zero, w);
+        unpack(rope ? load_row(p.cos + int64_t(pos) * D, c) : zero, cs);
+        unpack(rope ? load_row(p.sin + int64_t(pos) * D, c) : zero, sn);
 #pragma unroll
-        for (int i = 0; i < QH; ++i) {
-            const Row8 y = norm_rope_row(r[i], p.wq, w, p.cos, cs, sn, p.eps);
-            if (at < n && h0 + i < p.q_heads) store_row(dst + i * D, c, y);
+        for (int i = 0; i < RH; ++i) {
+            const Row8 y = norm_rope_row(r[i], wp, w, rope, cs, sn, p.eps);
+            __half* dst = kind == 0 ? p.q + tok * p.q_stride + (h0 + i) * D
+                                    : p.tails + half_off(tail, p.kv_heads, h0 + i, kind - 1) + pos % PT * D;
+            if (live && h0 + i < heads) store_row(dst, c, y);
         }
         return;
     }
-    const int item = (blockIdx.x - p.q_ctas) / (2 * p.kv_heads), hj = (blockIdx.x - p.q_ctas) % (2 * p.kv_heads);
+    const int item = (blockIdx.x - p.row_ctas) / (2 * p.kv_heads), hj = (blockIdx.x - p.row_ctas) % (2 * p.kv_heads);
     const int head = hj >> 1, j = hj & 1;
     const Block blk = p.blocks[item];
     const int b0 = blk.blk * PT;
-    const bool closes = blk.page >= 0;
     const __half* src = p.qkv + (p.q_heads + j * p.kv_heads + head) * int64_t(D) + int64_t(blk.row - blk.first) * p.qkv_stride;
     const __half* old = p.tails + half_off(blk.tail_in, p.kv_heads, head, j);
     Row8 r[4], cs[4], sn[4];
@@ -159,15 +178,15 @@ __global__ void __launch_bounds__(THREADS, 4) paged_append_kernel(const AppendPa
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int slot = i * 16 + part, pos = b0 + slot;
-        fresh[i] = pos >= blk.first && pos < blk.kv_len;
-        r[i] = cs[i] = sn[i] = zero;
+        fresh[i] = pos >= blk.first;
+        cs[i] = sn[i] = zero;
         if (fresh[i]) {
             r[i] = load_row(src + int64_t(pos) * p.qkv_stride, c);
             if (j == 0 && p.cos) {
                 cs[i] = load_row(p.cos + int64_t(pos) * D, c);
                 sn[i] = load_row(p.sin + int64_t(pos) * D, c);
             }
-        } else if (closes) {                                   // before `first`: the open page's token
+        } else {                                               // the open page's token
             r[i] = load_row(old + slot * D, c);
         }
     }
@@ -182,13 +201,6 @@ __global__ void __launch_bounds__(THREADS, 4) paged_append_kernel(const AppendPa
             const Row8 y = norm_rope_row(r[i], p.wk, w, p.cos, cf, sf, p.eps);
             if (fresh[i]) r[i] = y;
         }
-    }
-    if (!closes) {
-        __half* dst = p.tails + half_off(blk.tail_out, p.kv_heads, head, j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (fresh[i]) store_row(dst + (i * 16 + part) * D, c, r[i]);
-        return;
     }
     __shared__ __align__(8) uint32_t lims[8][2][D / 2];   // per warp: minima, maxima of each channel pair
     uint32_t mn[4], mx[4];
@@ -349,15 +361,18 @@ extern "C" int nova_paged_append(const nova_paged_append_args* a, const nova_pag
     p.scales = static_cast<__half*>(a->scales);
     p.tails = static_cast<__half*>(a->tails);
     p.pos = a->plan + info->pos_off;
+    p.open = reinterpret_cast<const OpenToken*>(a->plan + info->open_off);
+    p.n_open = int(info->n_open);
     p.blocks = reinterpret_cast<const Block*>(a->plan + info->write_off);
     p.tokens = int(info->tokens);
     p.n_write = int(info->n_write);
     p.q_heads = int(info->q_heads);
     p.kv_heads = int(info->kv_heads);
-    const int64_t q_ctas = (info->tokens * ((info->q_heads + QH - 1) / QH) + QITEMS - 1) / QITEMS;
-    const int64_t grid = q_ctas + info->n_write * 2 * info->kv_heads;
+    const int64_t rows = info->tokens * ((info->q_heads + RH - 1) / RH) + info->n_open * 2 * ((info->kv_heads + RH - 1) / RH);
+    const int64_t row_ctas = (rows + ITEMS - 1) / ITEMS;
+    const int64_t grid = row_ctas + info->n_write * 2 * info->kv_heads;
     if (grid >= (1ll << 31)) return fail(NOVA_ERR_UNSUPPORTED, "paged append: too many tokens in one step");
-    p.q_ctas = int(q_ctas);
+    p.row_ctas = int(row_ctas);
     launch(paged_append_kernel, dim3(unsigned(grid)), dim3(THREADS), 0, static_cast<cudaStream_t>(stream), p);
     return check_launch("paged append");
 }

@@ -15,8 +15,9 @@ struct Seq {                    // one request
     int q_start, q_len, kv_len, page_off, tail_in, tail_out, pad0, pad1;
 };
 struct RowsItem {               // few query rows x a range of 64-token blocks
-    int seq, row0, nrows, blk0, blk1, part0, split, n_splits;
-    int q_start, start, kv_len, page_off, tail, pad0, pad1, pad2;   // the request's: position of its first new token, ...
+    int row0, nrows, blk0, blk1, part0, split, n_splits;
+    int q_start, start, kv_len, page_off, tail;   // the request's: first token row, position of its first new token, ...
+    int page[4];                // of blocks blk0 .. blk0 + 3: each warp's first, so that its loads need no other record
 };
 struct TileSeg {                // many query rows (up to 256) x a range of blocks; part < 0: the whole tile
     int seq, head, row0, nrows, blk0, blk1, part, q_start;
@@ -25,7 +26,10 @@ struct TileSeg {                // many query rows (up to 256) x a range of bloc
 struct TileJoin {               // a tile whose segments left partials
     int seq, head, row0, nrows, part0, n_parts, pad0, pad1;
 };
-struct Block {                  // one 64-token block of a request (write and read lists)
+struct OpenToken {              // one new token whose page stays open
+    int row, pos, tail, pad;
+};
+struct Block {                  // one 64-token block of a request (write list: those that the step completes; read list)
     int blk, first, kv_len, row;         // row: token row of position `first`, the first new (written) or copied (read) one
     int tail_in, tail_out, page, pad;    // page: -1 while the block is open
 };

@@ -126,17 +126,18 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
     const int start = it.start;
     const int n_full = it.kv_len / PT;      // blocks past this one are the open page
 
-    auto issue = [&](int blk, int j) {     // one lane: K (j = 0) or V half of a page
+    auto issue = [&](int page, int j) {    // one lane: K (j = 0) or V half of a page
         uint64_t* bar = j ? bar_v : bar_k;
-        const int64_t ph = int64_t(p.pages[it.page_off + blk]) * p.kv_heads + head;
+        const int64_t ph = int64_t(page) * p.kv_heads + head;
         mbar_arrive_expect_tx(bar, TX_HALF);
         tma_load_2d(stage + j * 8192, &tm, 0, int((ph * 2 + j) * PT), bar);
         bulk_g2s(stage + SC + j * 512, p.scales + (ph * 4 + 2 * j) * D, 512, bar);
     };
     int blk = it.blk0 + warp;
     if (lane == 0 && blk < it.blk1 && blk < n_full) {
-        issue(blk, 0);
-        issue(blk, 1);
+        const int page = warp == 0 ? it.page[0] : warp == 1 ? it.page[1] : warp == 2 ? it.page[2] : it.page[3];
+        issue(page, 0);
+        issue(page, 1);
     }
 
     // Rows of this lane's columns: their positions (-1: no row) and the key range they see.
@@ -194,6 +195,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
     bool ok = true;
     for (; ok && blk < it.blk1 && blk < n_full; blk += NW) {
         const bool more = blk + NW < it.blk1 && blk + NW < n_full;
+        const int page = more && lane == 0 ? p.pages[it.page_off + blk + NW] : 0;   // read before it is needed
         if (!(ok = mbar_wait(bar_k, phase, p.err, 1))) {   // give up, but not while this page's V may still land
             mbar_wait(bar_v, phase, p.err, 1);
             mbar_wait(bar_k, phase, p.err, 1);
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
         __syncwarp();
         if (more && lane == 0) {
             fence_proxy_async();
-            issue(blk + NW, 0);
+            issue(page, 0);
         }
         softmax_step<NC, 8>(x, m, l, alpha);
         rescale();
@@ -300,14 +302,15 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
         __syncwarp();
         if (more && lane == 0) {
             fence_proxy_async();
-            issue(blk + NW, 1);
+            issue(page, 1);
         }
         phase ^= 1u;
     }
-    // The open page, 16 fp16 tokens at a time (one tile per warp), by the item that holds its block.
+    // The open page, 16 fp16 tokens at a time (one tile per warp, the first to the warp whose turn it is), by the
+    // item that holds its block.
     if (ok && it.blk1 > n_full && it.blk0 <= n_full) {
-        const int r0 = 16 * warp + g, base = n_full * PT;
-        if (base + 16 * warp < it.kv_len) {
+        const int tile = (warp - (n_full - it.blk0)) & (NW - 1), r0 = 16 * tile + g, base = n_full * PT;
+        if (base + 16 * tile < it.kv_len) {
             const __half* tk = p.tails + half_off(it.tail, p.kv_heads, head, 0);
             const __half* tv = tk + HALF_ROW;
             const bool live0 = base + r0 < it.kv_len, live1 = base + r0 + 8 < it.kv_len;
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
             softmax_step<NC, 2>(x, m, l, alpha);
             rescale();
             uint32_t v[4][8];
-            const int ta = 16 * warp + 2 * t;
+            const int ta = 16 * tile + 2 * t;
             const int tok[4] = {ta, ta + 1, ta + 8, ta + 9};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {

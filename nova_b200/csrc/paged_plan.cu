@@ -69,7 +69,7 @@ int check_requests(const nova_paged_plan_args& a) {
                         (long long)a.read_from[i], (long long)i, (long long)kv);
         tokens += q;
         rows += kv - (a.read_from ? a.read_from[i] : start / PT * PT);
-        if (tokens >= lim || rows >= lim || tokens * (a.q_heads + 2 * a.kv_heads) >= lim)
+        if (tokens >= lim || rows >= lim || tokens * (a.q_heads + 2 * a.kv_heads + 12) >= lim)
             return fail(NOVA_ERR_UNSUPPORTED, "plan: too many tokens in one step");
     }
     std::sort(bufs.begin(), bufs.end());
@@ -141,10 +141,13 @@ void rows_schedule(Builder& b, const nova_paged_schedule& s, bool more, nova_pag
             const int64_t c = std::max(chunk, ((b1 - b0 + 31) / 32 + 3) / 4 * 4);
             const int64_t splits = (b1 - b0 + c - 1) / c;
             for (int64_t k = 0; k < splits; ++k) {
-                RowsItem it{int(i), int(r), int(n), int(b0 + k * c), int(std::min(b1, b0 + (k + 1) * c)),
+                RowsItem it{int(r), int(n), int(b0 + k * c), int(std::min(b1, b0 + (k + 1) * c)),
                             splits > 1 ? int(list.n_parts) : -1, int(k), int(splits), int(q_start),
                             int(a.kv_lens[i] - a.q_lens[i]), int(a.kv_lens[i]), int(a.page_off[i]),
-                            a.kv_lens[i] % PT ? int(a.tail_out[i]) : 0, 0, 0, 0};
+                            a.kv_lens[i] % PT ? int(a.tail_out[i]) : 0, {-1, -1, -1, -1}};
+                for (int w = 0; w < 4; ++w)
+                    if (it.blk0 + w < std::min<int64_t>(it.blk1, a.kv_lens[i] / PT))
+                        it.page[w] = int(a.pages[a.page_off[i] + it.blk0 + w]);
                 b.put(it);
                 ++list.n;
             }
@@ -277,6 +280,13 @@ extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, i
         info->pos_off = b.at();
         for (int64_t i = 0; i < a.seqs; ++i)
             for (int64_t j = a.kv_lens[i] - a.q_lens[i]; j < a.kv_lens[i]; ++j) b.v.push_back(int32_t(j));
+        info->open_off = b.at();
+        int64_t first_row = 0;
+        for (int64_t i = 0; i < a.seqs; first_row += a.q_lens[i++]) {
+            const int64_t kv = a.kv_lens[i], start = kv - a.q_lens[i];
+            for (int64_t j = std::max(start, kv / PT * PT); j < kv; ++j, ++info->n_open)
+                b.put(OpenToken{int(first_row + j - start), int(j), int(a.tail_out[i]), 0});
+        }
         info->write_off = b.at();
         int64_t row = 0;
         auto block = [&](int64_t i, int64_t g, int64_t first, int64_t out_row) {
@@ -287,7 +297,7 @@ extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, i
         };
         for (int64_t i = 0; i < a.seqs; row += a.q_lens[i++]) {
             const int64_t start = a.kv_lens[i] - a.q_lens[i];
-            for (int64_t g = start / PT; a.q_lens[i] && g * PT < a.kv_lens[i]; ++g, ++info->n_write)
+            for (int64_t g = start / PT; a.q_lens[i] && (g + 1) * PT <= a.kv_lens[i]; ++g, ++info->n_write)
                 b.put(block(i, g, start, row));
         }
         info->read_off = b.at();

@@ -32,12 +32,13 @@ def test_records_and_lists():
     seqs = p.host[i.seq_off:i.seq_off + 32].reshape(4, 8)
     assert seqs[:, 0].tolist() == [0, 5, 6, 6] and seqs[:, 2].tolist() == [5, 130, 64, 300]
     assert p.tokens == 106
-    pos = p.host[i.pos_off:i.pos_off + 106]
-    assert pos.tolist() == [*range(5), 129, *range(200, 300)]
+    assert p.host[i.pos_off:i.pos_off + 106].tolist() == [*range(5), 129, *range(200, 300)]
+    open_tokens = p.host[i.open_off:i.open_off + 4 * i.n_open].reshape(-1, 4)       # row, position, tail buffer
+    assert open_tokens[:, :3].tolist() == ([[t, t, 0] for t in range(5)] + [[5, 129, 2]]
+                                           + [[6 + t - 200, t, 7] for t in range(256, 300)])
     write = p.host[i.write_off:i.write_off + 8 * i.n_write].reshape(-1, 8)
-    # block, first new position, length, its token row, tail before and after, page (-1: stays open)
-    assert write[:, :7].tolist() == [[0, 0, 5, 0, 0, 0, -1], [2, 129, 130, 5, 2, 2, -1], [3, 200, 300, 6, 6, 7, 6],
-                                     [4, 200, 300, 6, 6, 7, -1]]
+    # pages that fill: block, first new position, length, its token row, tail before and after, page
+    assert write[:, :7].tolist() == [[3, 200, 300, 6, 6, 7, 6]]
     assert p.read_rows == 5 + 2 + 0 + (300 - 192)
 
 
@@ -64,7 +65,10 @@ def test_every_row_sees_its_blocks_once(hq, hkv, window):
     p = make(q, kv, hq, hkv, windows=(window,))
     gq = hq // hkv
     seen = {}
-    for seq, row0, nrows, b0, b1, part0, split, n, q_start, start, kv_len, page_off, tail, *_ in rows_items(p).tolist():
+    at = {sum(q[:i]): i for i in range(len(q)) if q[i]}
+    for row0, nrows, b0, b1, part0, split, n, q_start, start, kv_len, page_off, tail, *first in rows_items(p).tolist():
+        seq = at[q_start]
+        assert first == [page_off + b if b < min(b1, kv_len // PAGE) else -1 for b in range(b0, b0 + 4)]
         assert (q_start, start, kv_len) == (sum(q[:seq]), kv[seq] - q[seq], kv[seq])
         assert page_off == sum(n // PAGE for n in kv[:seq]) and (not kv_len % PAGE or tail == p.tail_out[seq])
         assert 0 <= split < n and (part0 < 0) == (n == 1) and b1 > b0 and nrows >= 1
