@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
     }
     const int which = !p.allowed ? -1 : p.allowed_row ? p.allowed_row[row] : row;
     const float rep = p.repetition ? p.repetition[row] : 1.f;
+    const float inv = div_rn(1.f, rep);   // v * inv is within 2^-23 of v / rep, and no element waits for a division
     const float freq = p.frequency ? p.frequency[row] : 0.f;
     const float pres = p.presence ? p.presence[row] : 0.f;
     // 8 mask bits of this thread's tokens (all set: no mask)
@@ -150,13 +151,10 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         float v = to_float<T>(x.v[i]);
-        const int hi = h.v[i];
-        if (hi) {
-            const int times = hi & 0x7FFF;
-            v = v > 0.f ? div_rn(v, rep) : v * rep;
-            v -= freq * float(times);
-            v -= times ? pres : 0.f;
-        }
+        const int hi = h.v[i], times = hi & 0x7FFF;
+        v *= hi == 0 ? 1.f : v > 0.f ? inv : rep;
+        // times as a float: in the mantissa of 2^23, which is subtracted (a conversion runs at a quarter of the rate)
+        v -= times ? fmaf(freq, __int_as_float(0x4B000000 | times) - 8388608.f, pres) : 0.f;
         v += b[i];
         y.v[i] = from_float<T>((keep >> i) & 1u ? v : -INFINITY);
     }
