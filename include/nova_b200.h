@@ -705,10 +705,10 @@ NOVA_API int nova_paged_attention_read_error(void* workspace, int* host_value);
  * for the rows of adapter a; rows without an adapter: out = base.  x fp16
  * [tokens, k], base and out fp16 [tokens, n] (row strides in elements; out may
  * be base), A fp16 [adapters, max_rank, k], B fp16 [adapters, n, max_rank],
- * contiguous; scaling fp32 [adapters] or NULL (1).  tiles: int32 [n_tiles, 4]
- * = adapter (or -1), its rank, first entry in `rows`, number of entries (1 to
- * tile_rows); rows: int32 token rows, those of a tile all of its adapter, each
- * row in one tile.  Rows past a rank are never read.  k, n and max_rank
+ * contiguous; scaling fp32 [adapters] or NULL (1).  tiles: int32 [n_tiles, 4 +
+ * tile_rows] = adapter (or -1), its rank, number of rows (1 to tile_rows), 0,
+ * then the token rows, all of that adapter, padded with -1; each token row in one
+ * tile.  Rows past a rank are never read.  k, n and max_rank
  * multiples of 8, max_rank <= 128, tile_rows 16 or 64.  No counterpart in the
  * reference.
  */
@@ -723,7 +723,6 @@ typedef struct nova_lora_args {
     const void* b;
     const void* scaling;
     const int32_t* tiles;     /* device                                          */
-    const int32_t* rows;      /* device                                          */
     int64_t n_tiles, tile_rows, tokens, k, n, adapters, max_rank;
     int64_t top_rank;         /* the largest rank in tiles                       */
     void* workspace;          /* nova_lora_workspace_bytes()                     */

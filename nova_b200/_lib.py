@@ -174,7 +174,7 @@ class LoraArgs(ctypes.Structure):
 
     _fields_ = [
         ("x", _P), ("x_stride", _I), ("base", _P), ("base_stride", _I), ("out", _P), ("out_stride", _I),
-        ("a", _P), ("b", _P), ("scaling", _P), ("tiles", _P), ("rows", _P),
+        ("a", _P), ("b", _P), ("scaling", _P), ("tiles", _P),
         ("n_tiles", _I), ("tile_rows", _I), ("tokens", _I), ("k", _I), ("n", _I), ("adapters", _I), ("max_rank", _I),
         ("top_rank", _I), ("workspace", _P), ("workspace_bytes", _I),
     ]

@@ -39,7 +39,7 @@ struct PageHandle {
     int64_t buffer, workspace, workspace_bytes, device, stream;
 };
 struct LoraHandle {
-    int64_t tiles, rows, workspace, workspace_bytes, device, stream;
+    int64_t tiles, workspace, workspace_bytes, device, stream;
     int64_t n_tiles, tile_rows, tokens, adapters, top_rank;
 };
 
@@ -260,7 +260,6 @@ PyObject* lora_add(PyObject* const* o) {
     p.a = a.const_data_ptr();
     p.b = b.const_data_ptr();
     p.tiles = reinterpret_cast<const int32_t*>(h.tiles);
-    p.rows = reinterpret_cast<const int32_t*>(h.rows);
     p.n_tiles = h.n_tiles;
     p.tile_rows = h.tile_rows;
     p.tokens = h.tokens;

@@ -41,8 +41,7 @@ struct Params {
     const __half* a;
     const __half* b;
     const float* scaling;
-    const int4* tiles;
-    const int* rows;
+    const int* tiles;            // per tile: adapter, rank, rows, 0, then the rows (padded to the tile with -1)
     __half* h;                   // 64-row tiles: the first product, [tile][64][R]
     int k, n, max_rank, copy;    // copy: rows without an adapter are copied (out is not base)
 };
@@ -202,11 +201,15 @@ __device__ __forceinline__ void copy_rows(const Params& p, const int* row_of, in
                 *reinterpret_cast<const uint4*>(p.base + row_of[r] * p.base_stride + c);
 }
 
-__device__ __forceinline__ int4 tile_rows(const Params& p, int tile, int tm, int* row_of) {
-    const int4 t = p.tiles[tile];
-    if (int(threadIdx.x) < tm) row_of[threadIdx.x] = int(threadIdx.x) < t.w ? p.rows[t.z + threadIdx.x] : -1;
+struct Tile {
+    int adapter, rank, count;
+};
+__device__ __forceinline__ Tile read_tile(const Params& p, int tile, int tm, int* row_of) {
+    const int* rec = p.tiles + int64_t(tile) * (4 + tm);
+    if (int(threadIdx.x) < tm) row_of[threadIdx.x] = rec[4 + threadIdx.x];
+    const int4 head = *reinterpret_cast<const int4*>(rec);
     __syncthreads();
-    return t;
+    return {head.x, head.y, head.z};
 }
 
 // Both products of a 16-row tile in one launch (single tokens, few rows).
@@ -220,28 +223,28 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int cr = int(blockIdx.x) % CLUSTER;
     pdl_wait();
-    const int4 tile = tile_rows(p, blockIdx.x / CLUSTER, S::TM, row_of);
+    const Tile tile = read_tile(p, blockIdx.x / CLUSTER, S::TM, row_of);
     const int n32 = (p.n + 31) / 32, nb0 = cr * n32 / CLUSTER, nb1 = (cr + 1) * n32 / CLUSTER;
-    if (tile.x < 0) {       // the whole cluster has this tile: nobody waits below
-        if (p.copy) copy_rows(p, row_of, tile.w, nb0 * 32, nb1 * 32);
+    if (tile.adapter < 0) {       // the whole cluster has this tile: nobody waits below
+        if (p.copy) copy_rows(p, row_of, tile.count, nb0 * 32, nb1 * 32);
         return;
     }
-    shrink<RT, 1>(p, tile.x, tile.y, row_of, red, cr);
+    shrink<RT, 1>(p, tile.adapter, tile.rank, row_of, red, cr);
     // what the first product does not change is requested now, so that it arrives during the exchange
-    const __half* bw = p.b + int64_t(tile.x) * p.n * p.max_rank;
+    const __half* bw = p.b + int64_t(tile.adapter) * p.n * p.max_rank;
     Columns<RT, 1> c;
     int nb = nb0 + warp;
-    if (nb < nb1) c.load(p, bw, tile.y, row_of, nb, g, t);
+    if (nb < nb1) c.load(p, bw, tile.rank, row_of, nb, g, t);
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    gather<RT, 1>(cluster, red, cr, p.scaling ? p.scaling[tile.x] : 1.f, [&](int row, int col, __half2 h) {
+    gather<RT, 1>(cluster, red, cr, p.scaling ? p.scaling[tile.adapter] : 1.f, [&](int row, int col, __half2 h) {
 #pragma unroll
         for (int k = 0; k < CLUSTER; ++k) *reinterpret_cast<__half2*>(cluster.map_shared_rank(hs, k) + row * S::HP + col) = h;
     });
     cluster.sync();         // h is complete everywhere; no CTA reads or writes another's memory from here
     for (; nb < nb1; nb += WARPS) {
-        c.finish(p, hs, S::HP, tile.y, row_of, nb, g, t);
-        if (nb + WARPS < nb1) c.load(p, bw, tile.y, row_of, nb + WARPS, g, t);
+        c.finish(p, hs, S::HP, tile.rank, row_of, nb, g, t);
+        if (nb + WARPS < nb1) c.load(p, bw, tile.rank, row_of, nb + WARPS, g, t);
     }
 }
 
@@ -254,13 +257,13 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
     __shared__ int row_of[S::TM];
     const int cr = int(blockIdx.x) % CLUSTER, at = blockIdx.x / CLUSTER;
     pdl_wait();
-    const int4 tile = tile_rows(p, at, S::TM, row_of);
-    if (tile.x < 0) return;
-    shrink<RT, 4>(p, tile.x, tile.y, row_of, red, cr);
+    const Tile tile = read_tile(p, at, S::TM, row_of);
+    if (tile.adapter < 0) return;
+    shrink<RT, 4>(p, tile.adapter, tile.rank, row_of, red, cr);
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     __half* h_out = p.h + int64_t(at) * S::TM * S::R;
-    gather<RT, 4>(cluster, red, cr, p.scaling ? p.scaling[tile.x] : 1.f,
+    gather<RT, 4>(cluster, red, cr, p.scaling ? p.scaling[tile.adapter] : 1.f,
                   [&](int row, int col, __half2 h) { *reinterpret_cast<__half2*>(h_out + row * S::R + col) = h; });
     cluster.sync();         // the others have read this CTA's sums
 }
@@ -276,25 +279,25 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 3 : 2) lora_expand_kernel(c
     __shared__ int row_of[S::TM];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     pdl_wait();
-    const int4 tile = tile_rows(p, blockIdx.y, S::TM, row_of);
+    const Tile tile = read_tile(p, blockIdx.y, S::TM, row_of);
     const int c0 = int(blockIdx.x) * COLS, c1 = min(c0 + COLS, p.n);
-    if (tile.x < 0) {
-        if (p.copy) copy_rows(p, row_of, tile.w, c0, c1);
+    if (tile.adapter < 0) {
+        if (p.copy) copy_rows(p, row_of, tile.count, c0, c1);
         return;
     }
     const int* rows = row_of + (warp & 1) * 32;
-    const __half* bw = p.b + int64_t(tile.x) * p.n * p.max_rank;
+    const __half* bw = p.b + int64_t(tile.adapter) * p.n * p.max_rank;
     Columns<RT, 2> c;
     int nb = c0 / 32 + (warp >> 1);
     const int nb1 = (c1 + 31) / 32;
-    if (nb < nb1) c.load(p, bw, tile.y, rows, nb, g, t);
+    if (nb < nb1) c.load(p, bw, tile.rank, rows, nb, g, t);
     const uint4* h_in = reinterpret_cast<const uint4*>(p.h + int64_t(blockIdx.y) * S::TM * S::R);
     for (int i = threadIdx.x; i < S::TM * S::R / 8; i += THREADS)
         *reinterpret_cast<uint4*>(hs + i / RT * S::HP + i % RT * 8) = h_in[i];
     __syncthreads();
     for (; nb < nb1; nb += WARPS / 2) {
-        c.finish(p, hs + (warp & 1) * 32 * S::HP, S::HP, tile.y, rows, nb, g, t);
-        if (nb + WARPS / 2 < nb1) c.load(p, bw, tile.y, rows, nb + WARPS / 2, g, t);
+        c.finish(p, hs + (warp & 1) * 32 * S::HP, S::HP, tile.rank, rows, nb, g, t);
+        if (nb + WARPS / 2 < nb1) c.load(p, bw, tile.rank, rows, nb + WARPS / 2, g, t);
     }
 }
 
@@ -346,7 +349,7 @@ extern "C" int nova_lora_add(const nova_lora_args* a, void* stream) {
         return fail(NOVA_ERR_UNSUPPORTED, "lora add: max_rank %lld must be a multiple of 8 up to 128", (long long)a->max_rank);
     if (a->top_rank < 0 || a->top_rank > a->max_rank)
         return fail(NOVA_ERR_INVALID, "lora add: top_rank %lld above max_rank %lld", (long long)a->top_rank, (long long)a->max_rank);
-    if (!a->base || !a->out || !a->tiles || !a->rows || (a->adapters && (!a->x || !a->a || !a->b)))
+    if (!a->base || !a->out || !a->tiles || (a->adapters && (!a->x || !a->a || !a->b)))
         return fail(NOVA_ERR_INVALID, "lora add: NULL pointer");
     if (a->x_stride < a->k || a->base_stride < a->n || a->out_stride < a->n)
         return fail(NOVA_ERR_INVALID, "lora add: row strides below the row length");
@@ -364,8 +367,7 @@ extern "C" int nova_lora_add(const nova_lora_args* a, void* stream) {
     p.a = static_cast<const __half*>(a->a);
     p.b = static_cast<const __half*>(a->b);
     p.scaling = static_cast<const float*>(a->scaling);
-    p.tiles = reinterpret_cast<const int4*>(a->tiles);
-    p.rows = a->rows;
+    p.tiles = a->tiles;
     p.k = int(a->k);
     p.n = int(a->n);
     p.max_rank = int(a->max_rank);

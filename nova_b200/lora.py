@@ -52,22 +52,30 @@ class LoraPlan:
         # 16-row tiles are one launch, 8 CTAs each; once they no longer fit the GPU at once (two CTAs per SM), 64-row
         # tiles in two launches are faster: 300 rows 14 us against 22, 700 rows 22.5 and 21, 2800 rows 56 and 38
         self.tile_rows = 64 if (-(-busy // 16)).sum() > 40 else 16
-        tiles = []
-        for v, f, m in zip(values.tolist(), first.tolist(), n.tolist()):
-            r = int(rank[v]) if v >= 0 else 0
-            tiles += [(v, r, f + i, min(self.tile_rows, m - i)) for i in range(0, m, self.tile_rows)]
-        self.n_tiles = len(tiles)
-        host = np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), rows.astype(np.int32)])
+        # per tile: adapter, rank, rows, 0, then the rows, padded with -1
+        rec = 4 + self.tile_rows
+        counts = -(-n // self.tile_rows)
+        self.n_tiles = int(counts.sum())
+        tiles = np.full((self.n_tiles, rec), -1, dtype=np.int32)
+        group = np.repeat(np.arange(len(values)), counts)                       # which adapter's rows
+        nth = np.arange(self.n_tiles) - np.repeat(np.cumsum(counts) - counts, counts)
+        tiles[:, 0] = values[group]
+        tiles[:, 1] = np.where(values[group] >= 0, rank[values[group]] if len(rank) else 0, 0)
+        tiles[:, 2] = np.minimum(self.tile_rows, n[group] - nth * self.tile_rows)
+        tiles[:, 3] = 0
+        start = first[group] + nth * self.tile_rows
+        at = start[:, None] + np.arange(self.tile_rows)
+        inside = np.arange(self.tile_rows) < tiles[:, 2:3]
+        tiles[:, 4:][inside] = rows[at[inside]]
         self.device = torch.device(device)
-        self.buffer = torch.from_numpy(host).to(self.device)
+        self.buffer = torch.from_numpy(tiles.reshape(-1)).to(self.device)
         need = _lib.ctypes.c_int64(0)
         _lib.call("nova_lora_workspace_bytes", self.n_tiles, self.tile_rows, self.max_rank, _lib.ctypes.byref(need))
         self.workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device)
         self._handle = 0                      # on the host: for inspection only
         if self.buffer.is_cuda:               # what csrc/binding.cpp reads (LoraHandle)
-            at = self.buffer.data_ptr()
-            self._fields = (_lib.ctypes.c_int64 * 11)(
-                at, at + 16 * self.n_tiles, self.workspace.data_ptr(), need.value, self.buffer.get_device(),
+            self._fields = (_lib.ctypes.c_int64 * 10)(
+                self.buffer.data_ptr(), self.workspace.data_ptr(), need.value, self.buffer.get_device(),
                 _lib.stream_of(self.buffer.device), self.n_tiles, self.tile_rows, self.tokens, self.adapters, self.max_rank)
             self._handle = _lib.ctypes.addressof(self._fields)
 

@@ -131,14 +131,13 @@ def test_plan_gathers_rows_by_adapter():
 
     tokens, which, ranks = [3, 1, 0, 40, 2], [1, -1, 0, 0, 1], [4, 16, 9]
     p = LoraPlan(tokens, which, ranks, device="cpu")
-    tiles = p.buffer[:4 * p.n_tiles].view(-1, 4).tolist()
-    rows = p.buffer[4 * p.n_tiles:].tolist()
+    tiles = p.buffer.view(p.n_tiles, 4 + p.tile_rows).tolist()
     of_row = np.repeat(which, tokens).tolist()
+    rows = [r for t in tiles for r in t[4:4 + t[2]]]
     assert sorted(rows) == list(range(46)) and p.tile_rows == 16 and p.max_rank == 16
-    for adapter, rank, first, n in tiles:
-        assert 1 <= n <= p.tile_rows and rank == (ranks[adapter] if adapter >= 0 else 0)
-        assert all(of_row[r] == adapter for r in rows[first:first + n])
-    assert sum(t[3] for t in tiles) == 46
+    for adapter, rank, n, zero, *mine in tiles:
+        assert 1 <= n <= p.tile_rows and rank == (ranks[adapter] if adapter >= 0 else 0) and zero == 0
+        assert all(of_row[r] == adapter for r in mine[:n]) and all(r == -1 for r in mine[n:])
     assert LoraPlan([1] * 40, [0] * 20 + [1] * 20, [8, 8], device="cpu").tile_rows == 16
     assert LoraPlan([700, 500], [0, 1], [8, 8], device="cpu").tile_rows == 64
 
