@@ -4,12 +4,11 @@
 // 2 r (K + N) flops per row against 2 K + 4 N bytes of it and 2 r (K + N) of
 // its adapter: memory at any length, and for single tokens the latency of the
 // chain x A^T -> h -> h B^T.  The first product is split over K between the 8
-// CTAs of a cluster; of the partial sums (rows x rank, fp32) each CTA adds an
-// eighth, in CTA order, through distributed shared memory.  h is rounded to
-// fp16 for the second product (2^-11 of the adapter's term, which is added to
-// base in fp32 before the one rounding of the result).
-//   * few rows (16-row tiles): one launch; the clusters hand h to all of their
-//     CTAs, each of which goes on with an eighth of N;
+// CTAs of a cluster, whose partial sums (rows x rank, fp32) meet in distributed
+// shared memory and are added in CTA order.  h is rounded to fp16 for the second
+// product (2^-11 of the adapter's term, which is added to base in fp32 before the
+// one rounding of the result).
+//   * few rows (16-row tiles): one launch; each CTA goes on with an eighth of N;
 //   * many (64-row tiles): h goes through memory and a second launch takes the
 //     columns.  As one launch a cluster held its 8 CTAs for the whole of N, and
 //     37 of them did not fit the GPU at once: 93 us against 69 for 1.7k rows of
@@ -212,39 +211,60 @@ __device__ __forceinline__ Tile read_tile(const Params& p, int tile, int tm, int
     return {head.x, head.y, head.z};
 }
 
-// Both products of a 16-row tile in one launch (single tokens, few rows).
+// Both products of a 16-row tile in one launch (single tokens, few rows).  Every
+// CTA pushes its sums to all CTAs of the cluster, and each adds them up for
+// itself: one cluster barrier between the products, no remote load.
 template <int RT>
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lora_add_kernel(const Params p) {
     using S = Shape<RT, 1>;
+    constexpr int E = S::TM * S::R;                            // elements of h
     extern __shared__ __align__(16) uint8_t smem[];
-    float* red = reinterpret_cast<float*>(smem);
-    __half* hs = reinterpret_cast<__half*>(smem + S::RED);
+    float* red = reinterpret_cast<float*>(smem);               // [KS][E], this CTA's sums in [0]
+    float* from = reinterpret_cast<float*>(smem + S::RED);     // [CLUSTER][E]
+    __half* hs = reinterpret_cast<__half*>(smem + S::RED + CLUSTER * E * 4);
     __shared__ int row_of[S::TM];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int cr = int(blockIdx.x) % CLUSTER;
     pdl_wait();
     const Tile tile = read_tile(p, blockIdx.x / CLUSTER, S::TM, row_of);
     const int n32 = (p.n + 31) / 32, nb0 = cr * n32 / CLUSTER, nb1 = (cr + 1) * n32 / CLUSTER;
-    if (tile.adapter < 0) {       // the whole cluster has this tile: nobody waits below
+    if (tile.adapter < 0) { // the whole cluster has this tile: nobody waits below
         if (p.copy) copy_rows(p, row_of, tile.count, nb0 * 32, nb1 * 32);
         return;
     }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_arrive();                                  // this CTA runs: the others may write to it
     shrink<RT, 1>(p, tile.adapter, tile.rank, row_of, red, cr);
     // what the first product does not change is requested now, so that it arrives during the exchange
     const __half* bw = p.b + int64_t(tile.adapter) * p.n * p.max_rank;
-    Columns<RT, 1> c;
+    constexpr int AHEAD = RT <= 2 ? 3 : RT <= 4 ? 2 : 1;       // 32-column groups that registers hold
+    Columns<RT, 1> c[AHEAD];
     int nb = nb0 + warp;
-    if (nb < nb1) c.load(p, bw, tile.rank, row_of, nb, g, t);
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    gather<RT, 1>(cluster, red, cr, p.scaling ? p.scaling[tile.adapter] : 1.f, [&](int row, int col, __half2 h) {
 #pragma unroll
-        for (int k = 0; k < CLUSTER; ++k) *reinterpret_cast<__half2*>(cluster.map_shared_rank(hs, k) + row * S::HP + col) = h;
-    });
-    cluster.sync();         // h is complete everywhere; no CTA reads or writes another's memory from here
-    for (; nb < nb1; nb += WARPS) {
-        c.finish(p, hs, S::HP, tile.rank, row_of, nb, g, t);
-        if (nb + WARPS < nb1) c.load(p, bw, tile.rank, row_of, nb + WARPS, g, t);
+    for (int i = 0; i < AHEAD; ++i)
+        if (nb + i * WARPS < nb1) c[i].load(p, bw, tile.rank, row_of, nb + i * WARPS, g, t);
+    const float scale = p.scaling ? p.scaling[tile.adapter] : 1.f;
+    cluster.barrier_wait();
+    for (int i = threadIdx.x; i < E; i += THREADS) {           // the element that this thread has summed
+        const float v = red[i];
+#pragma unroll
+        for (int k = 0; k < CLUSTER; ++k) cluster.map_shared_rank(from, k)[cr * E + i] = v;
+    }
+    cluster.sync();         // every CTA's sums are here; no CTA touches another's memory from now on
+    for (int i = threadIdx.x; i < E; i += THREADS) {
+        float v = from[i];
+#pragma unroll
+        for (int k = 1; k < CLUSTER; ++k) v += from[k * E + i];
+        hs[i / S::R * S::HP + i % S::R] = __float2half_rn(v * scale);
+    }
+    __syncthreads();
+    for (; nb < nb1; nb += AHEAD * WARPS) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int at = nb + i * WARPS, later = at + AHEAD * WARPS;
+            if (at < nb1) c[i].finish(p, hs, S::HP, tile.rank, row_of, at, g, t);
+            if (later < nb1) c[i].load(p, bw, tile.rank, row_of, later, g, t);
+        }
     }
 }
 
@@ -318,7 +338,7 @@ int run(const Params& p, int64_t tiles, bool wide, cudaStream_t stream) {
     static bool ready[2][kMaxDevices];
     const dim3 grid(unsigned(tiles * CLUSTER)), block(THREADS);
     if (!wide) {
-        constexpr int bytes = Shape<RT, 1>::RED + Shape<RT, 1>::H;
+        constexpr int bytes = Shape<RT, 1>::RED + CLUSTER * 16 * 8 * RT * 4 + Shape<RT, 1>::H;
         if (int rc = allow_smem(&lora_add_kernel<RT>, bytes, ready[0])) return rc;
         launch(lora_add_kernel<RT>, grid, block, bytes, stream, p);
         return check_launch("lora add");

@@ -50,8 +50,10 @@ class LoraPlan:
         values, first, n = np.unique(of_row[rows], return_index=True, return_counts=True)
         busy = n[values >= 0]
         # 16-row tiles are one launch, 8 CTAs each; once they no longer fit the GPU at once (two CTAs per SM), 64-row
-        # tiles in two launches are faster: 300 rows 14 us against 22, 700 rows 22.5 and 21, 2800 rows 56 and 38
-        self.tile_rows = 64 if (-(-busy // 16)).sum() > 40 else 16
+        # tiles in two launches are faster if they are fewer: 300 rows of one adapter 14 us against 22, 700 rows 22.5
+        # and 21, 2800 rows 56 and 38; one row of each of 64 adapters 21 us against 29
+        small, large = (-(-busy // 16)).sum(), (-(-busy // 64)).sum()
+        self.tile_rows = 64 if small > 40 and 2 * large <= small else 16
         # per tile: adapter, rank, rows, 0, then the rows, padded with -1
         rec = 4 + self.tile_rows
         counts = -(-n // self.tile_rows)

@@ -140,6 +140,7 @@ def test_plan_gathers_rows_by_adapter():
         assert all(of_row[r] == adapter for r in mine[:n]) and all(r == -1 for r in mine[n:])
     assert LoraPlan([1] * 40, [0] * 20 + [1] * 20, [8, 8], device="cpu").tile_rows == 16
     assert LoraPlan([700, 500], [0, 1], [8, 8], device="cpu").tile_rows == 64
+    assert LoraPlan([1] * 64, list(range(64)), [8] * 64, device="cpu").tile_rows == 16
 
 
 @pytest.mark.parametrize("args,message", [
