@@ -608,7 +608,7 @@ typedef struct nova_paged_rows {
 typedef struct nova_paged_schedule {
     int64_t window;
     nova_paged_rows rows[2];                   /* up to 4 rows per KV head; more */
-    int64_t segs_off, ctas_off, n_ctas;        /* segments of many query rows    */
+    int64_t segs_off, n_segs, n_ctas;          /* segments of many query rows    */
     int64_t joins_off, n_joins, n_tile_parts;  /* tiles cut between CTAs         */
 } nova_paged_schedule;
 

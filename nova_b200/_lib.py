@@ -135,7 +135,7 @@ class PagedSchedule(ctypes.Structure):
     """Mirror of ``nova_paged_schedule``."""
 
     _fields_ = [("window", _I), ("rows", PagedRows * 2),
-                ("segs_off", _I), ("ctas_off", _I), ("n_ctas", _I), ("joins_off", _I), ("n_joins", _I), ("n_tile_parts", _I)]
+                ("segs_off", _I), ("n_segs", _I), ("n_ctas", _I), ("joins_off", _I), ("n_joins", _I), ("n_tile_parts", _I)]
 
 
 class PagedPlanInfo(ctypes.Structure):

@@ -20,8 +20,10 @@ struct RowsItem {               // few query rows x a range of 64-token blocks
     int page[4];                // of blocks blk0 .. blk0 + 3: each warp's first, so that its loads need no other record
 };
 struct TileSeg {                // many query rows (up to 256) x a range of blocks; part < 0: the whole tile
-    int seq, head, row0, nrows, blk0, blk1, part, q_start;
-    int start, kv_len, page_off, tail, pad0, pad1, pad2, pad3;   // the request's: position of its first new token, ...
+    int head, row0, nrows, blk0, blk1, part, q_start;
+    int start, kv_len, page_off, tail;   // the request's: position of its first new token, ...
+    int page[4];                // of blocks blk0 .. blk0 + 3, so that the first loads need no other record
+    int next;                   // the CTA's next segment, -1: none (segment c is CTA c's first)
 };
 struct TileJoin {               // a tile whose segments left partials
     int seq, head, row0, nrows, part0, n_parts, pad0, pad1;

@@ -50,7 +50,6 @@ struct Params {
     const Seq* seqs;                   // the joining kernel's; segments carry what they need
     const int* pages;
     const TileSeg* segs;
-    const int* cta_first;
     int* err;
     float* part;                       // [part][32][256][4]: four channels of all rows, then the next four
     float2* part_ml;
@@ -197,15 +196,15 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
         return false;
     };
     pdl_wait();
-    const int seg0 = p.cta_first[blockIdx.x], seg1 = p.cta_first[blockIdx.x + 1];
 
     if (warp >= 8 && warp < 12) {
         // ------------------------------------------------ loading warps
         reg_inc<REG_LOAD>();
         const int tid = threadIdx.x - 256, c = tid & 15, r0 = tid >> 4;   // 8 channels, first row (of 8)
         uint32_t kc = 0;               // steps so far
-        for (int sg = seg0; sg < seg1; ++sg) {
+        for (int sg = blockIdx.x; sg >= 0;) {
             const TileSeg it = p.segs[sg];
+            sg = it.next;
             const int n_full = it.kv_len / PT;
             const int steps = (it.blk1 - it.blk0 + 1) >> 1;
             const int* pages = p.pages + it.page_off;
@@ -253,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                 if (lane == 0) mbar_arrive(bar);
             };
             Raw k0, k1, v0, v1;
-            int pg0 = page_of(0), pg1 = page_of(1);
+            int pg0 = it.page[0], pg1 = it.blk0 + 1 < it.blk1 ? it.page[1] : -2;
             fetch(k0, pg0, 0);
             fetch(k1, pg1, 0);
             fetch(v0, pg0, 1);
@@ -307,8 +306,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                 if (elect_one()) tc_commit(bar);
                 __syncwarp();
             };
-            for (int sg = seg0; sg < seg1 && ok; ++sg) {
+            for (int sg = blockIdx.x; sg >= 0 && ok;) {
                 const TileSeg it = p.segs[sg];
+                sg = it.next;
                 const int steps = (it.blk1 - it.blk0 + 1) >> 1, halves = it.nrows > 128 ? 2 : 1;
                 if (!(ok = wait(&k_full[kc & 1u], (kc >> 1) & 1u))) break;
                 for (int i = 0; i < halves; ++i) {
@@ -356,9 +356,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
         const uint32_t s_addr = tmem + S_COL + half * 128 + lanes, o_addr = tmem + O_COL + half * 128 + lanes;
         uint32_t sc = 0, oc = 0;       // steps and segments of this half so far
         bool ok = true;
-        // First of the segments from sg on that has rows in this half.
+        // The CTA's first segment from sg on that has rows in this half.
         auto next_seg = [&](int sg) {
-            while (sg < seg1 && p.segs[sg].nrows <= half * 128) ++sg;
+            while (sg >= 0 && p.segs[sg].nrows <= half * 128) sg = p.segs[sg].next;
             return sg;
         };
         // This thread's row of a segment's Q into shared memory (rows past the segment's repeat its last one and are
@@ -375,9 +375,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[half]);
         };
-        int sg = next_seg(seg0);
-        if (sg < seg1) load_q(p.segs[sg]);
-        while (sg < seg1 && ok) {
+        int sg = next_seg(blockIdx.x);
+        if (sg >= 0) load_q(p.segs[sg]);
+        while (sg >= 0 && ok) {
             const TileSeg it = p.segs[sg];
             const int start = it.start, steps = (it.blk1 - it.blk0 + 1) >> 1;
             const int r = half * 128 + row;                          // row of the segment
@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
             }
             if (!ok) break;
             // the next segment's Q: its first scores are computed while this one's result is stored
-            sg = next_seg(sg + 1);
-            if (sg < seg1) load_q(p.segs[sg]);
+            sg = next_seg(it.next);
+            if (sg >= 0) load_q(p.segs[sg]);
             if (!(ok = wait(&o_full[half], oc & 1u))) break;
             ++oc;
             tc_fence_after();
@@ -495,41 +495,42 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
 }
 
 // Joins the partials of tiles that were cut, in segment order.  A CTA takes 32
-// rows, a lane one of them and a warp 16 channels: partials are read as they
-// were written, 512 consecutive bytes per warp and load.
+// rows, a lane one row and a warp 4 * C channels: partials are read as they were
+// written, 512 consecutive bytes per warp and load, eight or more loads in flight.
+// Few joins have many parts each and want all SMs at once (C = 1: 17 parts of 8
+// tiles take 8.1 us, 12.5 with C = 4); many joins fill the SMs by themselves and
+// want whole sectors written and few CTAs (C = 4: 64 tiles of 2 parts take 6.7 us,
+// 11 with C = 1).
+template <int C>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const Params p, const TileJoin* joins) {
     pdl_wait();
     const TileJoin it = joins[blockIdx.x];
-    const int r = int(blockIdx.y) * 32 + int(threadIdx.x & 31), w = threadIdx.x >> 5;
+    const int r = int(blockIdx.y) * 32 + int(threadIdx.x & 31), c = (int(blockIdx.z) * 8 + int(threadIdx.x >> 5)) * C;
     if (r >= it.nrows) return;
     const float2* ml = p.part_ml + int64_t(it.part0) * 256 + r;
-    const float4* part = reinterpret_cast<const float4*>(p.part) + (int64_t(it.part0) * 32 + 4 * w) * 256 + r;
+    const float4* part = reinterpret_cast<const float4*>(p.part) + (int64_t(it.part0) * 32 + c) * 256 + r;
     float M = -INFINITY, L = 0.f;
+#pragma unroll 8
     for (int k = 0; k < it.n_parts; ++k) M = fmaxf(M, ml[k * 256].x);
-    float4 o[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+    float4 o[C] = {};
+#pragma unroll C == 1 ? 8 : 2
     for (int k = 0; k < it.n_parts; ++k) {
         const float2 e = ml[k * 256];
+        float4 a[C];
+        for (int j = 0; j < C; ++j) a[j] = part[(int64_t(k) * 32 + j) * 256];
         const float wt = M == -INFINITY ? 0.f : exp2f(e.x - M);
         L += wt * e.y;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const float4 a = part[(int64_t(k) * 32 + c) * 256];
-            o[c].x += wt * a.x; o[c].y += wt * a.y; o[c].z += wt * a.z; o[c].w += wt * a.w;
+        for (int j = 0; j < C; ++j) {
+            o[j].x += wt * a[j].x; o[j].y += wt * a[j].y; o[j].z += wt * a[j].z; o[j].w += wt * a[j].w;
         }
     }
     const Seq s = p.seqs[it.seq];
     const int row = it.row0 + r, tok = row / p.gq, head = it.head * p.gq + row - tok * p.gq;
     const float inv = L > 0.f ? 1.0f / L : 0.f;
-    __half* dst = p.out + int64_t(s.q_start + tok) * p.o_t + int64_t(head) * p.o_h + 16 * w;
-#pragma unroll
-    for (int c = 0; c < 4; c += 2)
-        *reinterpret_cast<uint4*>(dst + 4 * c) =
-            make_uint4(pack_f16x2(o[c].x * inv, o[c].y * inv), pack_f16x2(o[c].z * inv, o[c].w * inv),
-                       pack_f16x2(o[c + 1].x * inv, o[c + 1].y * inv), pack_f16x2(o[c + 1].z * inv, o[c + 1].w * inv));
-    if (p.lse && w == 0)
+    for (int j = 0; j < C; ++j)
+        *reinterpret_cast<uint2*>(p.out + int64_t(s.q_start + tok) * p.o_t + int64_t(head) * p.o_h + 4 * (c + j)) =
+            make_uint2(pack_f16x2(o[j].x * inv, o[j].y * inv), pack_f16x2(o[j].z * inv, o[j].w * inv));
+    if (p.lse && c == 0)
         p.lse[int64_t(s.q_start + tok) * p.q_heads + head] = L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
 }
 
@@ -551,7 +552,6 @@ int launch_tiles(const nova_paged_attn_args* a, const nova_paged_plan_info* info
     p.seqs = reinterpret_cast<const Seq*>(a->plan + info->seq_off);
     p.pages = a->plan + info->page_off;
     p.segs = reinterpret_cast<const TileSeg*>(a->plan + s.segs_off);
-    p.cta_first = a->plan + s.ctas_off;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     p.err = reinterpret_cast<int*>(ws);
     p.part = reinterpret_cast<float*>(ws + ws_rows_bytes(s, info->kv_heads));
@@ -572,8 +572,9 @@ int launch_tiles(const nova_paged_attn_args* a, const nova_paged_plan_info* info
     launch(tc::paged_attn_tile_kernel, dim3(unsigned(s.n_ctas)), dim3(tc::THREADS), tc::SMEM, stream, p);
     if (int rc = check_launch("paged attention")) return rc;
     if (!s.n_joins) return NOVA_OK;
-    launch(tc::paged_attn_join_kernel, dim3(unsigned(s.n_joins), 8), dim3(256), 0, stream, p,
-           reinterpret_cast<const TileJoin*>(a->plan + s.joins_off));
+    const bool few = s.n_joins <= 16;  // fewer CTAs of 8 per join than SMs
+    launch(few ? tc::paged_attn_join_kernel<1> : tc::paged_attn_join_kernel<4>, dim3(unsigned(s.n_joins), 8, few ? 4 : 1),
+           dim3(256), 0, stream, p, reinterpret_cast<const TileJoin*>(a->plan + s.joins_off));
     return check_launch("paged attention");
 }
 

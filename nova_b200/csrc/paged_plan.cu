@@ -159,9 +159,10 @@ void rows_schedule(Builder& b, const nova_paged_schedule& s, bool more, nova_pag
 // in a row, request by request and head by head so that neighbouring CTAs read
 // the same cache, cut so that no CTA takes more than a share; the smallest share
 // that the SMs can hold is searched.  A segment costs about SEG_COST steps
-// besides its own (its result, the pipeline's fill), and a tile is not cut into
-// pieces below MIN_STEPS.
-constexpr int64_t SEG_COST = 4, MIN_STEPS = 3;
+// besides its own (its result, the pipeline's fill; taken as 2, 3 or 4 it gave times
+// within 5 % of one another), and a tile is not cut into pieces below MIN_STEPS
+// (64 tokens over 500 cached: 25.6 us with 1, 28.7 with 3; longer caches alike).
+constexpr int64_t SEG_COST = 4, MIN_STEPS = 1;
 
 struct Tile {
     int64_t seq, head, row0, nrows, b0, b1, q_start;
@@ -218,26 +219,34 @@ void tile_schedule(Builder& b, nova_paged_schedule& s) {
         if (deal(tiles, mid, none) <= a.sms) hi = mid;
         else lo = mid + 1;
     }
-    std::vector<int32_t> ctas;
+    std::vector<TileSeg> segs, first, more;    // segs in tile order; the CTAs' first ones go to the front
+    std::vector<int64_t> opens;                // segs that open a CTA
     std::vector<TileJoin> joins;
-    s.segs_off = b.at();
-    int64_t segs = 0;
     deal(tiles, hi, [&](const Tile& t, int64_t b0, int64_t end, bool fresh) {
-        if (fresh) ctas.push_back(int32_t(segs));
+        if (fresh) opens.push_back(int64_t(segs.size()));
         const bool cut = b0 != t.b0 || end != t.b1;
         if (cut && b0 == t.b0)
             joins.push_back(TileJoin{int(t.seq), int(t.head), int(t.row0), int(t.nrows), int(s.n_tile_parts), 0, 0, 0});
         if (cut) ++joins.back().n_parts;
-        b.put(TileSeg{int(t.seq), int(t.head), int(t.row0), int(t.nrows), int(b0), int(end),
-                      cut ? int(s.n_tile_parts++) : -1, int(t.q_start), int(a.kv_lens[t.seq] - a.q_lens[t.seq]),
-                      int(a.kv_lens[t.seq]), int(a.page_off[t.seq]), a.kv_lens[t.seq] % PT ? int(a.tail_out[t.seq]) : 0,
-                      0, 0, 0, 0});
-        ++segs;
+        const int64_t kv = a.kv_lens[t.seq], off = a.page_off[t.seq];
+        TileSeg g{int(t.head), int(t.row0), int(t.nrows), int(b0), int(end), cut ? int(s.n_tile_parts++) : -1, int(t.q_start),
+                  int(kv - a.q_lens[t.seq]), int(kv), int(off), kv % PT ? int(a.tail_out[t.seq]) : 0, {-1, -1, -1, -1}, -1};
+        for (int w = 0; w < 4; ++w)
+            if (b0 + w < std::min(end, kv / PT)) g.page[w] = int(a.pages[off + b0 + w]);
+        segs.push_back(g);
     });
-    ctas.push_back(int32_t(segs));
-    s.n_ctas = int64_t(ctas.size()) - 1;
-    s.ctas_off = b.at();
-    b.v.insert(b.v.end(), ctas.begin(), ctas.end());
+    s.n_ctas = int64_t(opens.size());
+    s.n_segs = int64_t(segs.size());
+    opens.push_back(s.n_segs);
+    for (int64_t c = 0; c < s.n_ctas; ++c)
+        for (int64_t k = opens[c]; k < opens[c + 1]; ++k) {
+            TileSeg& g = segs[k];
+            if (k + 1 < opens[c + 1]) g.next = int(s.n_ctas + int64_t(more.size()) + (k > opens[c]));
+            (k == opens[c] ? first : more).push_back(g);
+        }
+    s.segs_off = b.at();
+    for (const TileSeg& g : first) b.put(g);
+    for (const TileSeg& g : more) b.put(g);
     s.joins_off = b.at();
     s.n_joins = int64_t(joins.size());
     for (const TileJoin& j : joins) b.put(j);

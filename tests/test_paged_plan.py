@@ -76,12 +76,19 @@ def test_every_row_sees_its_blocks_once(hq, hkv, window):
             seen.setdefault((seq, r), []).extend(range(b0, b1))
     tiles = {}
     sched = p.info.sched[0]
-    ctas = p.host[sched.ctas_off:sched.ctas_off + sched.n_ctas + 1].tolist()
-    assert ctas == sorted(set(ctas)) and len(ctas) <= 149
-    segs = p.host[sched.segs_off:sched.segs_off + 16 * ctas[-1]].reshape(-1, 16).tolist() if sched.n_ctas else []
-    for seq, head, row0, nrows, b0, b1, part, q_start, start, kv_len, page_off, tail, *_ in segs:
+    segs = p.host[sched.segs_off:sched.segs_off + 16 * sched.n_segs].reshape(-1, 16).tolist()
+    assert sched.n_ctas <= 148
+    order = []                                  # every CTA's segments, one CTA after another: the tiles in order
+    for cta in range(sched.n_ctas):
+        while cta >= 0:
+            order.append(segs[cta])
+            cta = segs[cta][15]
+    assert len(order) == len(segs) and sorted(map(tuple, order)) == sorted(map(tuple, segs))
+    for head, row0, nrows, b0, b1, part, q_start, start, kv_len, page_off, tail, *first in order:
+        seq = at[q_start]
         assert (q_start, start, kv_len) == (sum(q[:seq]), kv[seq] - q[seq], kv[seq])
         assert page_off == sum(n // PAGE for n in kv[:seq]) and (not kv_len % PAGE or tail == p.tail_out[seq])
+        assert first[:4] == [page_off + b if b < min(b1, kv_len // PAGE) else -1 for b in range(b0, b0 + 4)]
         assert b1 > b0 and 1 <= nrows <= 256
         tiles.setdefault((seq, head, row0, nrows), []).append((b0, b1, part))
     joins = p.host[sched.joins_off:sched.joins_off + 8 * sched.n_joins].reshape(-1, 8).tolist()
