@@ -1,20 +1,27 @@
 // Controls of each request on its next-token logits (penalties for repeated
 // tokens, token biases, grammar masks), and the history they read.
 //
-// One pass: a thread takes 8 consecutive tokens of a row -- 16 bytes of fp16
-// logits, 16 of history, 8 mask bits -- and writes them once, so the kernel is
-// bound by HBM for many rows and by one round of loads for one.  Vectors start
-// at the 16-byte boundary at or before the row (the row's first and last
-// vector go token by token); a row whose logits, history and output do not
-// share such a boundary goes token by token throughout.
+// One pass: a thread takes two vectors of 8 consecutive tokens of a row -- 16
+// bytes of fp16 logits, 16 of history, 8 mask bits each -- and writes them once.
+// Few tokens are in a history or biased, so a vector passes as it came with the
+// mask applied to its words, and those tokens are then done one by one in fp32
+// with one rounding (all tokens through fp32: 44 instructions each and 20.1 us
+// for 64 rows of 151936 fp16 logits, 16.4 this way; fewer registers and 1 or
+// 4 vectors a thread measured slower).  Bound by instruction issue (64 %
+// busy) and, in turns, HBM: 58.8 MB at 3.6 TB/s; one row is a launch and two
+// dependent loads, 5.0 us.  Vectors start at the 16-byte boundary at or before
+// the row (the row's first and last vector go token by token); a row whose
+// logits, history and output do not share such a boundary goes token by token
+// throughout.
 #include "common.cuh"
 
 namespace nova {
 namespace logits {
 
-constexpr int THREADS = 256;
-constexpr int VEC = 8;                  // tokens per thread
-constexpr int CHUNK = THREADS * VEC;    // tokens per CTA, and per bias list
+constexpr int THREADS = 128;
+constexpr int VEC = 8;                  // tokens per vector
+constexpr int NV = 2;                   // vectors per thread: what a row costs besides its tokens is half as much
+constexpr int CHUNK = THREADS * VEC * NV;   // tokens per CTA, and per bias list
 
 struct Params {
     const uint8_t* logits;
@@ -53,14 +60,11 @@ struct alignas(16) Vec {
     T v[VEC];
 };
 
-// Biases of a CTA's tokens up to this many go from lane to lane: each lane holds
-// one, and a warp takes those of its own tokens.  More go through shared memory.
-constexpr int FEW_BIASES = 64;
-
 template <typename T>
 __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) {
-    __shared__ __align__(16) float bias_s[CHUNK];
-    const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31;
+    __shared__ float bias_s[CHUNK];              // of the tokens whose bit is set
+    __shared__ __align__(8) uint32_t biased_s[CHUNK / 32];
+    const int row = blockIdx.y, chunk = blockIdx.x;
     const T* src = reinterpret_cast<const T*>(p.logits) + row * p.lstride;
     T* dst = reinterpret_cast<T*>(p.out) + row * p.ostride;
     const int16_t* hist = p.history ? p.history + row * p.hstride : nullptr;
@@ -70,102 +74,103 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
                      (reinterpret_cast<uintptr_t>(dst) - lead * sizeof(T)) % 16 == 0;
     const int base = chunk * CHUNK - lead;                     // first token of this CTA
     if (base >= p.vocab) return;
-    const int t0 = base + int(threadIdx.x) * VEC;
-    const bool whole = vec && t0 >= 0 && t0 + VEC <= p.vocab;
+    auto first = [&](int q) { return base + (q * THREADS + int(threadIdx.x)) * VEC; };   // of vector q
+    auto whole = [&](int q) { return vec && first(q) >= 0 && first(q) + VEC <= p.vocab; };
     pdl_wait();
 
     // loads that nothing waits for, all in flight
-    Vec<T> x;
-    Vec<int16_t> h;
+    Vec<T> x[NV];
+    uint4 h[NV];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        x.v[i] = from_float<T>(0.f);
-        h.v[i] = 0;
-    }
-    if (whole) {
-        const uint4* s = reinterpret_cast<const uint4*>(src + t0);
+    for (int q = 0; q < NV; ++q) {
+        h[q] = make_uint4(0u, 0u, 0u, 0u);
+        if (!whole(q)) continue;
+        const uint4* s = reinterpret_cast<const uint4*>(src + first(q));
 #pragma unroll
-        for (int i = 0; i < int(sizeof(x) / 16); ++i) reinterpret_cast<uint4*>(&x)[i] = s[i];
-        if (hist) *reinterpret_cast<uint4*>(&h) = *reinterpret_cast<const uint4*>(hist + t0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (t0 + i >= 0 && t0 + i < p.vocab) {
-                x.v[i] = src[t0 + i];
-                if (hist) h.v[i] = hist[t0 + i];
-            }
-    }
-    int e0 = 0, e1 = 0;       // biases of this CTA's tokens: they lie in its list and, with a lead, in the one before
-    if (p.bias_off) {
-        const int* off = p.bias_off + int64_t(row) * p.chunks;
-        e0 = off[min(max(chunk - (lead > 0), 0), p.chunks)];
-        e1 = off[min(chunk + 1, p.chunks)];
+        for (int i = 0; i < int(sizeof(x[q]) / 16); ++i) reinterpret_cast<uint4*>(&x[q])[i] = s[i];
+        if (hist) h[q] = *reinterpret_cast<const uint4*>(hist + first(q));
     }
     const int which = !p.allowed ? -1 : p.allowed_row ? p.allowed_row[row] : row;
+    // mask words of each vector's tokens (no mask: all set; none allowed: none set)
+    uint32_t mask[NV][2];
+    auto shift = [&](int q) { return max(first(q), 0) & 31; };
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+        mask[q][0] = mask[q][1] = which < p.n_masks ? ~0u : 0u;
+        if (which < 0 || which >= p.n_masks) continue;
+        const uint32_t* m = p.allowed + which * p.mask_stride;
+        const int w = max(first(q), 0) >> 5, words = (p.vocab + 31) / 32;
+        mask[q][0] = w < words ? m[w] : 0u;
+        mask[q][1] = shift(q) > 32 - VEC && w + 1 < words ? m[w + 1] : 0u;
+    }
     const float rep = p.repetition ? p.repetition[row] : 1.f;
-    const float inv = div_rn(1.f, rep);   // v * inv is within 2^-23 of v / rep, and no element waits for a division
     const float freq = p.frequency ? p.frequency[row] : 0.f;
     const float pres = p.presence ? p.presence[row] : 0.f;
-    // 8 mask bits of this thread's tokens (all set: no mask)
-    uint32_t keep = 0xFFu;
-    if (which >= p.n_masks) {
-        keep = 0u;
-    } else if (which >= 0) {
-        const uint32_t* m = p.allowed + which * p.mask_stride;
-        const int f = max(t0, 0), words = (p.vocab + 31) / 32, w = f >> 5;
-        const uint32_t lo = w < words ? m[w] : 0u;
-        const uint32_t hi = (f & 31) > 32 - VEC && w + 1 < words ? m[w + 1] : 0u;
-        keep = __funnelshift_r(lo, hi, f & 31) << (f - t0);
-    }
-    float b[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) b[i] = 0.f;
-    const int count = e1 - e0;                                 // the same in the whole CTA
-    if (count > 0 && count <= FEW_BIASES) {
-        for (int e = e0; e < e1; e += 32) {
-            const bool have = e + lane < e1;
-            const int token = have ? p.bias_token[e + lane] : -1;
-            const float value = have ? p.bias_value[e + lane] : 0.f;
-            const int first = t0 - lane * VEC;                 // this warp's first token
-            unsigned mine = __ballot_sync(0xffffffffu, have && token >= first && token < first + 32 * VEC);
-            for (; mine; mine &= mine - 1) {
-                const int l = __ffs(mine) - 1, k = __shfl_sync(0xffffffffu, token, l) - t0;
-                const float v = __shfl_sync(0xffffffffu, value, l);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) b[i] = k == i ? v : b[i];
-            }
-        }
-    } else if (count > 0) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) bias_s[i * THREADS + threadIdx.x] = 0.f;
+    if (p.bias_off) {         // of this CTA's tokens: they lie in its list and, with a lead, in the one before
+        const int* off = p.bias_off + int64_t(row) * p.chunks;
+        const int e0 = off[min(max(chunk - (lead > 0), 0), p.chunks)], e1 = off[min(chunk + 1, p.chunks)];
+        if (threadIdx.x < CHUNK / 32) biased_s[threadIdx.x] = 0u;
         __syncthreads();
         for (int e = e0 + threadIdx.x; e < e1; e += THREADS) {
+            const float value = p.bias_value[e];               // asked for beside the token
             const int at = p.bias_token[e] - base;
-            if (at >= 0 && at < CHUNK) bias_s[at] = p.bias_value[e];
+            if (at < 0 || at >= CHUNK) continue;
+            bias_s[at] = value;
+            atomicOr(&biased_s[at / 32], 1u << (at % 32));     // set bits do not depend on the order
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) b[i] = bias_s[int(threadIdx.x) * VEC + i];
     }
-    Vec<T> y;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        float v = to_float<T>(x.v[i]);
-        const int hi = h.v[i], times = hi & 0x7FFF;
-        v *= hi == 0 ? 1.f : v > 0.f ? inv : rep;
-        // times as a float: in the mantissa of 2^23, which is subtracted (a conversion runs at a quarter of the rate)
-        v -= times ? fmaf(freq, __int_as_float(0x4B000000 | times) - 8388608.f, pres) : 0.f;
-        v += b[i];
-        y.v[i] = from_float<T>((keep >> i) & 1u ? v : -INFINITY);
-    }
-    if (whole) {
-        uint4* d = reinterpret_cast<uint4*>(dst + t0);
+    for (int q = 0; q < NV; ++q) {
+        const int t0 = first(q), at0 = t0 - base;
+        const uint32_t keep = __funnelshift_r(mask[q][0], mask[q][1], shift(q)) << (max(t0, 0) - t0) & 0xFFu;
+        uint32_t todo = p.bias_off ? reinterpret_cast<const uint8_t*>(biased_s)[at0 / 8] : 0u;   // tokens that change
+        if (whole(q)) {
+            const uint32_t hw[4] = {h[q].x, h[q].y, h[q].z, h[q].w};
+            if (hw[0] | hw[1] | hw[2] | hw[3]) {
 #pragma unroll
-        for (int i = 0; i < int(sizeof(y) / 16); ++i) d[i] = reinterpret_cast<const uint4*>(&y)[i];
-    } else {
+                for (int i = 0; i < 4; ++i)
+                    todo |= (hw[i] & 0xFFFFu ? 1u << 2 * i : 0u) | (hw[i] >> 16 ? 2u << 2 * i : 0u);
+            }
+            if (keep != 0xFFu) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(&x[q]);
+                auto ones = [&](int i) { return uint32_t(int(keep << (31 - i)) >> 31); };   // all bits of token i's mask bit
+                if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (t0 + i >= 0 && t0 + i < p.vocab) dst[t0 + i] = y.v[i];
+                    for (int k = 0; k < VEC / 2; ++k) {
+                        const uint32_t m = __byte_perm(ones(2 * k), ones(2 * k + 1), 0x5410);
+                        w[k] = (w[k] & m) | (0xFC00FC00u & ~m);        // fp16 -inf
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) w[i] = (w[i] & ones(i)) | (0xFF800000u & ~ones(i));
+                }
+            }
+            // Most tokens are neither in the history nor biased: they leave as they came, unconverted, in whole
+            // vectors.  The others follow one by one, read again (an output that is the input still holds them).
+            uint4* d = reinterpret_cast<uint4*>(dst + t0);
+#pragma unroll
+            for (int i = 0; i < int(sizeof(x[q]) / 16); ++i) d[i] = reinterpret_cast<const uint4*>(&x[q])[i];
+            todo &= keep;
+        } else {              // token by token, those of the row
+            const uint32_t in = t0 >= p.vocab || t0 + VEC <= 0
+                                    ? 0u
+                                    : (0xFFu << max(-t0, 0) & 0xFFu) & (0xFFu >> max(t0 + VEC - p.vocab, 0));
+            for (uint32_t no = in & ~keep; no; no &= no - 1) dst[t0 + __ffs(no) - 1] = from_float<T>(-INFINITY);
+            todo = in & keep;
+        }
+        if (!todo) continue;
+        const float inv = div_rn(1.f, rep);   // v * inv is within 2^-23 of v / rep, and no element waits for a division
+        const uint32_t biased = p.bias_off ? reinterpret_cast<const uint8_t*>(biased_s)[at0 / 8] : 0u;
+        for (; todo; todo &= todo - 1) {
+            const int i = __ffs(todo) - 1, t = t0 + i;
+            float v = to_float<T>(src[t]);
+            const int seen = hist ? hist[t] : 0, times = seen & 0x7FFF;
+            v *= seen == 0 ? 1.f : v > 0.f ? inv : rep;
+            v -= times ? fmaf(freq, float(times), pres) : 0.f;
+            if (biased >> i & 1u) v += bias_s[at0 + i];
+            dst[t] = from_float<T>(v);
+        }
     }
 }
 
