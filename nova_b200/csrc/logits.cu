@@ -6,8 +6,8 @@
 // Few tokens are in a history or biased, so a vector passes as it came with the
 // mask applied to its words, and those tokens are then done one by one in fp32
 // with one rounding (all tokens through fp32: 44 instructions each and 20.1 us
-// for 64 rows of 151936 fp16 logits, 16.4 this way; fewer registers and 1 or
-// 4 vectors a thread measured slower).  Bound by instruction issue (64 %
+// for 64 rows of 151936 fp16 logits, 16.4 this way; fewer registers a thread
+// for more CTAs per SM: 16.8 to 17.3).  Bound by instruction issue (64 %
 // busy) and, in turns, HBM: 58.8 MB at 3.6 TB/s; one row is a launch and two
 // dependent loads, 5.0 us.  Vectors start at the 16-byte boundary at or before
 // the row (the row's first and last vector go token by token); a row whose
