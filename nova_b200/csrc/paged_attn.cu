@@ -14,7 +14,10 @@
 // operand: S^T = K Q^T, O^T += V^T P^T, tokens and channels permuted so that
 // every shared-memory read is 16 bytes and conflict-free.  P is transposed
 // between the two products by movmatrix.  A tile's splits are joined in split
-// order by the CTA that arrives last.
+// order by the CTA that arrives last.  Measured: 32 requests of 8000 to 32768
+// tokens with 8 KV heads, 1.26 GB, 213 us alone and 231 in a row (5.9 and 5.5
+// TB/s); 16 requests of 40 to 8191, 70 MB, 20 us (the items are about three
+// pages deep per warp: latency); one request of 77 tokens 5.2 us.
 #include "paged.cuh"
 
 namespace nova {
