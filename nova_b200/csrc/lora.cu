@@ -11,13 +11,13 @@
 //   * few rows (16-row tiles): one launch; each CTA goes on with an eighth of N;
 //   * many (64-row tiles): h goes through memory and a second launch takes the
 //     columns.  As one launch a cluster held its 8 CTAs for the whole of N, and
-//     37 of them did not fit the GPU at once: 93 us against 69 for 1.7k rows of
-//     19456 columns at rank 64 (15 us for the first product, 54 for the second:
+//     37 of them did not fit the GPU at once: 93 us against 68 for 1.7k rows of
+//     19456 columns at rank 64 (14 us for the first product, 53 for the second:
 //     149 MB of DRAM traffic, 23 us of it, and 20 us of mma.sync).
 // 64 rows with 24 adapters of rank up to 16, 2560 -> 6144: 6.5 us in one launch.
 // Fragments of mma.sync m16n8k16 are read straight from global memory: the
-// contraction index is permuted so that a lane's operand registers are 16 (x, A)
-// or 8 (B) consecutive bytes, and the columns of four neighbouring tiles are
+// contraction index is permuted so that a lane's operand registers are 16
+// consecutive bytes (8 of B and h at rank 16), and the columns of four neighbouring tiles are
 // dealt so that a lane's results are 16 consecutive bytes of base and out.
 #include <cooperative_groups.h>
 
@@ -56,7 +56,7 @@ __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 template <int RT, int MT>
 struct Shape {
     static constexpr int R = 8 * RT, TM = 16 * MT, KS = WARPS / MT;   // KS warps share a row tile's part of K
-    static constexpr int HP = R + 16;                                 // padded row of h: its reads hit all banks
+    static constexpr int HP = R == 16 ? 32 : R == 32 ? 32 : R + 32;   // padded row of h: its reads hit all banks
     static constexpr int RED = KS * TM * R * 4, H = TM * HP * 2;      // bytes of partial sums, of h
 };
 
@@ -129,6 +129,23 @@ struct Columns {
     uint4 ba[MW], bb[MW];
     uint2 w[4][S];
 
+    // The lane's first of the four entries along the rank that it holds in step s: two steps' are neighbours, so that
+    // they come in one load of 16 bytes (1.7k rows of 19456 columns at rank 64: 70.2 us with loads of 8, 68.4 with 16).
+    static __device__ __forceinline__ int entry(int s, int t) { return S == 1 ? 4 * t : 32 * (s / 2) + 8 * t + 4 * (s % 2); }
+    // Those entries of every step, `n` of them to be read at `p`.
+    static __device__ __forceinline__ void entries(const __half* p, int n, int t, uint2 (&v)[S]) {
+        if constexpr (S == 1) {
+            v[0] = 4 * t < n ? *reinterpret_cast<const uint2*>(p + 4 * t) : make_uint2(0u, 0u);
+        } else {
+#pragma unroll
+            for (int s = 0; s < S; s += 2) {
+                const uint4 q = entry(s, t) < n ? *reinterpret_cast<const uint4*>(p + entry(s, t)) : zero4();
+                v[s] = make_uint2(q.x, q.y);
+                v[s + 1] = make_uint2(q.z, q.w);
+            }
+        }
+    }
+
     __device__ __forceinline__ void load(const Params& p, const __half* bw, int rank, const int* row_of, int nb, int g, int t) {
         const int n0 = nb * 32, col = n0 + 8 * t;
         const bool in = col < p.n;
@@ -141,12 +158,7 @@ struct Columns {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int c = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                w[j][s] = make_uint2(0u, 0u);
-                if (rank > 16 * s + 4 * t && c < p.n)
-                    w[j][s] = *reinterpret_cast<const uint2*>(bw + int64_t(c) * p.max_rank + 16 * s + 4 * t);
-            }
+            entries(bw + int64_t(c) * p.max_rank, c < p.n ? rank : 0, t, w[j]);
         }
     }
 
@@ -157,7 +169,7 @@ struct Columns {
         const bool in = col < p.n;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const int left = rank - (16 * s + 4 * t);          // entries of this rank that the lane's four hold
+            const int left = rank - entry(s, t);               // entries of this rank that the lane's four hold
             if (left >= 4) continue;
             const uint32_t mx = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u, my = left == 3 ? 0xFFFFu : 0u;
 #pragma unroll
@@ -172,11 +184,22 @@ struct Columns {
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                const uint2 lo = *reinterpret_cast<const uint2*>(hs + (m * 16 + g) * hp + 16 * s + 4 * t);
-                const uint2 hi = *reinterpret_cast<const uint2*>(hs + (m * 16 + g + 8) * hp + 16 * s + 4 * t);
+            for (int s = 0; s < S; s += 2) {
+                uint4 lo, hi;
+                if constexpr (S == 1) {
+                    const uint2 a = *reinterpret_cast<const uint2*>(hs + (m * 16 + g) * hp + 4 * t);
+                    const uint2 b = *reinterpret_cast<const uint2*>(hs + (m * 16 + g + 8) * hp + 4 * t);
+                    lo = make_uint4(a.x, a.y, 0u, 0u);
+                    hi = make_uint4(b.x, b.y, 0u, 0u);
+                } else {
+                    lo = *reinterpret_cast<const uint4*>(hs + (m * 16 + g) * hp + entry(s, t));
+                    hi = *reinterpret_cast<const uint4*>(hs + (m * 16 + g + 8) * hp + entry(s, t));
+                }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma_16816(acc[j], lo.x, hi.x, lo.y, hi.y, w[j][s].x, w[j][s].y);
+                for (int j = 0; j < 4; ++j) {
+                    mma_16816(acc[j], lo.x, hi.x, lo.y, hi.y, w[j][s].x, w[j][s].y);
+                    if constexpr (S > 1) mma_16816(acc[j], lo.z, hi.z, lo.w, hi.w, w[j][s + 1].x, w[j][s + 1].y);
+                }
             }
             const uint32_t wa[4] = {ba[m].x, ba[m].y, ba[m].z, ba[m].w}, wb[4] = {bb[m].x, bb[m].y, bb[m].z, bb[m].w};
             uint32_t oa[4], ob[4];
@@ -295,7 +318,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
 constexpr int COLS = 512;
 
 template <int RT>
-__global__ void __launch_bounds__(THREADS, RT <= 8 ? 3 : 2) lora_expand_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, RT <= 4 ? 3 : 2) lora_expand_kernel(const Params p) {
     using S = Shape<RT, 4>;
     __shared__ __align__(16) __half hs[S::TM * S::HP];
     __shared__ int row_of[S::TM];
