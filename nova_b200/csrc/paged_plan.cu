@@ -96,14 +96,15 @@ void seen_blocks(const nova_paged_plan_args& a, int64_t i, int64_t row0, int64_t
 // Which kernel takes request i.  A tile of the few-rows kernel holds 16 query
 // rows of a KV head, the tensor-core kernel's 256; the first starts and joins
 // faster, the second reads the cache once.  16 requests of up to 4000 tokens:
-// 32 rows each 67 us there, 97 us here; one of 8192 tokens, 64 rows: 48 and 36.
+// up to 32 rows each 64 us there, 88 in the other (four of 1000: 25 and 44); one of
+// 8192 tokens, 64 rows: 47 and 29.
 constexpr int64_t FEW_ROWS = 2 * ROWS_MAX;
 bool few_rows(const nova_paged_plan_args& a, int64_t i) { return a.q_lens[i] * (a.q_heads / a.kv_heads) <= FEW_ROWS; }
 
 // Work lists of the few-rows kernel: requests of up to 4 rows, whose tiles keep
-// the weights' low parts at no cost, and of more.  Every tile's blocks are cut into splits of at
-// least one block per warp (4), at most 32 per tile so that joining them stays
-// short.  A CTA costs a few blocks' time to start and to join, so where splits
+// the weights' low parts at no cost, and of more.  Every tile's blocks are cut
+// into splits of at least one block per warp (4), at most 32 per tile so that
+// joining them stays short.  A CTA costs a few blocks' time to start and to join, so where splits
 // of up to 48 blocks let all CTAs be resident at once (3 per SM) the smallest
 // such size is taken; 16 requests of 8191 tokens: 70 us, 76 in splits of 16.
 // Beyond that about four times as many CTAs as are resident even out ragged
