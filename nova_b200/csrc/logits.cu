@@ -6,10 +6,11 @@
 // Few tokens are in a history or biased, so a vector passes as it came with the
 // mask applied to its words, and those tokens are then done one by one in fp32
 // with one rounding (all tokens through fp32: 44 instructions each and 20.1 us
-// for 64 rows of 151936 fp16 logits, 16.4 this way; fewer registers a thread
-// for more CTAs per SM: 16.8 to 17.3).  Bound by instruction issue (64 %
-// busy) and, in turns, HBM: 58.8 MB at 3.6 TB/s; one row is a launch and two
-// dependent loads, 5.0 us.  Vectors start at the 16-byte boundary at or before
+// for 64 rows of 151936 fp16 logits; this way 18.4; 16.4 since the biases are on
+// their way while the vectors are written; fewer registers a thread for more CTAs
+// per SM are slower).  Bound by instruction issue and the latency of a few waves
+// of CTAs, then HBM: 58.8 MB at 3.6 TB/s; one row is a launch and two
+// dependent loads, 4.9 us.  Vectors start at the 16-byte boundary at or before
 // the row (the row's first and last vector go token by token); a row whose
 // logits, history and output do not share such a boundary goes token by token
 // throughout.
@@ -106,35 +107,37 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
     const float rep = p.repetition ? p.repetition[row] : 1.f;
     const float freq = p.frequency ? p.frequency[row] : 0.f;
     const float pres = p.presence ? p.presence[row] : 0.f;
-    if (p.bias_off) {         // of this CTA's tokens: they lie in its list and, with a lead, in the one before
+    // Biases of this CTA's tokens: they lie in its list and, with a lead, in the one before.  Each thread's first is
+    // on its way while the vectors are written.
+    int e = 0, e1 = 0, at = -1;
+    float value = 0.f;
+    if (p.bias_off) {
         const int* off = p.bias_off + int64_t(row) * p.chunks;
-        const int e0 = off[min(max(chunk - (lead > 0), 0), p.chunks)], e1 = off[min(chunk + 1, p.chunks)];
+        e = off[min(max(chunk - (lead > 0), 0), p.chunks)] + int(threadIdx.x);
+        e1 = off[min(chunk + 1, p.chunks)];
         if (threadIdx.x < CHUNK / 32) biased_s[threadIdx.x] = 0u;
         __syncthreads();
-        for (int e = e0 + threadIdx.x; e < e1; e += THREADS) {
-            const float value = p.bias_value[e];               // asked for beside the token
-            const int at = p.bias_token[e] - base;
-            if (at < 0 || at >= CHUNK) continue;
-            bias_s[at] = value;
-            atomicOr(&biased_s[at / 32], 1u << (at % 32));     // set bits do not depend on the order
+        if (e < e1) {
+            value = p.bias_value[e];
+            at = p.bias_token[e] - base;
         }
-        __syncthreads();
     }
+    // Most tokens are neither in the history nor biased: they leave as they came, unconverted, in whole vectors.
+    uint32_t keep = 0u, todo = 0u;                             // 8 bits per vector: the mask's; tokens that change
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-        const int t0 = first(q), at0 = t0 - base;
-        const uint32_t keep = __funnelshift_r(mask[q][0], mask[q][1], shift(q)) << (max(t0, 0) - t0) & 0xFFu;
-        uint32_t todo = p.bias_off ? reinterpret_cast<const uint8_t*>(biased_s)[at0 / 8] : 0u;   // tokens that change
+        const int t0 = first(q);
+        const uint32_t k8 = __funnelshift_r(mask[q][0], mask[q][1], shift(q)) << (max(t0, 0) - t0) & 0xFFu;
         if (whole(q)) {
             const uint32_t hw[4] = {h[q].x, h[q].y, h[q].z, h[q].w};
             if (hw[0] | hw[1] | hw[2] | hw[3]) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    todo |= (hw[i] & 0xFFFFu ? 1u << 2 * i : 0u) | (hw[i] >> 16 ? 2u << 2 * i : 0u);
+                    todo |= (hw[i] & 0xFFFFu ? 1u << (VEC * q + 2 * i) : 0u) | (hw[i] >> 16 ? 2u << (VEC * q + 2 * i) : 0u);
             }
-            if (keep != 0xFFu) {
+            if (k8 != 0xFFu) {
                 uint32_t* w = reinterpret_cast<uint32_t*>(&x[q]);
-                auto ones = [&](int i) { return uint32_t(int(keep << (31 - i)) >> 31); };   // all bits of token i's mask bit
+                auto ones = [&](int i) { return uint32_t(int(k8 << (31 - i)) >> 31); };   // all bits of token i's mask bit
                 if constexpr (sizeof(T) == 2) {
 #pragma unroll
                     for (int k = 0; k < VEC / 2; ++k) {
@@ -146,31 +149,49 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
                     for (int i = 0; i < VEC; ++i) w[i] = (w[i] & ones(i)) | (0xFF800000u & ~ones(i));
                 }
             }
-            // Most tokens are neither in the history nor biased: they leave as they came, unconverted, in whole
-            // vectors.  The others follow one by one, read again (an output that is the input still holds them).
             uint4* d = reinterpret_cast<uint4*>(dst + t0);
 #pragma unroll
             for (int i = 0; i < int(sizeof(x[q]) / 16); ++i) d[i] = reinterpret_cast<const uint4*>(&x[q])[i];
-            todo &= keep;
+            keep |= k8 << VEC * q;
         } else {              // token by token, those of the row
             const uint32_t in = t0 >= p.vocab || t0 + VEC <= 0
                                     ? 0u
                                     : (0xFFu << max(-t0, 0) & 0xFFu) & (0xFFu >> max(t0 + VEC - p.vocab, 0));
-            for (uint32_t no = in & ~keep; no; no &= no - 1) dst[t0 + __ffs(no) - 1] = from_float<T>(-INFINITY);
-            todo = in & keep;
+            for (uint32_t no = in & ~k8; no; no &= no - 1) dst[t0 + __ffs(no) - 1] = from_float<T>(-INFINITY);
+            todo |= (in & k8) << VEC * q;
+            keep |= (in & k8) << VEC * q;
         }
-        if (!todo) continue;
-        const float inv = div_rn(1.f, rep);   // v * inv is within 2^-23 of v / rep, and no element waits for a division
-        const uint32_t biased = p.bias_off ? reinterpret_cast<const uint8_t*>(biased_s)[at0 / 8] : 0u;
-        for (; todo; todo &= todo - 1) {
-            const int i = __ffs(todo) - 1, t = t0 + i;
-            float v = to_float<T>(src[t]);
-            const int seen = hist ? hist[t] : 0, times = seen & 0x7FFF;
-            v *= seen == 0 ? 1.f : v > 0.f ? inv : rep;
-            v -= times ? fmaf(freq, float(times), pres) : 0.f;
-            if (biased >> i & 1u) v += bias_s[at0 + i];
-            dst[t] = from_float<T>(v);
+    }
+    uint32_t biased = 0u;
+    if (p.bias_off) {
+        while (e < e1) {
+            if (at >= 0 && at < CHUNK) {
+                bias_s[at] = value;
+                atomicOr(&biased_s[at / 32], 1u << (at % 32));     // set bits do not depend on the order
+            }
+            e += THREADS;
+            if (e < e1) {
+                value = p.bias_value[e];
+                at = p.bias_token[e] - base;
+            }
         }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < NV; ++q)
+            biased |= uint32_t(reinterpret_cast<const uint8_t*>(biased_s)[q * THREADS + threadIdx.x]) << VEC * q;
+    }
+    // The others follow one by one, read again (an output that is the input still holds them).
+    todo = (todo | biased) & keep;
+    if (!todo) return;
+    const float inv = div_rn(1.f, rep);   // v * inv is within 2^-23 of v / rep, and no element waits for a division
+    for (; todo; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1, own = (i / VEC * THREADS + int(threadIdx.x)) * VEC + i % VEC, t = base + own;
+        float v = to_float<T>(src[t]);
+        const int seen = hist ? hist[t] : 0, times = seen & 0x7FFF;
+        v *= seen == 0 ? 1.f : v > 0.f ? inv : rep;
+        v -= times ? fmaf(freq, float(times), pres) : 0.f;
+        if (biased >> i & 1u) v += bias_s[own];
+        dst[t] = from_float<T>(v);
     }
 }
 
