@@ -106,6 +106,26 @@ def test_controls_are_optional(cuda_lib, drop):
     check(adjust_logits(x.cuda(), **dev), want, size, torch.float16)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("lead,v,biases", [(0, 4096, 1500), (5, 6001, 4000), (7, 2050, 900), (1, 2047, 300)])
+def test_many_biases_in_place(cuda_lib, lead, v, biases, dtype):
+    """Bias lists longer than a CTA has threads; rows that begin inside a vector, where a CTA's tokens
+    lie in two lists; the result written over the logits by whole vectors."""
+    from nova_b200.logits import LogitBias, adjust_logits
+
+    rows, width = 3, -(-(v + lead) // 8) * 8
+    x, hist, rep, freq, pres, entries, allowed = make(rows, v, dtype, seed=v, masks=rows, biases=biases)
+    want, size = reference(x, hist, rep, freq, pres, entries, allowed, None)
+    logits = torch.full((rows, width), 3.0, dtype=dtype, device="cuda")
+    history = torch.zeros(rows, width, dtype=torch.int16, device="cuda")
+    logits[:, lead:lead + v], history[:, lead:lead + v] = x.cuda(), hist.cuda()
+    out = logits[:, lead:lead + v]
+    adjust_logits(out, history=history[:, lead:lead + v], repetition=rep.cuda(), frequency=freq.cuda(),
+                  presence=pres.cuda(), bias=LogitBias(entries, v), allowed=allowed.cuda(), out=out)
+    check(out, want, size, dtype)
+    assert (logits[:, :lead] == 3.0).all() and (logits[:, lead + v:] == 3.0).all()
+
+
 def test_masks_override_everything(cuda_lib):
     """NaN, infinities and the type's lowest value in masked places; a mask that leaves nothing; a
     mask number past the masks."""
