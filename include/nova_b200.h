@@ -603,6 +603,7 @@ typedef struct nova_paged_plan_args {
 typedef struct nova_paged_rows {
     int64_t off, n, rows_per_tile;             /* work items of few query rows   */
     int64_t n_parts;                           /* partial results of split items */
+    int64_t counters_off, parts_off;           /* in the workspace, bytes        */
 } nova_paged_rows;
 
 typedef struct nova_paged_schedule {
@@ -610,12 +611,15 @@ typedef struct nova_paged_schedule {
     nova_paged_rows rows[2];                   /* up to 4 rows per KV head; more */
     int64_t segs_off, n_segs, n_ctas;          /* segments of many query rows    */
     int64_t joins_off, n_joins, n_tile_parts;  /* tiles cut between CTAs         */
+    int64_t tile_parts_off;                    /* in the workspace, bytes        */
 } nova_paged_schedule;
 
 /* What a plan holds and where (offsets in int32 from the plan's start). */
 typedef struct nova_paged_plan_info {
     int64_t ints;             /* length of the plan                              */
     int64_t workspace_bytes;  /* nova_paged_attention's workspace, zeroed once   */
+    int64_t head_bytes;       /* of it: error word and arrival counters; every
+                               * schedule's partials lie behind them             */
     int64_t seqs, tokens, read_rows, q_heads, kv_heads;
     int64_t max_page, max_tail;                /* largest page / tail number used */
     int64_t max_pos;          /* largest position of a new token, -1: none       */

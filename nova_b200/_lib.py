@@ -128,21 +128,22 @@ class PagedPlanArgs(ctypes.Structure):
 class PagedRows(ctypes.Structure):
     """Mirror of ``nova_paged_rows``."""
 
-    _fields_ = [("off", _I), ("n", _I), ("rows_per_tile", _I), ("n_parts", _I)]
+    _fields_ = [("off", _I), ("n", _I), ("rows_per_tile", _I), ("n_parts", _I), ("counters_off", _I), ("parts_off", _I)]
 
 
 class PagedSchedule(ctypes.Structure):
     """Mirror of ``nova_paged_schedule``."""
 
     _fields_ = [("window", _I), ("rows", PagedRows * 2),
-                ("segs_off", _I), ("n_segs", _I), ("n_ctas", _I), ("joins_off", _I), ("n_joins", _I), ("n_tile_parts", _I)]
+                ("segs_off", _I), ("n_segs", _I), ("n_ctas", _I), ("joins_off", _I), ("n_joins", _I), ("n_tile_parts", _I),
+                ("tile_parts_off", _I)]
 
 
 class PagedPlanInfo(ctypes.Structure):
     """Mirror of ``nova_paged_plan_info``."""
 
     _fields_ = [
-        ("ints", _I), ("workspace_bytes", _I), ("seqs", _I), ("tokens", _I), ("read_rows", _I), ("q_heads", _I),
+        ("ints", _I), ("workspace_bytes", _I), ("head_bytes", _I), ("seqs", _I), ("tokens", _I), ("read_rows", _I), ("q_heads", _I),
         ("kv_heads", _I), ("max_page", _I), ("max_tail", _I), ("max_pos", _I), ("seq_off", _I), ("page_off", _I),
         ("pos_off", _I), ("open_off", _I), ("n_open", _I), ("write_off", _I), ("n_write", _I), ("read_off", _I), ("n_read", _I), ("n_windows", _I),
         ("sched", PagedSchedule * PAGED_MAX_WINDOWS),

@@ -39,18 +39,7 @@ struct Block {                  // one 64-token block of a request (write list: 
 constexpr int ROWS_MAX = 16;    // query rows of one KV head that the few-rows kernel takes per tile
 constexpr int PART = 132;       // floats per row of a few-rows partial: m, l, 2 unused, acc[128]
 
-// Workspace of nova_paged_attention: error word, arrival counters and partials
-// of the two few-rows lists, partials of cut tiles.
-constexpr int64_t WS_HEAD = 256;
-inline int64_t ws_counters(const nova_paged_schedule& s, int64_t kv_heads) {
-    return ((s.rows[0].n_parts + s.rows[1].n_parts) * kv_heads * 4 + 255) / 256 * 256;
-}
-inline int64_t ws_list(const nova_paged_rows& r, int64_t kv_heads) {
-    return (r.n_parts * kv_heads * r.rows_per_tile * PART * 4 + 255) / 256 * 256;
-}
-inline int64_t ws_rows_bytes(const nova_paged_schedule& s, int64_t kv_heads) {
-    return WS_HEAD + ws_counters(s, kv_heads) + ws_list(s.rows[0], kv_heads) + ws_list(s.rows[1], kv_heads);
-}
+constexpr int64_t WS_HEAD = 256;   // bytes of the workspace before the arrival counters: the error word
 
 // Element offset of K (j = 0) or V (j = 1) of a page or tail buffer.
 __host__ __device__ __forceinline__ int64_t half_off(int64_t index, int kv_heads, int head, int j) {

@@ -540,16 +540,13 @@ extern "C" int nova_paged_attention(const nova_paged_attn_args* a, const nova_pa
     CUtensorMap tm{};
     if (a->num_pages > 0)
         if (int rc = make_tmap_u8_rows128(&tm, a->codes, uint64_t(code_rows), PT)) return rc;
-    int64_t counters = WS_HEAD, part = WS_HEAD + ws_counters(s, info->kv_heads);
     for (const nova_paged_rows& list : s.rows) {
         p.items = reinterpret_cast<const RowsItem*>(a->plan + list.off);
         p.tile_rows = int(list.rows_per_tile);
-        p.counters = reinterpret_cast<unsigned*>(ws + counters);
-        p.part = reinterpret_cast<float*>(ws + part);
+        p.counters = reinterpret_cast<unsigned*>(ws + list.counters_off);
+        p.part = reinterpret_cast<float*>(ws + list.parts_off);
         if (list.n)
             if (int rc = launch_rows(p, tm, list, st)) return rc;
-        counters += list.n_parts * info->kv_heads * 4;
-        part += ws_list(list, info->kv_heads);
     }
     return NOVA_OK;
 }

@@ -565,7 +565,7 @@ int launch_tiles(const nova_paged_attn_args* a, const nova_paged_plan_info* info
     p.segs = reinterpret_cast<const TileSeg*>(a->plan + s.segs_off);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     p.err = reinterpret_cast<int*>(ws);
-    p.part = reinterpret_cast<float*>(ws + ws_rows_bytes(s, info->kv_heads));
+    p.part = reinterpret_cast<float*>(ws + s.tile_parts_off);
     p.part_ml = reinterpret_cast<float2*>(p.part + s.n_tile_parts * 256 * D);
     p.q_heads = int(info->q_heads);
     p.kv_heads = int(info->kv_heads);

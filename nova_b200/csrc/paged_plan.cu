@@ -254,6 +254,37 @@ void tile_schedule(Builder& b, nova_paged_schedule& s) {
     for (const TileJoin& j : joins) b.put(j);
 }
 
+// Where everything lies in the workspace of nova_paged_attention: the error
+// word, the arrival counters (every launch leaves them at zero, so the schedules
+// share them, with room for those of the largest), then the partials (dead after
+// their launch, so the schedules share them too).  No schedule's partials may
+// reach another's counters: launches of different schedules follow one another
+// on one workspace, and only the plan's start zeroes it.
+void place_workspace(nova_paged_plan_info& info) {
+    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    const int64_t heads = info.kv_heads;
+    info.head_bytes = WS_HEAD;
+    for (int64_t w = 0; w < info.n_windows; ++w) {
+        int64_t at = WS_HEAD;
+        for (nova_paged_rows& r : info.sched[w].rows) {
+            r.counters_off = at;
+            at += r.n_parts * heads * 4;
+        }
+        info.head_bytes = std::max(info.head_bytes, up(at));
+    }
+    info.workspace_bytes = info.head_bytes;
+    for (int64_t w = 0; w < info.n_windows; ++w) {
+        nova_paged_schedule& s = info.sched[w];
+        int64_t at = info.head_bytes;
+        for (nova_paged_rows& r : s.rows) {
+            r.parts_off = at;
+            at += up(r.n_parts * heads * r.rows_per_tile * PART * 4);
+        }
+        s.tile_parts_off = at;
+        info.workspace_bytes = std::max(info.workspace_bytes, at + s.n_tile_parts * 256 * (D + 2) * 4);
+    }
+}
+
 }  // namespace
 
 extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, int64_t capacity,
@@ -324,9 +355,8 @@ extern "C" int nova_paged_plan(const nova_paged_plan_args* args, int32_t* out, i
             rows_schedule(b, s, false, s.rows[0]);
             rows_schedule(b, s, true, s.rows[1]);
             tile_schedule(b, s);
-            const int64_t bytes = ws_rows_bytes(s, a.kv_heads) + s.n_tile_parts * 256 * (D + 2) * 4;
-            info->workspace_bytes = std::max(info->workspace_bytes, bytes);
         }
+        place_workspace(*info);
         info->ints = int64_t(b.v.size());
         if (out && capacity >= info->ints) memcpy(out, b.v.data(), b.v.size() * sizeof(int32_t));
         return NOVA_OK;
