@@ -700,7 +700,8 @@ typedef struct nova_paged_attn_args {
 NOVA_API int nova_paged_attention(const nova_paged_attn_args* args, const nova_paged_plan_info* info, void* stream);
 
 /* Error word of a nova_paged_attention workspace (non-zero: a bounded wait
- * gave up and that launch's output is not valid), copied and cleared. */
+ * gave up and that launch's output is not valid), copied and cleared on the
+ * legacy default stream: wait for the launch's own stream first. */
 NOVA_API int nova_paged_attention_read_error(void* workspace, int* host_value);
 
 /*

@@ -124,7 +124,10 @@ class PagePlan:
 
     def check_errors(self) -> None:
         """Raises RuntimeError when a bounded wait of an attention launch with
-        this plan gave up (its output is then not valid); synchronises."""
+        this plan gave up (its output is then not valid).  Waits for the work of
+        every stream of the device: the word is copied by the legacy default
+        stream, which does not wait for PyTorch's other streams."""
+        torch.cuda.synchronize(self.buffer.device)
         v = _lib.ctypes.c_int(0)
         _lib.call("nova_paged_attention_read_error", self.workspace.data_ptr(), byref(v))
         if v.value:
