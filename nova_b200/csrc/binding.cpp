@@ -274,7 +274,7 @@ PyObject* lora_add(PyObject* const* o) {
     return THPVariable_Wrap(out);
 }
 
-// (logits, history, repetition, frequency, presence, bias shape and pointers or None, allowed, allowed_row, out)
+// (logits, history, repetition, frequency, presence, LogitBias._handle or None, allowed, allowed_row, out)
 PyObject* adjust_logits(PyObject* const* a) {
     const Tensor& logits = tensor(a[0], "logits");
     const at::ScalarType type = logits.scalar_type();
@@ -303,15 +303,23 @@ PyObject* adjust_logits(PyObject* const* a) {
             if (!history) refuse(std::string(names[i]) + " needs a history");
             *to[i] = t->const_data_ptr();
         }
-    if (a[5] != Py_None) {                      // LogitBias._handle: rows, vocab, device, offsets, tokens, values
-        long long v[6];
-        if (!PyArg_ParseTuple(a[5], "LLLLLL", v, v + 1, v + 2, v + 3, v + 4, v + 5)) throw std::domain_error("");
-        if (v[0] != rows || v[1] != vocab || v[2] != device)
-            refuse("bias is for [" + std::to_string(v[0]) + ", " + std::to_string(v[1]) + "] logits on device " +
-                   std::to_string(v[2]) + ", got " + shape_of(logits));
-        p.bias_off = reinterpret_cast<const int32_t*>(v[3]);
-        p.bias_token = reinterpret_cast<const int32_t*>(v[4]);
-        p.bias_value = reinterpret_cast<const void*>(v[5]);
+    const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(c10::DeviceIndex(device));
+    if (a[5] != Py_None) {                      // LogitBias._handle: rows, vocab, number of biases, stream, buffer
+        long long v[4];
+        PyObject* held;
+        if (!PyTuple_Check(a[5])) refuse("bias must be a LogitBias");
+        if (!PyArg_ParseTuple(a[5], "LLLLO", v, v + 1, v + 2, v + 3, &held)) throw std::domain_error("");
+        const Tensor& list = tensor(held, "the bias list");
+        if (v[0] != rows || v[1] != vocab || !on(list, device))
+            refuse("bias is for [" + std::to_string(v[0]) + ", " + std::to_string(v[1]) + "] logits on " +
+                   list.device().str() + ", got " + shape_of(logits));
+        if (v[2] > 0) {                         // offsets, then tokens, then values; no biases: no pointers
+            p.bias_off = static_cast<const int32_t*>(list.const_data_ptr());
+            p.bias_token = p.bias_off + (list.numel() - 2 * v[2]);
+            p.bias_value = p.bias_token + v[2];
+            // a stream other than the list's own reads it: the allocator must know
+            if (reinterpret_cast<int64_t>(stream.stream()) != v[3]) list.record_stream(stream.unwrap());
+        }
     }
     const Tensor *allowed = optional(a[6], "allowed"), *which = optional(a[7], "allowed_row");
     if (allowed) {
@@ -342,7 +350,7 @@ PyObject* adjust_logits(PyObject* const* a) {
     }
     p.out = out.mutable_data_ptr();
     p.out_stride = rows > 1 ? out.stride(0) : vocab;
-    done(nova_adjust_logits(&p, c10::cuda::getCurrentCUDAStream(c10::DeviceIndex(device)).stream()), "nova_adjust_logits");
+    done(nova_adjust_logits(&p, stream.stream()), "nova_adjust_logits");
     return THPVariable_Wrap(out);
 }
 

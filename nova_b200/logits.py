@@ -49,9 +49,8 @@ class LogitBias:
         m = len(off)
         self.off, self.token = self.buffer[:m], self.buffer[m:m + n]
         self.value = self.buffer[m + n:].view(torch.float32)
-        at = self.buffer.data_ptr()           # what csrc/binding.cpp reads; no biases: no pointers
-        self._handle = (self.rows, self.vocab, self.buffer.get_device(),
-                        *((at, at + 4 * m, at + 4 * (m + n)) if n else (0, 0, 0)))
+        own = _lib.stream_of(self.buffer.device) if self.buffer.is_cuda else 0
+        self._handle = (self.rows, self.vocab, n, own, self.buffer)      # what csrc/binding.cpp reads
 
 
 def new_history(rows: int, vocab: int, device: torch.device | str = "cuda") -> torch.Tensor:
