@@ -323,6 +323,18 @@ def stream_of(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+ctypes.pythonapi.PyCapsule_New.restype = ctypes.py_object
+ctypes.pythonapi.PyCapsule_New.argtypes = [_P, ctypes.c_char_p, _P]
+PAGE_PLAN, LORA_PLAN = b"nova_b200.PagePlan", b"nova_b200.LoraPlan"   # capsule names; csrc/binding.cpp asks for them
+
+
+def handle(fields: ctypes.Array, name: bytes):
+    """What the compiled binding takes a plan by: a capsule over its fields, which
+    the plan keeps alive.  Its name tells one kind of plan from another, and it
+    cannot be copied or pickled, so no copy of a plan points at another's memory."""
+    return ctypes.pythonapi.PyCapsule_New(ctypes.addressof(fields), name, None)
+
+
 _fast = None
 
 

@@ -32,13 +32,15 @@ std::string shape_of(const Tensor& t) {
     return s + "] on " + t.device().str();
 }
 
-// The plan's side: PagePlan._handle / LoraPlan._handle point at one of these
-// (written by Python as consecutive int64).
+// The plan's side: PagePlan._handle / LoraPlan._handle are capsules over one of
+// these (written by Python as consecutive int64), named after the plan's class.
 struct PageHandle {
+    static constexpr const char* name = "nova_b200.PagePlan";
     const nova_paged_plan_info* info;
     int64_t buffer, workspace, workspace_bytes, device, stream;
 };
 struct LoraHandle {
+    static constexpr const char* name = "nova_b200.LoraPlan";
     int64_t tiles, workspace, workspace_bytes, device, stream;
     int64_t n_tiles, tile_rows, tokens, adapters, top_rank;
 };
@@ -46,13 +48,16 @@ struct LoraHandle {
 PyObject* handle_name;     // "_handle"
 PyObject* other_name;      // "_on_other_stream"
 
-const void* handle_of(PyObject* plan) {
+template <typename H>
+const H& handle_of(PyObject* plan) {
     PyObject* h = PyObject_GetAttr(plan, handle_name);
     if (!h) throw std::domain_error("");                      // the Python error is set
-    const void* p = PyLong_AsVoidPtr(h);
-    Py_DECREF(h);
-    if (!p) refuse("the plan is not on a CUDA device");
-    return p;
+    const bool host = PyLong_Check(h), mine = !host && PyCapsule_IsValid(h, H::name);
+    const void* p = mine ? PyCapsule_GetPointer(h, H::name) : nullptr;
+    Py_DECREF(h);                                             // the plan holds it, and what it points at
+    if (host) refuse("the plan is not on a CUDA device");
+    if (!mine) refuse(std::string("the plan must be a ") + H::name + ", got " + Py_TYPE(plan)->tp_name);
+    return *static_cast<const H*>(p);
 }
 
 // The current stream; where it is not the plan's own, the plan tells the allocator.
@@ -123,7 +128,7 @@ double number(PyObject* o, double otherwise) {
 
 // (qkv, codes, scales, tails, plan, q_norm_weight, k_norm_weight, eps, cos, sin, out)
 PyObject* qkv_append(PyObject* const* a) {
-    const PageHandle& h = *static_cast<const PageHandle*>(handle_of(a[4]));
+    const PageHandle& h = handle_of<PageHandle>(a[4]);
     const nova_paged_plan_info& info = *h.info;
     const Cache c = cache(a + 1, h);
     const Tensor& qkv = tensor(a[0], "qkv");
@@ -172,7 +177,7 @@ PyObject* qkv_append(PyObject* const* a) {
 
 // (codes, scales, tails, plan)
 PyObject* paged_read(PyObject* const* a) {
-    const PageHandle& h = *static_cast<const PageHandle*>(handle_of(a[3]));
+    const PageHandle& h = handle_of<PageHandle>(a[3]);
     const Cache c = cache(a, h);
     const Tensor k = empty({h.info->read_rows, h.info->kv_heads, D}, at::kHalf, h.device);
     const Tensor v = empty({h.info->read_rows, h.info->kv_heads, D}, at::kHalf, h.device);
@@ -188,7 +193,7 @@ PyObject* paged_read(PyObject* const* a) {
 
 // (q, codes, scales, tails, plan, window, scale, out, lse_out)
 PyObject* paged_attention(PyObject* const* a) {
-    const PageHandle& h = *static_cast<const PageHandle*>(handle_of(a[4]));
+    const PageHandle& h = handle_of<PageHandle>(a[4]);
     const nova_paged_plan_info& info = *h.info;
     const Cache c = cache(a + 1, h);
     const Tensor& q = tensor(a[0], "q");
@@ -229,7 +234,7 @@ PyObject* paged_attention(PyObject* const* a) {
 
 // (x, base, a, b, plan, scaling, out)
 PyObject* lora_add(PyObject* const* o) {
-    const LoraHandle& h = *static_cast<const LoraHandle*>(handle_of(o[4]));
+    const LoraHandle& h = handle_of<LoraHandle>(o[4]);
     const Tensor &x = tensor(o[0], "x"), &base = tensor(o[1], "base"), &a = tensor(o[2], "a"), &b = tensor(o[3], "b");
     if (x.dim() != 2 || base.dim() != 2 || a.dim() != 3) refuse("x and base must be 2-D, a and b 3-D");
     const int64_t k = x.size(1), n = base.size(1), r = a.size(1);

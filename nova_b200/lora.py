@@ -79,7 +79,7 @@ class LoraPlan:
             self._fields = (_lib.ctypes.c_int64 * 10)(
                 self.buffer.data_ptr(), self.workspace.data_ptr(), need.value, self.buffer.get_device(),
                 _lib.stream_of(self.buffer.device), self.n_tiles, self.tile_rows, self.tokens, self.adapters, self.max_rank)
-            self._handle = _lib.ctypes.addressof(self._fields)
+            self._handle = _lib.handle(self._fields, _lib.LORA_PLAN)
 
     def _on_other_stream(self) -> None:
         """A stream other than the plan's own uses its buffers: the allocator must know."""

@@ -114,7 +114,7 @@ class PagePlan:
             self._fields = (_lib.ctypes.c_int64 * 6)(
                 addressof(self.info), self.buffer.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(),
                 self.buffer.get_device(), _lib.stream_of(self.buffer.device))
-            self._handle = addressof(self._fields)
+            self._handle = _lib.handle(self._fields, _lib.PAGE_PLAN)
 
     def _on_other_stream(self) -> None:
         """A stream other than the plan's own uses its buffers: the allocator must know."""
