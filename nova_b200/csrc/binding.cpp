@@ -4,10 +4,12 @@
 // a small step run; here it is 3 to 4, of which the launch is most.
 //
 // Every function raises ValueError for arguments that do not fit, before
-// anything is launched, as the ctypes wrappers do.
+// anything is launched, and works on its tensors' device, whichever is current:
+// a stream handle alone does not say which device it belongs to.
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <stdexcept>
@@ -129,6 +131,7 @@ double number(PyObject* o, double otherwise) {
 // (qkv, codes, scales, tails, plan, q_norm_weight, k_norm_weight, eps, cos, sin, out)
 PyObject* qkv_append(PyObject* const* a) {
     const PageHandle& h = handle_of<PageHandle>(a[4]);
+    const c10::cuda::CUDAGuard guard(c10::DeviceIndex(h.device));
     const nova_paged_plan_info& info = *h.info;
     const Cache c = cache(a + 1, h);
     const Tensor& qkv = tensor(a[0], "qkv");
@@ -178,6 +181,7 @@ PyObject* qkv_append(PyObject* const* a) {
 // (codes, scales, tails, plan)
 PyObject* paged_read(PyObject* const* a) {
     const PageHandle& h = handle_of<PageHandle>(a[3]);
+    const c10::cuda::CUDAGuard guard(c10::DeviceIndex(h.device));
     const Cache c = cache(a, h);
     const Tensor k = empty({h.info->read_rows, h.info->kv_heads, D}, at::kHalf, h.device);
     const Tensor v = empty({h.info->read_rows, h.info->kv_heads, D}, at::kHalf, h.device);
@@ -194,6 +198,7 @@ PyObject* paged_read(PyObject* const* a) {
 // (q, codes, scales, tails, plan, window, scale, out, lse_out)
 PyObject* paged_attention(PyObject* const* a) {
     const PageHandle& h = handle_of<PageHandle>(a[4]);
+    const c10::cuda::CUDAGuard guard(c10::DeviceIndex(h.device));
     const nova_paged_plan_info& info = *h.info;
     const Cache c = cache(a + 1, h);
     const Tensor& q = tensor(a[0], "q");
@@ -235,6 +240,7 @@ PyObject* paged_attention(PyObject* const* a) {
 // (x, base, a, b, plan, scaling, out)
 PyObject* lora_add(PyObject* const* o) {
     const LoraHandle& h = handle_of<LoraHandle>(o[4]);
+    const c10::cuda::CUDAGuard guard(c10::DeviceIndex(h.device));
     const Tensor &x = tensor(o[0], "x"), &base = tensor(o[1], "base"), &a = tensor(o[2], "a"), &b = tensor(o[3], "b");
     if (x.dim() != 2 || base.dim() != 2 || a.dim() != 3) refuse("x and base must be 2-D, a and b 3-D");
     const int64_t k = x.size(1), n = base.size(1), r = a.size(1);
@@ -286,6 +292,7 @@ PyObject* adjust_logits(PyObject* const* a) {
     if (!logits.is_cuda() || logits.dim() != 2 || (type != at::kHalf && type != at::kFloat) || logits.stride(1) != 1)
         refuse("logits must be CUDA float16 or float32 [rows, vocab] with a contiguous last dimension, got " + shape_of(logits));
     const int64_t rows = logits.size(0), vocab = logits.size(1), device = logits.get_device();
+    const c10::cuda::CUDAGuard guard(c10::DeviceIndex(device));
     nova_logits_args p{};
     p.rows = rows;
     p.vocab = vocab;

@@ -75,8 +75,9 @@ def _history_add(history: torch.Tensor, tokens: torch.Tensor, offsets: torch.Ten
     elif (offsets.dtype != torch.int32 or tuple(offsets.shape) != (rows + 1,) or offsets.device != history.device
           or not offsets.is_contiguous()):
         raise ValueError(f"offsets must be contiguous int32 [{rows + 1}] on the history's device")
-    _lib.call("nova_history_add", history.data_ptr(), history.stride(0), tokens.data_ptr(), _lib.ptr(offsets),
-              tokens.numel(), rows, vocab, int(prompt), _lib.stream_of(history.device))
+    with torch.cuda.device(history.device):       # the launch goes to the current device
+        _lib.call("nova_history_add", history.data_ptr(), history.stride(0), tokens.data_ptr(), _lib.ptr(offsets),
+                  tokens.numel(), rows, vocab, int(prompt), _lib.stream_of(history.device))
 
 
 def add_prompt(history: torch.Tensor, tokens: torch.Tensor, offsets: torch.Tensor | None = None) -> None:

@@ -129,7 +129,8 @@ class PagePlan:
         stream, which does not wait for PyTorch's other streams."""
         torch.cuda.synchronize(self.buffer.device)
         v = _lib.ctypes.c_int(0)
-        _lib.call("nova_paged_attention_read_error", self.workspace.data_ptr(), byref(v))
+        with torch.cuda.device(self.buffer.device):
+            _lib.call("nova_paged_attention_read_error", self.workspace.data_ptr(), byref(v))
         if v.value:
             raise RuntimeError(f"paged attention: a bounded wait gave up (code {v.value})")
 
