@@ -780,7 +780,7 @@ NOVA_API int nova_adjust_logits(const nova_logits_args* args, void* stream);
 /* Enters tokens in the history: int64 tokens[off[r] .. off[r + 1]) of row r
  * (off int32 [rows + 1]; NULL: one token per row).  prompt != 0: sets the top
  * bit; else adds one to the count (up to 32767).  Tokens outside [0, vocab)
- * are skipped. */
+ * are skipped, and so are offsets outside [0, n_tokens]. */
 NOVA_API int nova_history_add(void* history, int64_t history_stride, const int64_t* tokens, const int32_t* off,
                               int64_t n_tokens, int64_t rows, int64_t vocab, int prompt, void* stream);
 

@@ -196,14 +196,16 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
 }
 
 // A count or a prompt bit lives in half of a 32-bit word; both updates are
-// whole-number atomics on that word, so their order does not matter.
-__global__ void history_add_kernel(int16_t* history, int64_t stride, const int64_t* tokens, const int* off, int rows,
-                                   int vocab, int prompt) {
+// whole-number atomics on that word, so their order does not matter.  The
+// offsets are device data that the host has not seen: what they name outside the
+// n_tokens tokens is not read.
+__global__ void history_add_kernel(int16_t* history, int64_t stride, const int64_t* tokens, int64_t n_tokens,
+                                   const int* off, int vocab, int prompt) {
     pdl_wait();
     const int row = blockIdx.y;
-    const int64_t n = off ? off[row + 1] - off[row] : 1, first = off ? off[row] : row;
-    for (int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
-        const int64_t t = tokens[first + i];
+    const int64_t first = off ? max(off[row], 0) : row, end = off ? min(int64_t(off[row + 1]), n_tokens) : row + 1;
+    for (int64_t i = first + blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < end; i += int64_t(gridDim.x) * blockDim.x) {
+        const int64_t t = tokens[i];
         if (t < 0 || t >= vocab) continue;
         const uintptr_t at = reinterpret_cast<uintptr_t>(history + row * stride + t);
         unsigned* word = reinterpret_cast<unsigned*>(at & ~uintptr_t(3));
@@ -285,7 +287,7 @@ extern "C" int nova_history_add(void* history, int64_t history_stride, const int
     const int64_t per_row = off ? (n_tokens + rows - 1) / rows : 1;
     const unsigned gx = unsigned(std::min<int64_t>(32, (per_row + 255) / 256));
     launch(logits::history_add_kernel, dim3(gx, unsigned(rows)), dim3(off ? 256 : 32), 0,
-           static_cast<cudaStream_t>(stream), static_cast<int16_t*>(history), history_stride, tokens,
-           static_cast<const int*>(off), int(rows), int(vocab), prompt);
+           static_cast<cudaStream_t>(stream), static_cast<int16_t*>(history), history_stride, tokens, n_tokens,
+           static_cast<const int*>(off), int(vocab), prompt);
     return check_launch("history add");
 }

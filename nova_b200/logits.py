@@ -83,7 +83,7 @@ def _history_add(history: torch.Tensor, tokens: torch.Tensor, offsets: torch.Ten
 def add_prompt(history: torch.Tensor, tokens: torch.Tensor, offsets: torch.Tensor | None = None) -> None:
     """Enter prompt tokens: int64, row r's are ``tokens[offsets[r]:offsets[r + 1]]``
     (int32 offsets on the device; without them one token per row).  Tokens
-    outside the vocabulary are skipped."""
+    outside the vocabulary and offsets outside the tokens are skipped."""
     _history_add(history, tokens, offsets, True)
 
 
