@@ -6,8 +6,11 @@
 // chain x A^T -> h -> h B^T.  The first product is split over K between the 8
 // CTAs of a cluster, whose partial sums (rows x rank, fp32) meet in distributed
 // shared memory and are added in CTA order.  h is rounded to fp16 for the second
-// product (2^-11 of the adapter's term, which is added to base in fp32 before the
-// one rounding of the result).
+// product: each row is first multiplied by the power of two that brings its
+// largest entry to [2^14, 2^15), and that power and the adapter's scaling go on
+// the fp32 sums of the second product.  So the error is 2^-11 of the sum of
+// |s h_j B_j| at any size of x, A and s (entries 2^-28 below the row's largest
+// lose bits), and the result is rounded once, with base.
 //   * few rows (16-row tiles): one launch; each CTA goes on with an eighth of N;
 //   * many (64-row tiles): h goes through memory and a second launch takes the
 //     columns.  As one launch a cluster held its 8 CTAs for the whole of N, and
@@ -44,11 +47,15 @@ struct Params {
     const float* scaling;
     const int* tiles;            // per tile: adapter, rank, rows, 0, then the rows (padded to the tile with -1)
     __half* h;                   // 64-row tiles: the first product, [tile][64][R]
+    float* factor;               // and what its rows are to be multiplied by, [tile][64]
     int k, n, max_rank, copy;    // copy: rows without an adapter are copied (out is not base)
 };
 
 // The rank that the kernels are built for: what h has room for.
 inline int64_t rank_tile(int64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+// h and its rows' factors of 64-row tiles.
+inline int64_t h_bytes(int64_t tiles, int64_t r) { return tiles * 64 * r * 2; }
+inline int64_t workspace_bytes(int64_t tiles, int64_t r) { return h_bytes(tiles, r) + tiles * 64 * 4; }
 
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
@@ -104,22 +111,53 @@ __device__ __forceinline__ void shrink(const Params& p, int adapter, int rank, c
     }
 }
 
-// CTA i of the cluster adds the i-th eighth of h over all CTAs, in CTA order, and
-// hands each pair of elements to put(row, column, pair).
-template <int RT, int MT, typename Put>
-__device__ __forceinline__ void gather(cg::cluster_group& cluster, float* red, int cr, float scale, Put&& put) {
-    using S = Shape<RT, MT>;
-    constexpr int SHARE = S::TM * S::R / CLUSTER / 2;
-    for (int i = threadIdx.x; i < SHARE; i += THREADS) {
-        const int at = cr * SHARE + i;
+// What a row of h is multiplied by before it is rounded to fp16, and what undoes
+// it: the powers of two that bring its largest magnitude to [2^14, 2^15).  A sum
+// of products of fp16 numbers is a multiple of 2^-48 below 2^63; a row of zeros
+// takes the clamped power, and one that is not finite stays so.
+struct Power {
+    float to, back;
+};
+__device__ __forceinline__ Power row_power(float largest) {
+    const int e = max(int(__float_as_uint(largest) >> 23) - 127, -100);
+    return {__uint_as_float(uint32_t(127 + 14 - e) << 23), __uint_as_float(uint32_t(127 + e - 14) << 23)};
+}
+// Largest of N consecutive lanes, in all of them.
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int off = N / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+    return v;
+}
+
+// CTA i of the cluster adds the i-th eighth of h over all CTAs, in CTA order, a
+// warp one row: fp16 rows to h_out, what they are to be multiplied by to f_out.
+template <int RT>
+__device__ __forceinline__ void gather(cg::cluster_group& cluster, float* red, int cr, float scale, __half* h_out, float* f_out) {
+    using S = Shape<RT, 4>;
+    static_assert(S::TM / CLUSTER == WARPS, "a row of h per warp");
+    constexpr int N = (S::R / 2 + 31) / 32;                    // pairs per lane
+    const int row = cr * WARPS + int(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    float2 s[N];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int at = min(lane + 32 * i, S::R / 2 - 1);       // ranks up to 32: the last pair again
         float2 v[CLUSTER];
 #pragma unroll
-        for (int k = 0; k < CLUSTER; ++k) v[k] = reinterpret_cast<const float2*>(cluster.map_shared_rank(red, k))[at];
-        float2 s = v[0];
+        for (int k = 0; k < CLUSTER; ++k)
+            v[k] = reinterpret_cast<const float2*>(cluster.map_shared_rank(red, k))[row * (S::R / 2) + at];
+        s[i] = v[0];
 #pragma unroll
-        for (int k = 1; k < CLUSTER; ++k) s = make_float2(s.x + v[k].x, s.y + v[k].y);
-        put(2 * at / S::R, 2 * at % S::R, __floats2half2_rn(s.x * scale, s.y * scale));
+        for (int k = 1; k < CLUSTER; ++k) s[i] = make_float2(s[i].x + v[k].x, s[i].y + v[k].y);
+        top = fmaxf(top, fmaxf(fabsf(s[i].x), fabsf(s[i].y)));
     }
+    const Power pw = row_power(lanes_max<32>(top));
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (lane + 32 * i < S::R / 2)
+            *reinterpret_cast<__half2*>(h_out + row * S::R + 2 * (lane + 32 * i)) = __floats2half2_rn(s[i].x * pw.to, s[i].y * pw.to);
+    if (lane == 0) f_out[row] = pw.back * scale;
 }
 
 // 32 columns of the second product for MW row tiles of 16, B in registers once.
@@ -162,9 +200,9 @@ struct Columns {
         }
     }
 
-    // hs: the first row tile's h, rows of hp elements.
-    __device__ __forceinline__ void finish(const Params& p, const __half* hs, int hp, int rank, const int* row_of, int nb, int g,
-                                           int t) {
+    // hs: the first row tile's h, rows of hp elements; factor: what each row of the product is multiplied by.
+    __device__ __forceinline__ void finish(const Params& p, const __half* hs, int hp, const float* factor, int rank,
+                                           const int* row_of, int nb, int g, int t) {
         const int col = nb * 32 + 8 * t;
         const bool in = col < p.n;
 #pragma unroll
@@ -180,6 +218,7 @@ struct Columns {
         }
 #pragma unroll
         for (int m = 0; m < MW; ++m) {
+            const float xa = factor[m * 16 + g], xb = factor[m * 16 + g + 8];
             float acc[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
@@ -207,8 +246,8 @@ struct Columns {
             for (int j = 0; j < 4; ++j) {
                 const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&wa[j]));
                 const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&wb[j]));
-                oa[j] = pack_f16x2(fa.x + acc[j][0], fa.y + acc[j][1]);
-                ob[j] = pack_f16x2(fb.x + acc[j][2], fb.y + acc[j][3]);
+                oa[j] = pack_f16x2(fmaf(acc[j][0], xa, fa.x), fmaf(acc[j][1], xa, fa.y));
+                ob[j] = pack_f16x2(fmaf(acc[j][2], xb, fb.x), fmaf(acc[j][3], xb, fb.y));
             }
             const int ra = row_of[m * 16 + g], rb = row_of[m * 16 + g + 8];
             if (in && ra >= 0) *reinterpret_cast<uint4*>(p.out + ra * p.out_stride + col) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
@@ -248,6 +287,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
     float* from = reinterpret_cast<float*>(smem + S::RED);     // [CLUSTER][E]
     __half* hs = reinterpret_cast<__half*>(smem + S::RED + CLUSTER * E * 4);
     __shared__ int row_of[S::TM];
+    __shared__ float factor[S::TM];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int cr = int(blockIdx.x) % CLUSTER;
     pdl_wait();
@@ -276,24 +316,40 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
         for (int k = 0; k < CLUSTER; ++k) cluster.map_shared_rank(from, k)[cr * E + i] = v;
     }
     cluster.sync();         // every CTA's sums are here; no CTA touches another's memory from now on
-    for (int i = threadIdx.x; i < E; i += THREADS) {
-        float v = from[i];
+    // a warp adds up two rows: lanes 0-15 and 16-31 one each at rank 16, all lanes one after the other above
+    constexpr int N = 2 * S::R / 32, PER = S::R <= 32 ? 1 : S::R / 32;   // elements per lane; of one row
+    float v[N];
 #pragma unroll
-        for (int k = 1; k < CLUSTER; ++k) v += from[k * E + i];
-        hs[i / S::R * S::HP + i % S::R] = __float2half_rn(v * scale);
+    for (int i = 0; i < N; ++i) {
+        const int at = warp * 2 * S::R + 32 * i + lane;
+        v[i] = from[at];
+#pragma unroll
+        for (int k = 1; k < CLUSTER; ++k) v[i] += from[k * E + at];
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += PER) {
+        float top = fabsf(v[i]);
+#pragma unroll
+        for (int j = 1; j < PER; ++j) top = fmaxf(top, fabsf(v[i + j]));
+        const Power pw = row_power(lanes_max<(S::R < 32 ? S::R : 32)>(top));
+        const int row = (warp * 2 * S::R + 32 * i + lane) / S::R;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            hs[row * S::HP + (32 * (i + j) + lane) % S::R] = __float2half_rn(v[i + j] * pw.to);
+        if (lane % (S::R < 32 ? S::R : 32) == 0) factor[row] = pw.back * scale;
     }
     __syncthreads();
     for (; nb < nb1; nb += AHEAD * WARPS) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             const int at = nb + i * WARPS, later = at + AHEAD * WARPS;
-            if (at < nb1) c[i].finish(p, hs, S::HP, tile.rank, row_of, at, g, t);
+            if (at < nb1) c[i].finish(p, hs, S::HP, factor, tile.rank, row_of, at, g, t);
             if (later < nb1) c[i].load(p, bw, tile.rank, row_of, later, g, t);
         }
     }
 }
 
-// The first product of 64-row tiles -> h (fp16 [tile][64][R]) in the workspace.
+// The first product of 64-row tiles -> h (fp16 [tile][64][R]) and its rows' factors in the workspace.
 template <int RT>
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lora_shrink_kernel(const Params p) {
     using S = Shape<RT, 4>;
@@ -307,9 +363,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) lo
     shrink<RT, 4>(p, tile.adapter, tile.rank, row_of, red, cr);
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    __half* h_out = p.h + int64_t(at) * S::TM * S::R;
-    gather<RT, 4>(cluster, red, cr, p.scaling ? p.scaling[tile.adapter] : 1.f,
-                  [&](int row, int col, __half2 h) { *reinterpret_cast<__half2*>(h_out + row * S::R + col) = h; });
+    gather<RT>(cluster, red, cr, p.scaling ? p.scaling[tile.adapter] : 1.f, p.h + int64_t(at) * S::TM * S::R,
+               p.factor + int64_t(at) * S::TM);
     cluster.sync();         // the others have read this CTA's sums
 }
 
@@ -322,6 +377,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 3 : 2) lora_expand_kernel(c
     using S = Shape<RT, 4>;
     __shared__ __align__(16) __half hs[S::TM * S::HP];
     __shared__ int row_of[S::TM];
+    __shared__ float factor[S::TM];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     pdl_wait();
     const Tile tile = read_tile(p, blockIdx.y, S::TM, row_of);
@@ -339,9 +395,10 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 3 : 2) lora_expand_kernel(c
     const uint4* h_in = reinterpret_cast<const uint4*>(p.h + int64_t(blockIdx.y) * S::TM * S::R);
     for (int i = threadIdx.x; i < S::TM * S::R / 8; i += THREADS)
         *reinterpret_cast<uint4*>(hs + i / RT * S::HP + i % RT * 8) = h_in[i];
+    if (threadIdx.x < S::TM) factor[threadIdx.x] = p.factor[int64_t(blockIdx.y) * S::TM + threadIdx.x];
     __syncthreads();
     for (; nb < nb1; nb += WARPS / 2) {
-        c.finish(p, hs + (warp & 1) * 32 * S::HP, S::HP, tile.rank, rows, nb, g, t);
+        c.finish(p, hs + (warp & 1) * 32 * S::HP, S::HP, factor + (warp & 1) * 32, tile.rank, rows, nb, g, t);
         if (nb + WARPS / 2 < nb1) c.load(p, bw, tile.rank, rows, nb + WARPS / 2, g, t);
     }
 }
@@ -420,9 +477,10 @@ extern "C" int nova_lora_add(const nova_lora_args* a, void* stream) {
     p.h = static_cast<__half*>(a->workspace);
     const bool wide = a->tile_rows == 64;
     const int64_t r = rank_tile(a->top_rank);
-    if (wide && a->adapters && (!a->workspace || a->workspace_bytes < a->n_tiles * 64 * r * 2))
+    if (wide && a->adapters && (!a->workspace || a->workspace_bytes < workspace_bytes(a->n_tiles, r)))
         return fail(NOVA_ERR_INVALID, "lora add: workspace of %lld bytes, %lld are needed", (long long)a->workspace_bytes,
-                    (long long)(a->n_tiles * 64 * r * 2));
+                    (long long)workspace_bytes(a->n_tiles, r));
+    p.factor = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + h_bytes(a->n_tiles, r));
     if (wide && a->n_tiles > 65535) return fail(NOVA_ERR_UNSUPPORTED, "lora add: %lld tiles", (long long)a->n_tiles);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return r == 16 ? run<2>(p, a->n_tiles, wide, s) : r == 32 ? run<4>(p, a->n_tiles, wide, s)
@@ -432,6 +490,6 @@ extern "C" int nova_lora_add(const nova_lora_args* a, void* stream) {
 extern "C" int nova_lora_workspace_bytes(int64_t n_tiles, int64_t tile_rows, int64_t top_rank, int64_t* bytes) {
     if (!bytes || n_tiles < 0 || top_rank < 0 || top_rank > 128)
         return fail(NOVA_ERR_INVALID, "lora workspace: tiles=%lld, top_rank=%lld", (long long)n_tiles, (long long)top_rank);
-    *bytes = tile_rows == 64 ? n_tiles * 64 * lora::rank_tile(top_rank) * 2 : 0;
+    *bytes = tile_rows == 64 ? lora::workspace_bytes(n_tiles, lora::rank_tile(top_rank)) : 0;
     return NOVA_OK;
 }
