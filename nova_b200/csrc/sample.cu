@@ -223,15 +223,18 @@ __global__ void __launch_bounds__(ST, 1) sample_topk_kernel(const __grid_constan
                     kept += pi;
                 }
                 for (int i = n_keep; i < K; ++i) prob[i] = 0.f;
+                // The first candidate whose running sum passes u.  The sum may round to less than u: then the last one
+                // that has a probability, for one without (a masked token among the top k) is never drawn.
                 float acc = 0.f;
-                int pick = n_keep - 1;
+                int pick = -1, last = n_keep - 1;
                 const float u = p.uniform ? p.uniform[row] : 0.f;
                 for (int i = 0; i < n_keep; ++i) {
                     prob[i] = __fdiv_rn(prob[i], kept);
                     acc += prob[i];
-                    if (u < acc && pick == n_keep - 1) pick = i;
+                    if (u < acc && pick < 0) pick = i;
+                    if (prob[i] > 0.f) last = i;
                 }
-                s_pick = pick;
+                s_pick = pick < 0 ? last : pick;
             }
             __syncwarp();
         }
