@@ -186,7 +186,8 @@ class PagedKVCache:
         cache.release(a)
 
     :meth:`plan` reserves the pages and advances the lengths, so every plan it
-    returns is to be run once, in order.
+    returns is to be run once, in order; :meth:`take_back` undoes one that did
+    not run to its end.
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, num_q_heads: int, num_pages: int, max_requests: int, *,
@@ -246,9 +247,25 @@ class PagedKVCache:
                         tail_out=[2 * r["slot"] + f for r, f in zip(rs, flips)], windows=self.windows,
                         read_from=read_from, device=self.device)
         del self._free[len(self._free) - sum(need):]
+        plan._before = [(i, r, dict(r), p) for i, r, p in zip(requests, rs, pages)]      # what take_back() restores
         for r, k, p, f in zip(rs, kv, pages, flips):
             r["length"], r["pages"], r["flip"] = k, p, f
         return plan
+
+    def take_back(self, plan: PagePlan) -> None:
+        """Undoes :meth:`plan` for a step that did not run to its end: its requests
+        have the lengths and pages of before, and the step can be planned and run
+        again, whatever of it has run (a step leaves the tokens of before as they
+        were).  Only for the latest plan of its requests."""
+        before = getattr(plan, "_before", None)
+        if before is None:
+            raise ValueError("not a plan of this cache, or taken back already")
+        if any(self._requests.get(i) is not r or r["pages"] is not pages for i, r, _, pages in before):
+            raise ValueError("a request of the plan has been planned again or released")
+        for _, r, was, pages in reversed(before):
+            self._free.extend(pages[len(was["pages"]):])
+            r.update(was)
+        plan._before = None
 
     def append(self, layer: int, qkv: torch.Tensor, plan: PagePlan, **kwargs) -> torch.Tensor:
         """:func:`qkv_append` on one layer."""

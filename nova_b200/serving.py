@@ -22,6 +22,7 @@ from __future__ import annotations
 
 from collections import deque
 from dataclasses import dataclass, field
+from itertools import islice
 from typing import Mapping, Sequence
 
 import torch
@@ -31,7 +32,7 @@ from .decoder import DecoderConfig, DecoderWeights, NF4Weight, rope_tables
 from .kernels import build_nf4_lut, fused_rms_norm, gemm_workspace, nf4_gemm, residual_rms_norm
 from .logits import LogitBias, add_generated, add_prompt, adjust_logits, new_history
 from .lora import LoraPlan, lora_add
-from .paged import PagedKVCache
+from .paged import PagedKVCache, PagePlan
 from .quant import nf4_codebook
 from .sampling import sample_topk
 
@@ -168,7 +169,8 @@ class RequestServer:
     def step(self, requests: Sequence[int] | None = None) -> dict[int, int]:
         """One forward pass of ``requests`` (default: all): the next chunk of each
         unfinished prompt, the last token of every other.  Returns the new token
-        of each request whose prompt is complete."""
+        of each request whose prompt is complete.  A step that raises leaves every
+        request as it was before (draws of the sampler excepted)."""
         rids = list(self._requests) if requests is None else list(requests)
         if not rids:
             return {}
@@ -176,8 +178,26 @@ class RequestServer:
         counts = [min(len(r.todo), self.chunk) or 1 for r in rs]
         if any(self.cache.length(i) + n > self.max_len for i, n in zip(rids, counts)):
             raise RuntimeError(f"a request would pass max_len {self.max_len}")
-        plan = self.cache.plan(rids, counts)                 # before any prompt is consumed: it may lack pages
-        fresh = [[r.todo.popleft() for _ in range(n)] if r.todo else None for r, n in zip(rs, counts)]
+        plan = self.cache.plan(rids, counts)
+        try:
+            done, tok, mine, history = self._forward(rs, counts, plan)
+            tokens = tok.tolist()                            # the step has run
+        except BaseException:
+            self.cache.take_back(plan)
+            raise
+        for r, n in zip(rs, counts):
+            for _ in range(n if r.todo else 0):
+                r.todo.popleft()
+        if done:
+            add_generated(history, tok)
+            self.history[mine] = history
+            self.tokens[mine] = tok
+        return {rids[i]: t for i, t in zip(done, tokens)}
+
+    def _forward(self, rs: list[_Request], counts: list[int], plan: PagePlan) -> tuple:
+        """The step's kernels: which of ``rs`` get a token, those tokens, their slots and a copy of their histories.
+        Of the server's state only the cache's memory changes."""
+        fresh = [list(islice(r.todo, n)) if r.todo else None for r, n in zip(rs, counts)]
         cfg, bank = self.cfg, self.adapters
         slots = torch.tensor([r.slot for r in rs], dtype=torch.int64, device=self.device)
         ids = torch.tensor([t for f in fresh for t in (f or [0])], dtype=torch.int64, device=self.device)
@@ -204,9 +224,9 @@ class RequestServer:
             act = self._linear(xn, w.gate_up, _lib.NF4_SILU_MUL, half=True)
             x = self._linear(act, w.down, _lib.NF4_RESIDUAL, residual=x)
 
-        done = [i for i, r in enumerate(rs) if not r.todo]
+        done = [i for i, r in enumerate(rs) if len(r.todo) <= counts[i]]
         if not done:
-            return {}
+            return [], torch.empty(0, dtype=torch.int64), None, None
         last = torch.tensor([starts[i] + counts[i] - 1 for i in done], dtype=torch.int64, device=self.device)
         mine = slots[torch.tensor(done, dtype=torch.int64, device=self.device)]
         self.raw_logits = self._linear(fused_rms_norm(x[last], self.w.final_norm, cfg.rms_norm_eps), self.w.lm_head)
@@ -220,7 +240,4 @@ class RequestServer:
             allowed=self.masks, allowed_row=allowed_row)
         u = torch.rand(len(done), generator=self.gen, device=self.device) if self.temperature > 0 else None
         tok = sample_topk(self.logits, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, uniform=u)
-        add_generated(history, tok)
-        self.history[mine] = history
-        self.tokens[mine] = tok
-        return {rids[i]: t for i, t in zip(done, tok.tolist())}
+        return done, tok, mine, history

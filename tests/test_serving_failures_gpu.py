@@ -1,0 +1,68 @@
+"""GPU: the request server when a step fails on the host or a kernel reports an
+error.  Nothing here makes a GPU fail: exceptions are raised and error words set
+by the test."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_serving_gpu import small_cfg
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def weights(cuda_lib):
+    from nova_b200.decoder import DecoderWeights
+
+    return DecoderWeights.random_init(small_cfg(), seed=6)
+
+
+def server(weights, **kw):
+    from nova_b200.serving import RequestServer
+
+    srv = RequestServer(weights, num_pages=32, max_requests=3, chunk=100, **kw)
+    g = torch.Generator().manual_seed(1)
+    for n, controls in ((250, {"repetition": 1.3}), (63, {"frequency": 0.7, "presence": 0.2}), (1, {"bias": {7: 2.0}})):
+        srv.submit(torch.randint(0, 4096, (n,), generator=g).tolist(), **controls)
+    return srv
+
+
+def state(srv):
+    return ({i: (srv.length(i), list(r.todo)) for i, r in srv._requests.items()}, srv.cache.free_pages(),
+            srv.history.cpu().clone(), srv.tokens.cpu().clone())
+
+
+def same(x, y):
+    return x[:2] == y[:2] and torch.equal(x[2], y[2]) and torch.equal(x[3], y[3])
+
+
+def fail_at(srv, monkeypatch, layer):
+    """Every attention from `layer` on raises, once."""
+    attend = srv.cache.attend
+
+    def broken(li, *a, **kw):
+        if li == layer:
+            monkeypatch.setattr(srv.cache, "attend", attend)
+            raise MemoryError("no memory for this layer")
+        return attend(li, *a, **kw)
+
+    monkeypatch.setattr(srv.cache, "attend", broken)
+
+
+def test_a_step_that_raises_can_be_taken_again(weights, monkeypatch):
+    """Failures in the middle of prompt chunks, of the steps in which pages fill, and of decoding: every request is
+    as it was, and the steps that follow give the bits of a server that never failed."""
+    good, bad = server(weights), server(weights)
+    for i in range(7):
+        before = state(bad)
+        fail_at(bad, monkeypatch, i % 2)
+        with pytest.raises(MemoryError):
+            bad.step()
+        assert same(state(bad), before)
+        want = good.step()
+        assert bad.step() == want
+        if want:
+            assert torch.equal(good.raw_logits, bad.raw_logits) and torch.equal(good.logits, bad.logits)
+    assert same(state(good), state(bad))
