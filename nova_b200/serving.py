@@ -170,7 +170,8 @@ class RequestServer:
         """One forward pass of ``requests`` (default: all): the next chunk of each
         unfinished prompt, the last token of every other.  Returns the new token
         of each request whose prompt is complete.  A step that raises leaves every
-        request as it was before (draws of the sampler excepted)."""
+        request as it was before (draws of the sampler excepted); it raises
+        RuntimeError, too, where a kernel reports that its result is not valid."""
         rids = list(self._requests) if requests is None else list(requests)
         if not rids:
             return {}
@@ -181,7 +182,8 @@ class RequestServer:
         plan = self.cache.plan(rids, counts)
         try:
             done, tok, mine, history = self._forward(rs, counts, plan)
-            tokens = tok.tolist()                            # the step has run
+            tokens = tok.tolist()
+            self._check_errors(plan)
         except BaseException:
             self.cache.take_back(plan)
             raise
@@ -193,6 +195,16 @@ class RequestServer:
             self.history[mine] = history
             self.tokens[mine] = tok
         return {rids[i]: t for i, t in zip(done, tokens)}
+
+    def _check_errors(self, plan: PagePlan) -> None:
+        """Waits for the step and raises RuntimeError where a bounded wait of its attention or GEMM kernels gave up:
+        its tokens, and what it put into the cache, are not valid then."""
+        plan.check_errors()
+        code = _lib.ctypes.c_int(0)
+        with torch.cuda.device(self.device):
+            _lib.call("nova_nf4_gemm_read_error", self.gemm_ws.data_ptr(), _lib.ctypes.byref(code))
+        if code.value:
+            raise RuntimeError(f"NF4 GEMM: a bounded wait gave up (code {code.value})")
 
     def _forward(self, rs: list[_Request], counts: list[int], plan: PagePlan) -> tuple:
         """The step's kernels: which of ``rs`` get a token, those tokens, their slots and a copy of their histories.

@@ -66,3 +66,27 @@ def test_a_step_that_raises_can_be_taken_again(weights, monkeypatch):
         if want:
             assert torch.equal(good.raw_logits, bad.raw_logits) and torch.equal(good.logits, bad.logits)
     assert same(state(good), state(bad))
+
+
+@pytest.mark.parametrize("kernel", ["attention", "gemm"])
+def test_error_words_are_read(weights, monkeypatch, kernel):
+    """What a bounded wait that gives up leaves in a workspace stops the step, prompt chunks without a token included."""
+    good, bad = server(weights), server(weights)
+    attend = bad.cache.attend
+    for i in range(4):
+        before = state(bad)
+        requests = list(bad._requests)[:1] if i == 0 else None      # first a chunk of the longest prompt alone
+
+        def reports(li, q, plan, **kw):
+            out = attend(li, q, plan, **kw)
+            if li == 1:
+                (plan.workspace[:4] if kernel == "attention" else bad.gemm_ws[4:8]).view(torch.int32).fill_(2)
+            return out
+
+        monkeypatch.setattr(bad.cache, "attend", reports)
+        with pytest.raises(RuntimeError, match="bounded wait"):
+            bad.step(requests)
+        monkeypatch.setattr(bad.cache, "attend", attend)
+        assert same(state(bad), before)
+        assert bad.step(requests) == good.step(requests)
+    assert same(state(good), state(bad))
