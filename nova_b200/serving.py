@@ -171,7 +171,9 @@ class RequestServer:
         unfinished prompt, the last token of every other.  Returns the new token
         of each request whose prompt is complete.  A step that raises leaves every
         request as it was before (draws of the sampler excepted); it raises
-        RuntimeError, too, where a kernel reports that its result is not valid."""
+        RuntimeError, too, where a kernel reports that its result is not valid and
+        where a request's mask and biases leave no token (give it another mask, or
+        step without it)."""
         rids = list(self._requests) if requests is None else list(requests)
         if not rids:
             return {}
@@ -182,8 +184,11 @@ class RequestServer:
         plan = self.cache.plan(rids, counts)
         try:
             done, tok, mine, history = self._forward(rs, counts, plan)
-            tokens = tok.tolist()
+            tokens, ruled_out = tok.tolist()
             self._check_errors(plan)
+            if any(ruled_out):
+                which = [rids[i] for i, out in zip(done, ruled_out) if out]
+                raise RuntimeError(f"no token is left for requests {which}: their masks and biases rule out all")
         except BaseException:
             self.cache.take_back(plan)
             raise
@@ -191,9 +196,9 @@ class RequestServer:
             for _ in range(n if r.todo else 0):
                 r.todo.popleft()
         if done:
-            add_generated(history, tok)
+            add_generated(history, tok[0])
             self.history[mine] = history
-            self.tokens[mine] = tok
+            self.tokens[mine] = tok[0]
         return {rids[i]: t for i, t in zip(done, tokens)}
 
     def _check_errors(self, plan: PagePlan) -> None:
@@ -207,8 +212,9 @@ class RequestServer:
             raise RuntimeError(f"NF4 GEMM: a bounded wait gave up (code {code.value})")
 
     def _forward(self, rs: list[_Request], counts: list[int], plan: PagePlan) -> tuple:
-        """The step's kernels: which of ``rs`` get a token, those tokens, their slots and a copy of their histories.
-        Of the server's state only the cache's memory changes."""
+        """The step's kernels: which of ``rs`` get a token; those tokens, and whether each one is ruled out (logit
+        -inf, so every other is too); their slots; a copy of their histories.  Of the server's state only the cache's
+        memory changes."""
         fresh = [list(islice(r.todo, n)) if r.todo else None for r, n in zip(rs, counts)]
         cfg, bank = self.cfg, self.adapters
         slots = torch.tensor([r.slot for r in rs], dtype=torch.int64, device=self.device)
@@ -238,7 +244,7 @@ class RequestServer:
 
         done = [i for i, r in enumerate(rs) if len(r.todo) <= counts[i]]
         if not done:
-            return [], torch.empty(0, dtype=torch.int64), None, None
+            return [], torch.empty(2, 0, dtype=torch.int64), None, None
         last = torch.tensor([starts[i] + counts[i] - 1 for i in done], dtype=torch.int64, device=self.device)
         mine = slots[torch.tensor(done, dtype=torch.int64, device=self.device)]
         self.raw_logits = self._linear(fused_rms_norm(x[last], self.w.final_norm, cfg.rms_norm_eps), self.w.lm_head)
@@ -252,4 +258,5 @@ class RequestServer:
             allowed=self.masks, allowed_row=allowed_row)
         u = torch.rand(len(done), generator=self.gen, device=self.device) if self.temperature > 0 else None
         tok = sample_topk(self.logits, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, uniform=u)
-        return done, tok, mine, history
+        ruled_out = self.logits.gather(1, tok[:, None])[:, 0] == -float("inf")
+        return done, torch.stack([tok, ruled_out.to(torch.int64)]), mine, history

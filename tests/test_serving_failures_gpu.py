@@ -90,3 +90,30 @@ def test_error_words_are_read(weights, monkeypatch, kernel):
         assert same(state(bad), before)
         assert bad.step(requests) == good.step(requests)
     assert same(state(good), state(bad))
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_a_mask_that_leaves_nothing_gives_no_token(weights, temperature):
+    """An empty mask, a mask of which a bias takes the last token: no forbidden token comes out, nobody loses one, and
+    the others go on once the request has another mask or is left out."""
+    cfg = small_cfg()
+    srv = server(weights, temperature=temperature)
+    words = -(-cfg.vocab_size // 32)
+    a, b, c = srv._requests
+    srv.step()
+    srv.step()
+    empty, one = (torch.zeros(words, dtype=torch.int32, device="cuda") for _ in range(2))
+    one[3] = 1 << 5                                           # token 101 alone
+    srv.set_allowed(b, empty)
+    before = state(srv)
+    with pytest.raises(RuntimeError, match=rf"no token is left for requests \[{b}\]"):
+        srv.step()
+    assert same(state(srv), before)
+    assert set(srv.step([a, c])) == {a, c}
+    srv.set_allowed(b, one)
+    assert srv.step()[b] == 101
+    srv.biases[srv._requests[b].slot] = {101: -float("inf")}
+    before = state(srv)
+    with pytest.raises(RuntimeError, match="no token is left"):
+        srv.step([b])
+    assert same(state(srv), before)
