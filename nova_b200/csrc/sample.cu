@@ -202,7 +202,8 @@ __global__ void __launch_bounds__(ST, 1) sample_topk_kernel(const __grid_constan
             const float x0 = __fdiv_rn(key_value(uint32_t(cand[0] >> 32)), T);
             float s = 0.f;
             for (int i = tid; i < K; i += 32) {
-                const float ei = expf(__fdiv_rn(key_value(uint32_t(cand[i] >> 32)), T) - x0);
+                const float x = __fdiv_rn(key_value(uint32_t(cand[i] >> 32)), T);
+                const float ei = x == x0 ? 1.f : expf(x - x0);   // also where both are infinite (a large bias): no NaN
                 prob[i] = ei;
                 s += ei;
             }
