@@ -32,7 +32,7 @@ from .decoder import DecoderConfig, DecoderWeights, NF4Weight, rope_tables
 from .kernels import build_nf4_lut, fused_rms_norm, gemm_workspace, nf4_gemm, residual_rms_norm
 from .logits import LogitBias, add_generated, add_prompt, adjust_logits, new_history
 from .lora import LoraPlan, lora_add
-from .paged import PagedKVCache, PagePlan
+from .paged import PAGE, PagedKVCache, PagePlan
 from .quant import nf4_codebook
 from .sampling import sample_topk
 
@@ -72,6 +72,15 @@ class _Request:
     slot: int
     adapter: int
     todo: deque = field(default_factory=deque)   # prompt tokens that are not in the cache yet
+
+
+class RequestError(RuntimeError):
+    """A step that cannot be taken because of some of its requests: ``requests``
+    are those to change, to release or to leave out of ``step(requests)``."""
+
+    def __init__(self, message: str, requests: Sequence[int]) -> None:
+        super().__init__(message.format(list(requests)))
+        self.requests = list(requests)
 
 
 class RequestServer:
@@ -116,12 +125,16 @@ class RequestServer:
                presence: float = 0.0, bias: Mapping[int, float] | None = None, allowed: torch.Tensor | None = None) -> int:
         """A new request; its number.  ``allowed``: int32 bit mask ``[ceil(vocab /
         32)]`` of the tokens that may follow (:meth:`set_allowed` changes it)."""
-        prompt = [int(t) for t in prompt]
+        prompt, adapter = [int(t) for t in prompt], int(adapter)
+        repetition, frequency, presence = float(repetition), float(frequency), float(presence)
+        bias = {int(t): float(v) for t, v in (bias or {}).items()}
         if not prompt or min(prompt) < 0 or max(prompt) >= self.cfg.vocab_size:
             raise ValueError("the prompt must hold at least one token, all within the vocabulary")
+        if len(prompt) > self.max_len:
+            raise ValueError(f"a prompt of {len(prompt)} tokens is longer than max_len {self.max_len}")
         if adapter >= (len(self.adapters.ranks) if self.adapters else 0):
             raise ValueError(f"no adapter {adapter}")
-        if repetition <= 0:
+        if not repetition > 0:
             raise ValueError("repetition must be positive")
         if bias and (min(bias) < 0 or max(bias) >= self.cfg.vocab_size):
             raise ValueError("bias tokens must lie within the vocabulary")
@@ -129,19 +142,19 @@ class RequestServer:
             self._check_mask(allowed)
         rid = self.cache.add()
         slot = self._free.pop()
-        self._requests[rid] = _Request(rid, slot, int(adapter), deque(prompt))
+        self._requests[rid] = _Request(rid, slot, adapter, deque(prompt))
         self.history[slot].zero_()
         ids = torch.tensor(prompt, dtype=torch.int64, device=self.device)
         add_prompt(self.history[slot:slot + 1], ids, torch.tensor([0, len(prompt)], dtype=torch.int32, device=self.device))
         self.repetition[slot], self.frequency[slot], self.presence[slot] = repetition, frequency, presence
-        self.biases[slot] = dict(bias or {})
+        self.biases[slot] = bias
         self.masked[slot] = allowed is not None
         if allowed is not None:
             self.masks[slot].copy_(allowed)
         return rid
 
     def _check_mask(self, allowed: torch.Tensor) -> None:
-        if allowed.dtype != torch.int32 or allowed.shape != self.masks.shape[1:]:
+        if not torch.is_tensor(allowed) or allowed.dtype != torch.int32 or allowed.shape != self.masks.shape[1:]:
             raise ValueError(f"allowed must be int32 [{self.masks.shape[1]}]")
 
     def set_allowed(self, request: int, allowed: torch.Tensor | None) -> None:
@@ -170,25 +183,31 @@ class RequestServer:
         """One forward pass of ``requests`` (default: all): the next chunk of each
         unfinished prompt, the last token of every other.  Returns the new token
         of each request whose prompt is complete.  A step that raises leaves every
-        request as it was before (draws of the sampler excepted); it raises
-        RuntimeError, too, where a kernel reports that its result is not valid and
-        where a request's mask and biases leave no token (give it another mask, or
-        step without it)."""
+        request as it was before (draws of the sampler excepted).  It raises
+        :class:`RequestError` for requests that would pass ``max_len``, that need
+        more pages than are free, or whose mask and biases leave no token, and
+        RuntimeError where a kernel reports that its result is not valid."""
         rids = list(self._requests) if requests is None else list(requests)
         if not rids:
             return {}
         rs = [self._requests[i] for i in rids]
         counts = [min(len(r.todo), self.chunk) or 1 for r in rs]
-        if any(self.cache.length(i) + n > self.max_len for i, n in zip(rids, counts)):
-            raise RuntimeError(f"a request would pass max_len {self.max_len}")
+        have = [self.cache.length(i) for i in rids]
+        past = [i for i, h, n in zip(rids, have, counts) if h + n > self.max_len]
+        if past:
+            raise RequestError(f"requests {{}} would pass max_len {self.max_len}", past)
+        need = {i: (h + n) // PAGE - h // PAGE for i, h, n in zip(rids, have, counts)}
+        if sum(need.values()) > self.cache.free_pages():
+            raise RequestError(f"requests {{}} need {sum(need.values())} pages, {self.cache.free_pages()} are free",
+                               [i for i in rids if need[i]])
         plan = self.cache.plan(rids, counts)
         try:
             done, tok, mine, history = self._forward(rs, counts, plan)
             tokens, ruled_out = tok.tolist()
             self._check_errors(plan)
             if any(ruled_out):
-                which = [rids[i] for i, out in zip(done, ruled_out) if out]
-                raise RuntimeError(f"no token is left for requests {which}: their masks and biases rule out all")
+                raise RequestError("no token is left for requests {}: their masks and biases rule out all",
+                                   [rids[i] for i, out in zip(done, ruled_out) if out])
         except BaseException:
             self.cache.take_back(plan)
             raise
