@@ -183,12 +183,11 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Params p) 
     // The others follow one by one, read again (an output that is the input still holds them).
     todo = (todo | biased) & keep;
     if (!todo) return;
-    const float inv = div_rn(1.f, rep);   // v * inv is within 2^-23 of v / rep, and no element waits for a division
     for (; todo; todo &= todo - 1) {
         const int i = __ffs(todo) - 1, own = (i / VEC * THREADS + int(threadIdx.x)) * VEC + i % VEC, t = base + own;
         float v = to_float<T>(src[t]);
         const int seen = hist ? hist[t] : 0, times = seen & 0x7FFF;
-        v *= seen == 0 ? 1.f : v > 0.f ? inv : rep;
+        if (seen) v = v > 0.f ? div_rn(v, rep) : v * rep;
         v -= times ? fmaf(freq, float(times), pres) : 0.f;
         if (biased >> i & 1u) v += bias_s[own];
         dst[t] = from_float<T>(v);
