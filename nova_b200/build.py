@@ -75,10 +75,15 @@ def build_binding(force: bool = False) -> Path:
     """``nova_b200/_fast.so``, linked to the CUDA library beside it."""
     src = CSRC / "binding.cpp"
     deps = max(src.stat().st_mtime, (INCLUDE / "nova_b200.h").stat().st_mtime, Path(__file__).stat().st_mtime)
-    if not force and FAST.exists() and FAST.stat().st_mtime >= deps:
-        return FAST
     import torch
 
+    # torch's C++ interface and Python's differ between versions: built for others it may load and then misbehave
+    built_for = f"torch {torch.__version__}, python {sys.version}"
+    OBJ.mkdir(exist_ok=True)
+    stamp = OBJ / "fast.built_for"
+    if (not force and FAST.exists() and FAST.stat().st_mtime >= deps and stamp.exists()
+            and stamp.read_text() == built_for):
+        return FAST
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
     includes = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
@@ -89,6 +94,7 @@ def build_binding(force: bool = False) -> Path:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+    stamp.write_text(built_for)
     return FAST
 
 
