@@ -751,11 +751,13 @@ NOVA_API int nova_lora_add(const nova_lora_args* args, void* stream);
  * allowed: uint32 [n_masks, mask_stride words], bit t % 32 of word t / 32;
  * allowed_row: int32 [rows], the mask of a row, negative: none (NULL: row i
  * uses mask i); a number past n_masks masks the whole row.  Biases are lists
- * by (row, 2048-token chunk): entries [bias_off[row * chunks + c], bias_off[row
- * * chunks + c + 1]) with chunks = ceil(vocab / 2048), token numbers of that
+ * by (row, chunk of NOVA_LOGITS_CHUNK tokens): entries [bias_off[row * chunks + c], bias_off[row
+ * * chunks + c + 1]) with chunks = ceil(vocab / NOVA_LOGITS_CHUNK), token numbers of that
  * chunk in any order, none twice.  The repetition rule is the reference's
  * (src/chat.py:58-61); the others have no counterpart there.
  */
+#define NOVA_LOGITS_CHUNK 2048
+
 typedef struct nova_logits_args {
     const void* logits;
     int64_t logits_stride, logits_fp32;

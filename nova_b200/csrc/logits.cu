@@ -23,6 +23,7 @@ constexpr int THREADS = 128;
 constexpr int VEC = 8;                  // tokens per vector
 constexpr int NV = 2;                   // vectors per thread: what a row costs besides its tokens is half as much
 constexpr int CHUNK = THREADS * VEC * NV;   // tokens per CTA, and per bias list
+static_assert(CHUNK == NOVA_LOGITS_CHUNK, "callers build the bias lists by this number");
 
 struct Params {
     const uint8_t* logits;

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 
-CHUNK = 2048     # tokens per bias list (one CTA's tokens)
+CHUNK = 2048     # tokens per bias list: NOVA_LOGITS_CHUNK of include/nova_b200.h
 
 
 class LogitBias:
