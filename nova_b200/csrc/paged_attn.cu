@@ -401,12 +401,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
     const int d0 = lane * 4;
     auto finish = [&](int r, float M, float L, float4 o) {   // one row, a warp: out and lse
         const int row = it.row0 + r, tok = row / p.gq, qh = head * p.gq + row - tok * p.gq;
-        const float inv = L > 0.f ? 1.0f / L : 0.f;
+        const float inv = L == 0.f ? 0.f : 1.0f / L;
         const uint2 h = make_uint2(pack_f16x2(o.x * inv, o.y * inv), pack_f16x2(o.z * inv, o.w * inv));
         *reinterpret_cast<uint2*>(p.out + int64_t(it.q_start + tok) * p.o_t + int64_t(qh) * p.o_h + d0) = h;
         if (p.lse && lane == 0)
             p.lse[int64_t(it.q_start + tok) * p.q_heads + qh] =
-                L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+                L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     };
     const int64_t slot = (int64_t(it.part0) * p.kv_heads + head * int64_t(it.n_splits));
     float* part = p.part + (slot + it.split) * p.tile_rows * PART;   // [part0 ..][head][split][row][PART]

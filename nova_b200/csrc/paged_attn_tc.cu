@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
             if (!(ok = wait(&o_full[half], oc & 1u))) break;
             ++oc;
             tc_fence_after();
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
             __half* dst = p.out + int64_t(it.q_start + tok) * p.o_t + int64_t(head) * p.o_h;
             float4* prow = reinterpret_cast<float4*>(p.part) + int64_t(it.part) * 32 * 256 + r;
 #pragma unroll
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_tile_kernel(const __gri
                     p.part_ml[int64_t(it.part) * 256 + r] = make_float2(m, l);
                 else if (p.lse)
                     p.lse[int64_t(it.q_start + tok) * p.q_heads + head] =
-                        l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                        l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
             }
             tc_fence_before();         // the next segment's first product overwrites O after this half's next p_ready
         }
@@ -537,12 +537,12 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const Params p, co
     }
     const Seq s = p.seqs[it.seq];
     const int row = it.row0 + r, tok = row / p.gq, head = it.head * p.gq + row - tok * p.gq;
-    const float inv = L > 0.f ? 1.0f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
     for (int j = 0; j < C; ++j)
         *reinterpret_cast<uint2*>(p.out + int64_t(s.q_start + tok) * p.o_t + int64_t(head) * p.o_h + 4 * (c + j)) =
             make_uint2(pack_f16x2(o[j].x * inv, o[j].y * inv), pack_f16x2(o[j].z * inv, o[j].w * inv));
     if (p.lse && c == 0)
-        p.lse[int64_t(s.q_start + tok) * p.q_heads + head] = L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+        p.lse[int64_t(s.q_start + tok) * p.q_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace tc
