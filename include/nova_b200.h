@@ -676,7 +676,8 @@ NOVA_API int nova_paged_read(const void* codes, const void* scales, const void* 
  * Attention of the step's new tokens over the paged cache (after the append):
  * the query at position p of a request sees its keys j <= p, and j > p -
  * window where window > 0.  q fp16 [tokens, q_heads, 128], out fp16 [tokens,
- * q_heads, 128] (element strides; the last dimension contiguous), lse
+ * q_heads, 128] (element strides; the last dimension contiguous; out's rows
+ * must not overlap, and out may be q), lse
  * (optional) fp32 [tokens, q_heads] contiguous.  sched: which of the plan's
  * windows.  q_heads a multiple of kv_heads.
  */

@@ -507,6 +507,12 @@ extern "C" int nova_paged_attention(const nova_paged_attn_args* a, const nova_pa
     if (off(a->q, 16) || off(a->out, 16) || off(a->lse, 4) || off(a->workspace, 16) || a->q_t_stride % 8 ||
         a->q_h_stride % 8 || a->o_t_stride % 8 || a->o_h_stride % 8)
         return fail(NOVA_ERR_ALIGN, "paged attention: pointers need 16-byte alignment, strides multiples of 8");
+    // out: one place for each row, or rows of different CTAs would write over one another
+    const int64_t t = a->o_t_stride, h = a->o_h_stride;
+    const bool many_t = info->tokens > 1, many_h = info->q_heads > 1;
+    if ((many_t && t < D) || (many_h && h < D) ||
+        (many_t && many_h && (t < h ? h < t * (info->tokens - 1) + D : t < h * (info->q_heads - 1) + D)))
+        return fail(NOVA_ERR_INVALID, "paged attention: rows of out overlap (strides %lld and %lld)", (long long)t, (long long)h);
     if (a->workspace_bytes < info->workspace_bytes || !a->workspace)
         return fail(NOVA_ERR_INVALID, "paged attention: workspace of %lld bytes, %lld are needed",
                     (long long)a->workspace_bytes, (long long)info->workspace_bytes);
