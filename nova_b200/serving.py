@@ -202,9 +202,11 @@ class RequestServer:
                                [i for i in rids if need[i]])
         plan = self.cache.plan(rids, counts)
         try:
-            done, tok, mine, history = self._forward(rs, counts, plan)
-            tokens, ruled_out = tok.tolist()
-            self._check_errors(plan)
+            done, tok, mine, history, report = self._forward(rs, counts, plan)
+            report = report.tolist()                         # the step has run
+            words, tokens, ruled_out = report[:2], report[2:2 + len(done)], report[2 + len(done):]
+            if any(words):
+                self._raise_errors(plan)
             if any(ruled_out):
                 raise RequestError("no token is left for requests {}: their masks and biases rule out all",
                                    [rids[i] for i, out in zip(done, ruled_out) if out])
@@ -215,25 +217,24 @@ class RequestServer:
             for _ in range(n if r.todo else 0):
                 r.todo.popleft()
         if done:
-            add_generated(history, tok[0])
             self.history[mine] = history
-            self.tokens[mine] = tok[0]
+            self.tokens[mine] = tok
         return {rids[i]: t for i, t in zip(done, tokens)}
 
-    def _check_errors(self, plan: PagePlan) -> None:
-        """Waits for the step and raises RuntimeError where a bounded wait of its attention or GEMM kernels gave up:
-        its tokens, and what it put into the cache, are not valid then."""
-        plan.check_errors()
+    def _raise_errors(self, plan: PagePlan) -> None:
+        """Raises RuntimeError, and clears the error words, where a bounded wait of the step's attention or GEMM
+        kernels gave up: its tokens, and what it put into the cache, are not valid then."""
         code = _lib.ctypes.c_int(0)
-        with torch.cuda.device(self.device):
+        with torch.cuda.device(self.device):                 # the server's workspace first: it outlives the plan's
             _lib.call("nova_nf4_gemm_read_error", self.gemm_ws.data_ptr(), _lib.ctypes.byref(code))
+        plan.check_errors()
         if code.value:
             raise RuntimeError(f"NF4 GEMM: a bounded wait gave up (code {code.value})")
 
     def _forward(self, rs: list[_Request], counts: list[int], plan: PagePlan) -> tuple:
-        """The step's kernels: which of ``rs`` get a token; those tokens, and whether each one is ruled out (logit
-        -inf, so every other is too); their slots; a copy of their histories.  Of the server's state only the cache's
-        memory changes."""
+        """The step's kernels: which of ``rs`` get a token, those tokens, their slots, their histories with the tokens,
+        and one tensor for the host: the error words of attention and GEMM, the tokens, and whether each one is ruled
+        out (logit -inf, so every other is too).  Of the server's state only the cache's memory changes."""
         fresh = [list(islice(r.todo, n)) if r.todo else None for r, n in zip(rs, counts)]
         cfg, bank = self.cfg, self.adapters
         slots = torch.tensor([r.slot for r in rs], dtype=torch.int64, device=self.device)
@@ -261,9 +262,10 @@ class RequestServer:
             act = self._linear(xn, w.gate_up, _lib.NF4_SILU_MUL, half=True)
             x = self._linear(act, w.down, _lib.NF4_RESIDUAL, residual=x)
 
+        words = (plan.workspace[:4].view(torch.int32), self.gemm_ws[4:8].view(torch.int32))
         done = [i for i, r in enumerate(rs) if len(r.todo) <= counts[i]]
         if not done:
-            return [], torch.empty(2, 0, dtype=torch.int64), None, None
+            return [], None, None, None, torch.cat(words)
         last = torch.tensor([starts[i] + counts[i] - 1 for i in done], dtype=torch.int64, device=self.device)
         mine = slots[torch.tensor(done, dtype=torch.int64, device=self.device)]
         self.raw_logits = self._linear(fused_rms_norm(x[last], self.w.final_norm, cfg.rms_norm_eps), self.w.lm_head)
@@ -278,4 +280,6 @@ class RequestServer:
         u = torch.rand(len(done), generator=self.gen, device=self.device) if self.temperature > 0 else None
         tok = sample_topk(self.logits, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, uniform=u)
         ruled_out = self.logits.gather(1, tok[:, None])[:, 0] == -float("inf")
-        return done, torch.stack([tok, ruled_out.to(torch.int64)]), mine, history
+        report = torch.cat((*words, tok, ruled_out))
+        add_generated(history, tok)
+        return done, tok, mine, history, report

@@ -117,3 +117,18 @@ def test_a_mask_that_leaves_nothing_gives_no_token(weights, temperature):
     with pytest.raises(RuntimeError, match="no token is left"):
         srv.step([b])
     assert same(state(srv), before)
+
+
+def test_both_error_words_are_cleared(weights):
+    good, bad = server(weights), server(weights)
+    bad.gemm_ws[4:8].view(torch.int32).fill_(3)
+    plan = bad.cache.plan
+    bad.cache.plan = lambda *a, **kw: (bad.cache.__dict__.pop("plan"), set_word(plan(*a, **kw)))[1]
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        bad.step()
+    assert bad.step() == good.step() and same(state(good), state(bad))
+
+
+def set_word(plan):
+    plan.workspace[:4].view(torch.int32).fill_(2)
+    return plan
