@@ -100,8 +100,8 @@ __device__ __forceinline__ Row8 norm_rope_row(const Row8& in, bool norm, const f
     return pack(x);
 }
 
-// Code of a value: rint((v - low) / step) of the framework's quantizer, bit for
-// bit.  The quotient by the reciprocal is within 4e-5 of the divided one (it is
+// Code of a finite value: rint((v - low) / step) of the framework's quantizer, bit
+// for bit.  The quotient by the reciprocal is within 4e-5 of the divided one (it is
 // at most 255), so only one that close to a tie is divided; adding 1.5 * 2^23
 // rounds to the nearest even integer and leaves it in the low mantissa bits.
 __device__ __forceinline__ uint32_t code_of(float v, float low, float step, float inv) {
@@ -112,12 +112,14 @@ __device__ __forceinline__ uint32_t code_of(float v, float low, float step, floa
     return __float_as_uint(t) & 0xFFu;
 }
 
+// A NaN among a channel's tokens is its minimum and maximum: the page's scale says
+// so, and no code stands for a number that was none.
 __device__ __forceinline__ uint32_t hmin2u(uint32_t a, uint32_t b) {
-    __half2 r = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    __half2 r = __hmin2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
-    __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&r);
 }
 
