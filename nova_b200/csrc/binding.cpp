@@ -1,7 +1,7 @@
 // Python binding of the serving operators (nova_b200._fast): argument checks,
-// output allocation and the C call in one function each.  The same through
-// ctypes takes 7 to 9 us a call in the interpreter, longer than the kernels of
-// a small step run; here it is 3 to 4, of which the launch is most.
+// output allocation and the C call in one function each.  Through ctypes a call
+// takes about 10 us of host time, longer than the kernels of a small step run;
+// here it is 4 to 7, of which the launch is most.
 //
 // Every function raises ValueError for arguments that do not fit, before
 // anything is launched, and works on its tensors' device, whichever is current:

@@ -7,10 +7,10 @@
 // mask applied to its words, and those tokens are then done one by one in fp32
 // with one rounding (all tokens through fp32: 44 instructions each and 20.1 us
 // for 64 rows of 151936 fp16 logits; this way 18.4; 16.4 since the biases are on
-// their way while the vectors are written; fewer registers a thread for more CTAs
-// per SM are slower).  Bound by instruction issue and the latency of a few waves
-// of CTAs, then HBM: 58.8 MB at 3.6 TB/s; one row is a launch and two
-// dependent loads, 4.9 us.  Vectors start at the 16-byte boundary at or before
+// their way while the vectors are written, 16.6 since the penalty divides; fewer
+// registers a thread for more CTAs per SM are slower).  Bound by instruction issue and the latency of a few waves
+// of CTAs, then HBM: 58.8 MB at 3.5 TB/s; one row is a launch and two
+// dependent loads, 5.1 us.  Vectors start at the 16-byte boundary at or before
 // the row (the row's first and last vector go token by token); a row whose
 // logits, history and output do not share such a boundary goes token by token
 // throughout.

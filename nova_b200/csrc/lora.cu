@@ -14,10 +14,12 @@
 //   * few rows (16-row tiles): one launch; each CTA goes on with an eighth of N;
 //   * many (64-row tiles): h goes through memory and a second launch takes the
 //     columns.  As one launch a cluster held its 8 CTAs for the whole of N, and
-//     37 of them did not fit the GPU at once: 93 us against 68 for 1.7k rows of
-//     19456 columns at rank 64 (14 us for the first product, 53 for the second:
-//     149 MB of DRAM traffic, 23 us of it, and 20 us of mma.sync).
-// 64 rows with 24 adapters of rank up to 16, 2560 -> 6144: 6.5 us in one launch.
+//     37 of them did not fit the GPU at once: 93 us against 69 for 2217 rows (1750
+//     of them with an adapter) of 19456 columns at rank 64.  It is 71.5 since h's
+//     rows have powers of their own (16 us for the first product, 54 for the second:
+//     144 MB of DRAM traffic, 22 us of it, and 20 us of mma.sync).
+// 64 rows with 24 adapters of rank up to 16, 2560 -> 6144: one launch, 8.2 us a
+// call, 9.7 of kernel with cold caches.
 // Fragments of mma.sync m16n8k16 are read straight from global memory: the
 // contraction index is permuted so that a lane's operand registers are 16
 // consecutive bytes (8 of B and h at rank 16), and the columns of four neighbouring tiles are
@@ -168,7 +170,8 @@ struct Columns {
     uint2 w[4][S];
 
     // The lane's first of the four entries along the rank that it holds in step s: two steps' are neighbours, so that
-    // they come in one load of 16 bytes (1.7k rows of 19456 columns at rank 64: 70.2 us with loads of 8, 68.4 with 16).
+    // they come in one load of 16 bytes (2217 rows of 19456 columns at rank 64, h then unscaled: 70.2 us with loads of
+    // 8, 68.4 with 16).
     static __device__ __forceinline__ int entry(int s, int t) { return S == 1 ? 4 * t : 32 * (s / 2) + 8 * t + 4 * (s % 2); }
     // Those entries of every step, `n` of them to be read at `p`.
     static __device__ __forceinline__ void entries(const __half* p, int n, int t, uint2 (&v)[S]) {

@@ -49,8 +49,8 @@ class LoraPlan:
         rows = np.argsort(of_row, kind="stable")
         values, first, n = np.unique(of_row[rows], return_index=True, return_counts=True)
         busy = n[values >= 0]
-        # 16-row tiles are one launch, 8 CTAs each; once they no longer fit the GPU at once (two CTAs per SM), 64-row
-        # tiles in two launches are faster if they are fewer: 300 rows of one adapter 14 us against 22, 700 rows 22.5
+        # 16-row tiles are one launch, 8 CTAs each; once they no longer fit the GPU at once (two CTAs on each of 148 SMs
+        # are 37 tiles: about 40), 64-row tiles in two launches are faster if they are fewer: 300 rows of one adapter 14 us against 22, 700 rows 22.5
         # and 21, 2800 rows 56 and 38; one row of each of 64 adapters 21 us against 29
         small, large = (-(-busy // 16)).sum(), (-(-busy // 64)).sum()
         self.tile_rows = 64 if small > 40 and 2 * large <= small else 16
@@ -90,12 +90,14 @@ class LoraPlan:
 
 def lora_add(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan, *,
              scaling: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """``base + scaling[a] * (x A_a^T) B_a^T`` for every row's adapter ``a``, one launch.
+    """``base + scaling[a] * (x A_a^T) B_a^T`` for every row's adapter ``a``: one
+    launch, or two where the plan has 64-row tiles.
 
     ``x`` fp16 ``[tokens, K]``; ``base`` fp16 ``[tokens, N]`` (the shared
     projection's output); ``a`` fp16 ``[adapters, R, K]``; ``b`` fp16 ``[adapters,
     N, R]``, R a multiple of 8 up to 128 and at least every rank (entries past an
     adapter's rank are not read); ``scaling`` fp32 ``[adapters]``.  ``out`` may be
     ``base``; rows without an adapter are then left alone.  Returns fp16
-    ``[tokens, N]``."""
+    ``[tokens, N]``.  Between the products a row of ``x A_a^T`` is fp16 at a power
+    of two of its own, so any size of ``x``, ``a`` and ``scaling`` keeps its 11 bits."""
     return _lib.fast().lora_add(x, base, a, b, plan, scaling, out)

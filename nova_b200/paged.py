@@ -6,7 +6,8 @@ none).  The storage of a layer is three tensors:
 
 * ``codes``  uint8 ``[num_pages, H_kv, 2, 64, 128]`` (K, V): a page is one
   64-token group of the int8t64 format (``nova_b200.kvquant``), the same codes
-  and scales that ``quantize_int8(..., 64, "token")`` gives;
+  and scales that ``quantize_int8(..., 64, "token")`` gives for finite values
+  (one that is not leaves no finite value in its channel of the page);
 * ``scales`` fp16 ``[num_pages, H_kv, 4, 128]``: K min, K step, V min, V step;
 * ``tails``  fp16 ``[num_tails, H_kv, 2, 64, 128]``: the tokens of pages that
   are not full yet (position p at slot p % 64).
@@ -168,8 +169,14 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     dimension contiguous).  The query at position p of a request sees its keys
     ``j <= p`` (``window`` > 0, one of the plan's: also ``j > p - window``).
     ``scale``: of the scores (default ``128 ** -0.5``).  ``lse_out``: fp32
-    ``[tokens, H_q]``, log-sum-exp of the scaled scores.  Returns fp16
-    ``[tokens, H_q, 128]``."""
+    ``[tokens, H_q]``, log-sum-exp of the scaled scores.  ``out`` may be ``q``.
+    Returns fp16 ``[tokens, H_q, 128]``.
+
+    Scores and sums are fp32; weights are fp16 in the second product (with their
+    low parts for requests of up to 4 query rows per KV head), so an output is
+    within 2^-11 of the sum of its weighted values.  Cached values have to be
+    finite: an infinity or NaN in V reaches every query whose work takes in its
+    64-token block, with a weight of zero too."""
     return _lib.fast().paged_attention(q, codes, scales, tails, plan, window, scale, out, lse_out)
 
 
